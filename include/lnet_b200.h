@@ -438,6 +438,77 @@ const char *lnet_b200_last_error(void);
 /* Library version string. */
 const char *lnet_b200_version(void);
 
+/* ---------------------------------------------------------------- feed-forward operators
+ * No reference counterpart: what a block of channel mixing around the temporal
+ * mixing, its training and its 8-bit serving need.  Rows are the tokens of every
+ * leading dimension; tensors are contiguous and row-major, offsets are 64 bits.
+ *
+ * Residual addition and RMSNorm over the last dimension:
+ *   h = round(x + residual) in `dtype` (stream_out; without a residual h = x and
+ *   stream_out is not written), rstd = (mean(h^2) + eps)^-1/2, y = h rstd weight.
+ * `dtype` (x, residual, y, stream) is LNET_F32 or LNET_BF16, `weight_dtype` too.
+ * rstd [rows] may be NULL; the gradient needs it.  Outputs must not overlap inputs. */
+int lnet_b200_residual_rms_norm(const void *x, const void *residual, const void *weight,
+                                int32_t dtype, int32_t weight_dtype, int64_t rows, int64_t dim,
+                                float eps, void *y, void *stream_out, float *rstd,
+                                lnet_stream_t stream);
+
+/* The same norm with an 8-bit output: scales[row] = max|y| / 448 (fp32) and
+ * values = e4m3(y / scale), rounded to nearest even; a zero row has scale 0 and values 0. */
+int lnet_b200_residual_rms_norm_fp8(const void *x, const void *residual, const void *weight,
+                                    int32_t dtype, int32_t weight_dtype, int64_t rows,
+                                    int64_t dim, float eps, uint8_t *values, float *scales,
+                                    void *stream_out, lnet_stream_t stream);
+
+/* Gradient of lnet_b200_residual_rms_norm from its stream and rstd: dx [rows, dim]
+ * (also the residual's gradient) and dweight [dim] in `weight_dtype` (NULL: not
+ * wanted).  dstream is the gradient of the stream output (NULL: zero).  The column
+ * sums are joined in a fixed order: the same bits every time. */
+int lnet_b200_residual_rms_norm_workspace_size(int32_t dtype, int64_t rows, int64_t dim,
+                                               size_t *bytes);
+int lnet_b200_residual_rms_norm_backward(const void *stream_in, const float *rstd,
+                                         const void *weight, const void *dy, const void *dstream,
+                                         int32_t dtype, int32_t weight_dtype, int64_t rows,
+                                         int64_t dim, void *dx, void *dweight, void *workspace,
+                                         size_t workspace_bytes, lnet_stream_t stream);
+
+/* Distillation from a teacher's top logits, mixed with hard labels.  Row i has the
+ * entries j with teacher_indices[i, j] >= 0 and teacher_logits[i, j] > -inf:
+ *   p = softmax(teacher_logits / temperature) over them, q = softmax(logits / temperature),
+ *   loss_i = alpha temperature^2 sum_j p_j (log p_j - log q_j)            [rows with entries]
+ *          + (1 - alpha) (logsumexp(logits_i) - logits[i, labels_i])      [labels_i >= 0].
+ * labels may be NULL.  A part of weight 0 is left out.  reduction: 0 the rows'
+ * losses [rows], 1 their sum, 2 their mean over the rows that have an entry or a
+ * label (0 without any).  An index or a label past `classes` makes its row's loss
+ * and gradient NaN. */
+typedef struct lnet_b200_distill_request {
+  int64_t rows;
+  int64_t classes;
+  int64_t top;
+  int32_t dtype; /* of logits and dlogits: LNET_F32 or LNET_BF16 */
+  int32_t reduction;
+  const void *logits;              /* [rows, classes] */
+  const int64_t *teacher_indices;  /* [rows, top] */
+  const float *teacher_logits;     /* [rows, top] */
+  const int64_t *labels;           /* [rows] or NULL */
+  float temperature;
+  float alpha;
+} lnet_b200_distill_request;
+
+int lnet_b200_distill_workspace_size(const lnet_b200_distill_request *req, size_t *bytes);
+/* loss (fp32: [rows] or one value) and, where dlogits is not NULL, the gradient of
+ * the reduced loss (of the rows' sum where reduction is 0) in the same call. */
+int lnet_b200_distill_forward(const lnet_b200_distill_request *req, void *workspace,
+                              size_t workspace_bytes, float *loss, void *dlogits,
+                              lnet_stream_t stream);
+/* The gradient for the loss's gradient dloss (device, fp32: [rows] or one value). */
+int lnet_b200_distill_backward(const lnet_b200_distill_request *req, void *workspace,
+                               size_t workspace_bytes, const float *dloss, void *dlogits,
+                               lnet_stream_t stream);
+/* dlogits *= scale[0] in place (device, fp32); leaves it alone where the scale is 1. */
+int lnet_b200_distill_scale(void *dlogits, int32_t dtype, int64_t count, const float *scale,
+                            lnet_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

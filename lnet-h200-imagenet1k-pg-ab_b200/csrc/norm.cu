@@ -1,0 +1,559 @@
+// Residual addition + RMSNorm, its gradient, and its 8-bit output.
+//
+//   h = round(x + r)              the stream, in the inputs' type
+//   rstd = (mean(h^2) + eps)^-1/2 fp32, over the stream as it is stored
+//   y = h rstd w
+//   8 bits: s = max|y| / 448, q = e4m3(y / s)   (s = 0: q = 0)
+//   gradient: g = dy w, c = mean(g h rstd),
+//     dx = dr = rstd (g - h rstd c) + dh,  dw = sum over rows of dy h rstd
+//
+// Every pass is bound by HBM: a row is read once, held in registers (packed
+// loads of 16 bytes, up to 4 a thread) through both of its reductions, and
+// written once.  A row of up to 128 chunks belongs to 4, 8, 16 or 32 lanes of a
+// warp (the fewest that hold it in 4 chunks each, so that a 96-wide bf16 row
+// uses 4 lanes x 3 chunks and no lane idles); a longer one to a block of up to
+// 512 threads; one that 512 threads cannot hold is read again from L2 (wide
+// kernels).
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "rows.cuh"
+
+namespace lnet {
+namespace {
+
+constexpr float kE4m3Max = 448.f;
+constexpr int kSubThreads = 256;    // block of the kernels that put several rows in a warp
+constexpr int kBlockThreads = 512;  // largest block of the row-per-block kernels
+constexpr int kWideThreads = 1024;
+constexpr int kReduceLanes = 32;
+
+// chunks a thread may hold
+template <int VEC>
+__host__ __device__ constexpr int chunks_of() {
+  return VEC == 1 ? 16 : 4;
+}
+
+__device__ __forceinline__ float weight_at(const void *w, bool w_bf16, int64_t i) {
+  return w_bf16 ? load_f(reinterpret_cast<const __nv_bfloat16 *>(w), i)
+                : __ldg(reinterpret_cast<const float *>(w) + i);
+}
+
+// q = e4m3(y / s), saturating; s = 0 means that the row is zero.
+__device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+template <int VEC>
+__device__ __forceinline__ void store_e4m3(uint8_t *p, const float *v, float s) {
+  const float d = s == 0.f ? 1.f : s;
+  if (VEC == 1) {
+    *p = (uint8_t)(e4m3_pair(v[0] / d, 0.f) & 0xFF);
+  } else {
+    uint32_t w[VEC >= 4 ? VEC / 4 : 1];
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i)
+      w[i] = e4m3_pair(v[4 * i] / d, v[4 * i + 1] / d) |
+             (e4m3_pair(v[4 * i + 2] / d, v[4 * i + 3] / d) << 16);
+    if (VEC == 8)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[VEC == 8 ? 1 : 0]);
+    else
+      *reinterpret_cast<uint32_t *>(p) = w[0];
+  }
+}
+
+struct NormArgs {
+  const void *x, *r, *w;
+  void *y, *h;
+  uint8_t *q;
+  float *scales, *rstd;
+  int64_t rows, dim;
+  float eps;
+  int w_bf16;
+};
+
+template <typename T, int VEC, int G, bool FP8>
+__global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
+norm_forward_kernel(const NormArgs a) {
+  constexpr int NV = chunks_of<VEC>();
+  __shared__ float scratch[33];
+  const int g = G ? G : blockDim.x;
+  const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
+  const int nvec = (int)(a.dim / VEC);
+  const T *x = reinterpret_cast<const T *>(a.x), *r = reinterpret_cast<const T *>(a.r);
+  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
+       base += (int64_t)gridDim.x * per) {
+    const int64_t row = base + sub;
+    const bool live = row < a.rows;
+    const int64_t off = row * a.dim;
+    RowChunk<T, VEC> cx[NV], cr[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      cx[j].zero();
+      if (live && c < nvec) cx[j].load(x + off + (int64_t)c * VEC);
+    }
+    if (r) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = lane + j * g;
+        cr[j].zero();
+        if (live && c < nvec) cr[j].load(r + off + (int64_t)c * VEC);
+      }
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      float v[VEC];
+      cx[j].get(v);
+      if (r) {
+        float u[VEC];
+        cr[j].get(u);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] += u[i];
+        cx[j].put(v);  // the stream, rounded to its type
+        if (live && c < nvec) cx[j].store(reinterpret_cast<T *>(a.h) + off + (int64_t)c * VEC);
+        cx[j].get(v);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) ss = fmaf(v[i], v[i], ss);
+    }
+    ss = group_reduce<G, SumOp>(ss, scratch);
+    const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
+    if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
+    float amax = 0.f, scale = 0.f;
+    if (FP8) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int c = lane + j * g;
+        if (c >= nvec) continue;
+        float v[VEC];
+        cx[j].get(v);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          amax = MaxNanOp::of(
+              amax, fabsf(v[i] * rstd * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i)));
+      }
+      amax = group_reduce<G, MaxNanOp>(amax, scratch);
+      scale = amax / kE4m3Max;
+      if (live && lane == 0) a.scales[row] = scale;
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      if (!live || c >= nvec) continue;
+      float v[VEC];
+      cx[j].get(v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] *= rstd * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i);
+      if (FP8) {
+        store_e4m3<VEC>(a.q + off + (int64_t)c * VEC, v, scale);
+      } else {
+        cx[j].put(v);
+        cx[j].store(reinterpret_cast<T *>(a.y) + off + (int64_t)c * VEC);
+      }
+    }
+  }
+}
+
+// Rows that a block cannot hold: three sweeps, the later ones over the stream (or x) in L2.
+template <typename T, bool FP8>
+__global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const NormArgs a) {
+  __shared__ float scratch[33];
+  const T *x = reinterpret_cast<const T *>(a.x), *r = reinterpret_cast<const T *>(a.r);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t off = row * a.dim;
+    const T *h = r ? reinterpret_cast<const T *>(a.h) : x;
+    float ss = 0.f;
+    for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+      float v = load_f(x, off + c);
+      if (r) {
+        RowChunk<T, 1> k;
+        v += load_f(r, off + c);
+        k.put(&v);
+        k.store(reinterpret_cast<T *>(a.h) + off + c);
+        k.get(&v);
+      }
+      ss = fmaf(v, v, ss);
+    }
+    ss = group_reduce<0, SumOp>(ss, scratch);
+    const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+    float scale = 0.f;
+    if (FP8) {
+      float amax = 0.f;
+      for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x)
+        amax = MaxNanOp::of(amax, fabsf(load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c)));
+      amax = group_reduce<0, MaxNanOp>(amax, scratch);
+      scale = amax / kE4m3Max;
+      if (threadIdx.x == 0) a.scales[row] = scale;
+    }
+    for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+      const float v = load_f(h, off + c) * (rstd * weight_at(a.w, a.w_bf16, c));
+      if (FP8)
+        store_e4m3<1>(a.q + off + c, &v, scale);
+      else
+        store_f(reinterpret_cast<T *>(a.y), off + c, v);
+    }
+  }
+}
+
+struct NormGradArgs {
+  const void *h, *w, *dy, *dh;
+  const float *rstd;
+  void *dx;
+  float *partial;  // [grid, dim] column sums of the blocks, or null
+  int64_t rows, dim;
+  int w_bf16;
+};
+
+template <typename T, int VEC, int G>
+__global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
+norm_backward_kernel(const NormGradArgs a) {
+  constexpr int NV = chunks_of<VEC>();
+  __shared__ float scratch[33];
+  __shared__ float columns[G ? G * NV * VEC : 1];
+  const int g = G ? G : blockDim.x;
+  const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
+  const int nvec = (int)(a.dim / VEC);
+  const T *hp = reinterpret_cast<const T *>(a.h), *dyp = reinterpret_cast<const T *>(a.dy);
+  const T *dhp = reinterpret_cast<const T *>(a.dh);
+  float dw[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
+  for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
+       base += (int64_t)gridDim.x * per) {
+    const int64_t row = base + sub;
+    const bool live = row < a.rows;
+    const int64_t off = row * a.dim;
+    RowChunk<T, VEC> ch[NV], cy[NV], cs[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      ch[j].zero(), cy[j].zero(), cs[j].zero();
+      if (live && c < nvec) {
+        ch[j].load(hp + off + (int64_t)c * VEC);
+        cy[j].load(dyp + off + (int64_t)c * VEC);
+        if (dhp) cs[j].load(dhp + off + (int64_t)c * VEC);
+      }
+    }
+    const float rstd = live ? __ldg(a.rstd + row) : 0.f;
+    float dot = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      if (c >= nvec) continue;
+      float h[VEC], dy[VEC];
+      ch[j].get(h), cy[j].get(dy);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float t = dy[i] * (h[i] * rstd);
+        dw[j][i] += t;
+        dot = fmaf(t, weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i), dot);
+      }
+    }
+    dot = group_reduce<G, SumOp>(dot, scratch);
+    const float k = dot / (float)a.dim * rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      if (!live || c >= nvec) continue;
+      float h[VEC], dy[VEC], s[VEC];
+      ch[j].get(h), cy[j].get(dy), cs[j].get(s);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float gi = dy[i] * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i);
+        s[i] = fmaf(rstd, gi - h[i] * k, s[i]);
+      }
+      cs[j].put(s);
+      cs[j].store(reinterpret_cast<T *>(a.dx) + off + (int64_t)c * VEC);
+    }
+  }
+  if (!a.partial) return;
+  float *out = a.partial + (int64_t)blockIdx.x * a.dim;
+  if (G == 0) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      if (c >= nvec) continue;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[(int64_t)c * VEC + i] = dw[j][i];
+    }
+  } else {  // the warp's rows, then one warp after another: the same order every time
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+#pragma unroll
+        for (int o = 16; o >= (G ? G : 32); o >>= 1)
+          dw[j][i] += __shfl_xor_sync(0xFFFFFFFFu, dw[j][i], o);
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+      if ((int)threadIdx.x / 32 == w && (threadIdx.x & 31) < (unsigned)g) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int c = lane + j * g;
+          if (c >= nvec) continue;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float *p = columns + c * VEC + i;
+            *p = w ? *p + dw[j][i] : dw[j][i];
+          }
+        }
+      }
+      __syncthreads();
+    }
+    for (int c = threadIdx.x; c < (int)a.dim; c += blockDim.x) out[c] = columns[c];
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kWideThreads) norm_backward_wide_kernel(const NormGradArgs a) {
+  __shared__ float scratch[33];
+  const T *hp = reinterpret_cast<const T *>(a.h), *dyp = reinterpret_cast<const T *>(a.dy);
+  const T *dhp = reinterpret_cast<const T *>(a.dh);
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const int64_t off = row * a.dim;
+    const float rstd = __ldg(a.rstd + row);
+    const bool first = row == blockIdx.x;
+    float dot = 0.f;
+    for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+      const float t = load_f(dyp, off + c) * (load_f(hp, off + c) * rstd);
+      dot = fmaf(t, weight_at(a.w, a.w_bf16, c), dot);
+      if (a.partial) {  // a thread's own columns
+        float *p = a.partial + (int64_t)blockIdx.x * a.dim + c;
+        *p = first ? t : *p + t;
+      }
+    }
+    dot = group_reduce<0, SumOp>(dot, scratch);
+    const float k = dot / (float)a.dim * rstd;
+    for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
+      const float gi = load_f(dyp, off + c) * weight_at(a.w, a.w_bf16, c);
+      const float s = dhp ? load_f(dhp, off + c) : 0.f;
+      store_f(reinterpret_cast<T *>(a.dx), off + c,
+              fmaf(rstd, gi - load_f(hp, off + c) * k, s));
+    }
+  }
+}
+
+// dw = column sums of the blocks' partial sums, in block order.
+__global__ void __launch_bounds__(32 * kReduceLanes)
+norm_columns_kernel(const float *__restrict__ partial, int blocks, int64_t dim, void *dw,
+                    int w_bf16) {
+  __shared__ float part[kReduceLanes][33];
+  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < dim) {
+#pragma unroll 4
+    for (int b = threadIdx.y; b < blocks; b += kReduceLanes) s += partial[(int64_t)b * dim + c];
+  }
+  part[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < dim) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kReduceLanes; ++i) s += part[i][threadIdx.x];
+    if (w_bf16)
+      store_f(reinterpret_cast<__nv_bfloat16 *>(dw), c, s);
+    else
+      reinterpret_cast<float *>(dw)[c] = s;
+  }
+}
+
+// Threads, lanes a row and blocks of a call (lanes 0: a block a row; wide: see above).
+struct NormPlan {
+  int lanes, threads, blocks;
+  bool vec, wide;
+};
+
+NormPlan norm_plan(int64_t rows, int64_t dim, int elem, bool aligned, int blocks_per_sm) {
+  NormPlan p{};
+  const int vec = 16 / elem;
+  p.vec = aligned && dim % vec == 0;
+  const int nv = p.vec ? 4 : 16;
+  const int64_t nvec = p.vec ? dim / vec : dim;
+  int64_t per = 1;
+  if (nvec <= (int64_t)32 * nv) {
+    p.lanes = 4;
+    while ((int64_t)p.lanes * nv < nvec) p.lanes *= 2;
+    p.threads = kSubThreads;
+    per = kSubThreads / p.lanes;
+  } else if (nvec <= (int64_t)kBlockThreads * nv) {
+    p.threads = (int)((cdiv(nvec, nv) + 31) / 32 * 32);
+  } else {
+    p.wide = true;
+    p.threads = kWideThreads;
+  }
+  p.blocks = (int)std::min<int64_t>(cdiv(rows, per), (int64_t)sm_count() * blocks_per_sm);
+  return p;
+}
+
+// blocks of an SM: forward blocks of 256 threads fill it; the gradient's hold more registers,
+// and each writes its column sums
+constexpr int kForwardBlocks = 8, kBackwardBlocks = 4;
+
+template <typename T, int VEC, bool FP8>
+void launch_forward(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
+  switch (p.lanes) {
+    case 4: norm_forward_kernel<T, VEC, 4, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 8: norm_forward_kernel<T, VEC, 8, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 16: norm_forward_kernel<T, VEC, 16, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 32: norm_forward_kernel<T, VEC, 32, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    default: norm_forward_kernel<T, VEC, 0, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+  }
+}
+
+template <typename T, bool FP8>
+int forward_typed(const NormArgs &a, cudaStream_t s) {
+  const bool aligned = aligned16(a.x) && aligned16(a.r) && aligned16(a.h) && aligned16(a.y) &&
+                       aligned16(a.q);
+  const NormPlan p = norm_plan(a.rows, a.dim, sizeof(T), aligned, kForwardBlocks);
+  if (p.wide)
+    norm_forward_wide_kernel<T, FP8><<<p.blocks, p.threads, 0, s>>>(a);
+  else if (p.vec)
+    launch_forward<T, vec_of<T>(), FP8>(p, a, s);
+  else
+    launch_forward<T, 1, FP8>(p, a, s);
+  return after_launch("norm_forward_kernel");
+}
+
+template <typename T, int VEC>
+void launch_backward(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
+  switch (p.lanes) {
+    case 4: norm_backward_kernel<T, VEC, 4><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 8: norm_backward_kernel<T, VEC, 8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 16: norm_backward_kernel<T, VEC, 16><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 32: norm_backward_kernel<T, VEC, 32><<<p.blocks, p.threads, 0, s>>>(a); break;
+    default: norm_backward_kernel<T, VEC, 0><<<p.blocks, p.threads, 0, s>>>(a); break;
+  }
+}
+
+int check_norm(const char *what, int64_t rows, int64_t dim, int dtype, int weight_dtype,
+               float eps) {
+  if (rows < 0 || dim < 1)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: rows %lld, dim %lld", what, (long long)rows,
+                (long long)dim);
+  if (dim > (int64_t)1 << 30 || (rows > 0 && dim > ((int64_t)1 << 46) / rows))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: %lld x %lld elements are too many", what,
+                (long long)rows, (long long)dim);
+  if (dtype != LNET_F32 && dtype != LNET_BF16)
+    return fail(LNET_ERR_UNSUPPORTED, "%s: dtype must be fp32 or bf16", what);
+  if (weight_dtype != LNET_F32 && weight_dtype != LNET_BF16)
+    return fail(LNET_ERR_UNSUPPORTED, "%s: the weight must be fp32 or bf16", what);
+  if (!(eps >= 0.f)) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: eps must be >= 0", what);
+  return LNET_OK;
+}
+
+int norm_grad_blocks(int64_t rows, int64_t dim, int elem) {
+  // the larger of the aligned and the unaligned plan: the size query does not see the pointers
+  return std::max(norm_plan(rows, dim, elem, true, kBackwardBlocks).blocks,
+                  norm_plan(rows, dim, elem, false, kBackwardBlocks).blocks);
+}
+
+}  // namespace
+}  // namespace lnet
+
+using namespace lnet;
+
+extern "C" int lnet_b200_residual_rms_norm(const void *x, const void *residual, const void *weight,
+                                           int32_t dtype, int32_t weight_dtype, int64_t rows,
+                                           int64_t dim, float eps, void *y, void *stream_out,
+                                           float *rstd, lnet_stream_t stream) {
+  const char *what = "residual_rms_norm";
+  LNET_TRY(check_norm(what, rows, dim, dtype, weight_dtype, eps));
+  reset_launches();
+  if (rows == 0) return LNET_OK;
+  if (!x || !weight || !y || (residual && !stream_out))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: x, weight, y%s must not be NULL", what,
+                residual ? ", stream_out" : "");
+  begin_entry(stream);
+  NormArgs a{x, residual, weight, y, stream_out, nullptr, nullptr, rstd, rows, dim, eps,
+             weight_dtype == LNET_BF16};
+  return dtype == LNET_BF16 ? forward_typed<__nv_bfloat16, false>(a, stream)
+                            : forward_typed<float, false>(a, stream);
+}
+
+extern "C" int lnet_b200_residual_rms_norm_fp8(const void *x, const void *residual,
+                                               const void *weight, int32_t dtype,
+                                               int32_t weight_dtype, int64_t rows, int64_t dim,
+                                               float eps, uint8_t *values, float *scales,
+                                               void *stream_out, lnet_stream_t stream) {
+  const char *what = "residual_rms_norm_fp8";
+  LNET_TRY(check_norm(what, rows, dim, dtype, weight_dtype, eps));
+  reset_launches();
+  if (rows == 0) return LNET_OK;
+  if (!x || !weight || !values || !scales || (residual && !stream_out))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: x, weight, values, scales%s must not be NULL",
+                what, residual ? ", stream_out" : "");
+  begin_entry(stream);
+  NormArgs a{x, residual, weight, nullptr, stream_out, values, scales, nullptr, rows, dim, eps,
+             weight_dtype == LNET_BF16};
+  return dtype == LNET_BF16 ? forward_typed<__nv_bfloat16, true>(a, stream)
+                            : forward_typed<float, true>(a, stream);
+}
+
+extern "C" int lnet_b200_residual_rms_norm_workspace_size(int32_t dtype, int64_t rows, int64_t dim,
+                                                          size_t *bytes) {
+  const char *what = "residual_rms_norm_workspace_size";
+  LNET_TRY(check_norm(what, rows, dim, dtype, LNET_F32, 0.f));
+  if (!bytes) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: bytes must not be NULL", what);
+  *bytes = rows == 0 ? 0
+                     : (size_t)norm_grad_blocks(rows, dim, dtype == LNET_BF16 ? 2 : 4) *
+                           (size_t)dim * sizeof(float);
+  return LNET_OK;
+}
+
+extern "C" int lnet_b200_residual_rms_norm_backward(
+    const void *stream_in, const float *rstd, const void *weight, const void *dy,
+    const void *dstream, int32_t dtype, int32_t weight_dtype, int64_t rows, int64_t dim, void *dx,
+    void *dweight, void *workspace, size_t workspace_bytes, lnet_stream_t stream) {
+  const char *what = "residual_rms_norm_backward";
+  LNET_TRY(check_norm(what, rows, dim, dtype, weight_dtype, 0.f));
+  reset_launches();
+  if (rows > 0 && (!stream_in || !rstd || !weight || !dy || !dx))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: stream, rstd, weight, dy, dx must not be NULL",
+                what);
+  begin_entry(stream);
+  if (rows == 0) {
+    if (dweight)
+      LNET_TRY(cuda_check(cudaMemsetAsync(dweight, 0, dim * (weight_dtype == LNET_BF16 ? 2 : 4),
+                                          stream),
+                          what));
+    return LNET_OK;
+  }
+  const int elem = dtype == LNET_BF16 ? 2 : 4;
+  const bool aligned =
+      aligned16(stream_in) && aligned16(dy) && aligned16(dstream) && aligned16(dx);
+  const NormPlan p = norm_plan(rows, dim, elem, aligned, kBackwardBlocks);
+  const size_t need = dweight ? (size_t)p.blocks * (size_t)dim * sizeof(float) : 0;
+  if (need > workspace_bytes || (need && !workspace))
+    return fail(LNET_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", what, need,
+                workspace_bytes);
+  NormGradArgs a{stream_in, weight, dy, dstream, rstd, dx,
+                 dweight ? reinterpret_cast<float *>(workspace) : nullptr, rows, dim,
+                 weight_dtype == LNET_BF16};
+  if (dtype == LNET_BF16) {
+    if (p.wide)
+      norm_backward_wide_kernel<__nv_bfloat16><<<p.blocks, p.threads, 0, stream>>>(a);
+    else if (p.vec)
+      launch_backward<__nv_bfloat16, 8>(p, a, stream);
+    else
+      launch_backward<__nv_bfloat16, 1>(p, a, stream);
+  } else {
+    if (p.wide)
+      norm_backward_wide_kernel<float><<<p.blocks, p.threads, 0, stream>>>(a);
+    else if (p.vec)
+      launch_backward<float, 4>(p, a, stream);
+    else
+      launch_backward<float, 1>(p, a, stream);
+  }
+  LNET_TRY(after_launch("norm_backward_kernel"));
+  if (dweight) {
+    norm_columns_kernel<<<(unsigned)cdiv(dim, 32), dim3(32, kReduceLanes), 0, stream>>>(
+        a.partial, p.blocks, dim, dweight, a.w_bf16);
+    LNET_TRY(after_launch("norm_columns_kernel"));
+  }
+  return LNET_OK;
+}

@@ -1,0 +1,139 @@
+// Row-wise helpers of the feed-forward and distillation operators: 16-byte or
+// scalar chunks of a row in fp32, reductions over a group of lanes or a block.
+#pragma once
+
+#include "common.cuh"
+
+namespace lnet {
+
+// VEC consecutive elements of a row: 16 bytes, or one element where the row's
+// pitch or base does not keep 16-byte alignment.
+template <typename T, int VEC>
+struct RowChunk {
+  static_assert(VEC == 1 || VEC * sizeof(T) == 16, "a chunk is one element or 16 bytes");
+};
+
+template <>
+struct RowChunk<float, 1> {
+  float raw;
+  __device__ __forceinline__ void load(const float *p) { raw = __ldg(p); }
+  __device__ __forceinline__ void store(float *p) const { *p = raw; }
+  __device__ __forceinline__ void zero() { raw = 0.f; }
+  __device__ __forceinline__ void get(float *v) const { v[0] = raw; }
+  __device__ __forceinline__ void put(const float *v) { raw = v[0]; }
+};
+template <>
+struct RowChunk<__nv_bfloat16, 1> {
+  uint16_t raw;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+    raw = __ldg(reinterpret_cast<const uint16_t *>(p));
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16 *p) const {
+    *reinterpret_cast<uint16_t *>(p) = raw;
+  }
+  __device__ __forceinline__ void zero() { raw = 0; }
+  __device__ __forceinline__ void get(float *v) const {
+    v[0] = __uint_as_float((uint32_t)raw << 16);
+  }
+  __device__ __forceinline__ void put(const float *v) {
+    raw = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+  }
+};
+template <>
+struct RowChunk<float, 4> {
+  float4 raw;
+  __device__ __forceinline__ void load(const float *p) {
+    raw = __ldg(reinterpret_cast<const float4 *>(p));
+  }
+  __device__ __forceinline__ void store(float *p) const { *reinterpret_cast<float4 *>(p) = raw; }
+  __device__ __forceinline__ void zero() { raw = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void get(float *v) const {
+    v[0] = raw.x, v[1] = raw.y, v[2] = raw.z, v[3] = raw.w;
+  }
+  __device__ __forceinline__ void put(const float *v) {
+    raw = make_float4(v[0], v[1], v[2], v[3]);
+  }
+};
+template <>
+struct RowChunk<__nv_bfloat16, 8> {
+  uint4 raw;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+    raw = __ldg(reinterpret_cast<const uint4 *>(p));
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16 *p) const {
+    *reinterpret_cast<uint4 *>(p) = raw;
+  }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void get(float *v) const {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+  __device__ __forceinline__ void put(const float *v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+    raw = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+};
+
+template <typename T>
+__host__ __device__ constexpr int vec_of() {
+  return 16 / (int)sizeof(T);
+}
+
+struct SumOp {
+  static __device__ __forceinline__ float id() { return 0.f; }
+  static __device__ __forceinline__ float of(float a, float b) { return a + b; }
+};
+// Maximum that keeps a NaN of either side.
+struct MaxNanOp {
+  static __device__ __forceinline__ float id() { return 0.f; }  // of absolute values
+  static __device__ __forceinline__ float of(float a, float b) {
+    return (a != a || a > b) ? a : b;
+  }
+};
+
+// Reduction over G lanes of a warp (G a power of two), or over the block where
+// G = 0 (`scratch`: 33 floats of shared memory; the block's size is a multiple
+// of 32).  Every thread gets the result.
+template <int G, typename Op>
+__device__ __forceinline__ float group_reduce(float v, float *scratch) {
+  constexpr int W = G == 0 ? 32 : G;
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  if (G == 0) {
+    const int warps = blockDim.x >> 5;
+    if (warps == 1) return v;
+    __syncthreads();  // the scratch of an earlier reduction has been read
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = (threadIdx.x & 31) < warps ? scratch[threadIdx.x & 31] : Op::id();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  }
+  return v;
+}
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// SMs of the current device (queried once per process; every GPU of a box is
+// the same part).
+inline int sm_count() {
+  static const int n = [] {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess ||
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1)
+      v = 148;
+    return v;
+  }();
+  return n;
+}
+
+}  // namespace lnet

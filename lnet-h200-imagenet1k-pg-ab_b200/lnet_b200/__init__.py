@@ -19,6 +19,9 @@ Laplace layer behind the reference ``lnet`` module API.
   GPU (:meth:`B200Alphabet.forward_images`).
 * :mod:`lnet_b200.pipeline` — host-fed serving loop overlapping the copies of
   the next batch with the current forward.
+* :mod:`lnet_b200.norm` — residual addition + RMSNorm, its gradient and an 8-bit
+  output.
+* :mod:`lnet_b200.distill` — distillation loss against a teacher's top logits.
 * :mod:`lnet_b200.graph` — CUDA-graph capture and replay of a prepared forward.
 
 All compute runs in the C-ABI CUDA library ``_lib/liblnet_b200.so`` built by
@@ -27,6 +30,7 @@ All compute runs in the C-ABI CUDA library ``_lib/liblnet_b200.so`` built by
 
 from . import ops  # registers the lnet_b200:: custom ops
 from .alphabet import AlphabetConfig, B200Alphabet
+from .distill import distillation_loss
 from .inference import prepare_compiled_inference, prepare_maskless_inference
 from .train_runtime import (
     AlphabetTrainingRuntime,
@@ -38,6 +42,7 @@ from .laplace import (
     LaplaceParameterError,
     LaplaceShapeError,
 )
+from .norm import residual_rms_norm, residual_rms_norm_fp8
 
 __all__ = [
     "AlphabetConfig",
@@ -46,9 +51,12 @@ __all__ = [
     "B200PoleResidueTemporalMixing",
     "LaplaceParameterError",
     "LaplaceShapeError",
+    "distillation_loss",
     "ops",
     "prepare_aggressive_training",
     "prepare_compiled_inference",
     "prepare_exact_split_training",
     "prepare_maskless_inference",
+    "residual_rms_norm",
+    "residual_rms_norm_fp8",
 ]

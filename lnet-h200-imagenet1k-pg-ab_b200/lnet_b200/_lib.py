@@ -79,6 +79,22 @@ class AlphabetGrads(ctypes.Structure):
     _fields_ = [(name, _c_p) for name in PARAM_POINTER_FIELDS]
 
 
+class DistillRequest(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64),
+        ("classes", _i64),
+        ("top", _i64),
+        ("dtype", _i32),
+        ("reduction", _i32),
+        ("logits", _c_p),
+        ("teacher_indices", _c_p),
+        ("teacher_logits", _c_p),
+        ("labels", _c_p),
+        ("temperature", ctypes.c_float),
+        ("alpha", ctypes.c_float),
+    ]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "lnet_b200_alphabet_train_workspace_size": (
@@ -199,6 +215,34 @@ SIGNATURES = {
         [_c_p, _c_p, _c_p, _c_p, _i32, _i32, ctypes.c_double, ctypes.c_double, _i32, _c_p, _i64,
          _i64, _c_p, _c_p],
     ),
+    "lnet_b200_residual_rms_norm": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _i32, _i32, _i64, _i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "lnet_b200_residual_rms_norm_fp8": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _i32, _i32, _i64, _i64, ctypes.c_float, _c_p, _c_p, _c_p, _c_p],
+    ),
+    "lnet_b200_residual_rms_norm_workspace_size": (
+        ctypes.c_int, [_i32, _i64, _i64, ctypes.POINTER(ctypes.c_size_t)]
+    ),
+    "lnet_b200_residual_rms_norm_backward": (
+        ctypes.c_int,
+        [_c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, ctypes.c_size_t,
+         _c_p],
+    ),
+    "lnet_b200_distill_workspace_size": (
+        ctypes.c_int, [ctypes.POINTER(DistillRequest), ctypes.POINTER(ctypes.c_size_t)]
+    ),
+    "lnet_b200_distill_forward": (
+        ctypes.c_int,
+        [ctypes.POINTER(DistillRequest), _c_p, ctypes.c_size_t, _c_p, _c_p, _c_p],
+    ),
+    "lnet_b200_distill_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(DistillRequest), _c_p, ctypes.c_size_t, _c_p, _c_p, _c_p],
+    ),
+    "lnet_b200_distill_scale": (ctypes.c_int, [_c_p, _i32, _i64, _c_p, _c_p]),
     "lnet_b200_trace_enable": (ctypes.c_int, [ctypes.c_int]),
     "lnet_b200_trace_read": (ctypes.c_int, [ctypes.POINTER(ctypes.c_ulonglong)]),
     "lnet_b200_trace_read_async": (ctypes.c_int, [ctypes.POINTER(ctypes.c_ulonglong), _c_p]),
