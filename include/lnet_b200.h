@@ -38,6 +38,7 @@ enum lnet_b200_dtype {
   LNET_F32 = 0,
   LNET_BF16 = 1,
   LNET_F64 = 2,
+  LNET_E4M3 = 3, /* 8-bit operands of lnet_b200_linear_* only */
 };
 
 /* Effective ALPHABET parameters, all fp32 device pointers.  Frames are the
@@ -460,6 +461,10 @@ int lnet_b200_residual_rms_norm_fp8(const void *x, const void *residual, const v
                                     int64_t dim, float eps, uint8_t *values, float *scales,
                                     void *stream_out, lnet_stream_t stream);
 
+/* Rows of a matrix (LNET_F32 or LNET_BF16) in e4m3, scales[row] = max|x| / 448. */
+int lnet_b200_quantize_rows_fp8(const void *x, int32_t dtype, int64_t rows, int64_t dim,
+                                uint8_t *values, float *scales, lnet_stream_t stream);
+
 /* Gradient of lnet_b200_residual_rms_norm from its stream and rstd: dx [rows, dim]
  * (also the residual's gradient) and dweight [dim] in `weight_dtype` (NULL: not
  * wanted).  dstream is the gradient of the stream output (NULL: zero).  The column
@@ -471,6 +476,44 @@ int lnet_b200_residual_rms_norm_backward(const void *stream_in, const float *rst
                                          int32_t dtype, int32_t weight_dtype, int64_t rows,
                                          int64_t dim, void *dx, void *dweight, void *workspace,
                                          size_t workspace_bytes, lnet_stream_t stream);
+
+/* Matrix product with bias, activation and residual in its epilogue:
+ *   a = x weight^T (* x_scale[row] weight_scale[col], 8-bit operands) + bias,
+ *   y = f(a) + residual,  f: 0 identity, 1 ReLU, 2 SiLU, 3 GELU (erf).
+ * `dtype` is the operands' type: LNET_BF16, or LNET_E4M3 with a scale for every row
+ * of x and of weight.  bias, residual, y are bf16; bias and residual may be NULL.
+ * Sums are fp32, y is rounded once.  Operands whose rows do not start on 16-byte
+ * boundaries are copied to the workspace first. */
+typedef struct lnet_b200_linear_request {
+  int64_t rows;
+  int64_t inner;
+  int64_t outer;
+  int32_t dtype;
+  int32_t activation;
+  const void *x;             /* [rows, inner] */
+  const void *weight;        /* [outer, inner] */
+  const void *bias;          /* [outer] or NULL */
+  const void *residual;      /* [rows, outer] or NULL */
+  const float *x_scale;      /* [rows] (8-bit operands) */
+  const float *weight_scale; /* [outer] (8-bit operands) */
+} lnet_b200_linear_request;
+
+int lnet_b200_linear_workspace_size(const lnet_b200_linear_request *req, size_t *bytes);
+/* preact [rows, outer] bf16 receives a where it is not NULL: the gradient through an
+ * activation needs it. */
+int lnet_b200_linear_forward(const lnet_b200_linear_request *req, void *workspace,
+                             size_t workspace_bytes, void *y, void *preact,
+                             lnet_stream_t stream);
+/* Gradient (bf16 operands): da = dy f'(preact), dx = da weight, dweight = da^T x,
+ * dbias = column sums of da; each output may be NULL.  da is rounded to bf16 as an
+ * operand of the products.  The residual's gradient is dy.  The same bits every time. */
+int lnet_b200_linear_backward_workspace_size(const lnet_b200_linear_request *req,
+                                             const void *preact, const void *dy, int32_t want_dx,
+                                             int32_t want_dweight, int32_t want_dbias,
+                                             size_t *bytes);
+int lnet_b200_linear_backward(const lnet_b200_linear_request *req, const void *preact,
+                              const void *dy, void *workspace, size_t workspace_bytes, void *dx,
+                              void *dweight, void *dbias, lnet_stream_t stream);
 
 /* Distillation from a teacher's top logits, mixed with hard labels.  Row i has the
  * entries j with teacher_indices[i, j] >= 0 and teacher_logits[i, j] > -inf:

@@ -1,0 +1,605 @@
+// Matrix product with bias, activation and residual in its epilogue, its
+// gradient, and its 8-bit form.
+//
+//   a = x W^T (* x_scale[row] weight_scale[col]) + bias,  y = f(a) + residual
+//   gradient: da = dy f'(a),  dx = da W,  dW = da^T x,  dbias = sum over rows of da
+//
+// Three shapes of work:
+//   * up to 8 rows: every weight is used once or a few times, so the call is
+//     bound by reading them; a warp takes a column, 16 bytes of weights a lane
+//     and step, and multiplies on the CUDA cores (vector_kernel);
+//   * more rows: tensor cores (gemm_tiles.cuh); where the output has fewer tiles
+//     than SMs and k is long, k is split and the fp32 partial sums are joined,
+//     with the epilogue, in a second kernel;
+//   * the elementwise slope da, rounded to bf16 as the operand of the two
+//     products (fp32 on the way, and in the bias' column sums).
+// TMA wants 16-byte aligned rows: an operand with other rows is first copied to
+// the workspace with its rows padded.
+#include <algorithm>
+#include <atomic>
+
+#include "gemm_tiles.cuh"
+#include "rows.cuh"
+
+namespace lnet {
+namespace {
+
+constexpr int kVectorRows = 8;
+constexpr int kVectorThreads = 256;
+constexpr int kPackThreads = 256;
+constexpr int kSlopeLanes = 8;  // row lanes of a block of the slope kernel
+
+struct VectorArgs {
+  const void *x, *w;
+  TileEpilogue e;
+  int64_t N, K;
+  int rows;
+};
+
+__device__ __forceinline__ float2 e4m3_pair_value(uint16_t q) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)q, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2 *>(&h));
+}
+
+// 16 bytes of operand: 8 bf16 or 16 e4m3.
+template <bool FP8>
+__device__ __forceinline__ void operand_values(const uint4 &u, float *v) {
+  const uint32_t q[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (FP8) {
+      const float2 a = e4m3_pair_value((uint16_t)(q[i] & 0xFFFF));
+      const float2 b = e4m3_pair_value((uint16_t)(q[i] >> 16));
+      v[4 * i] = a.x, v[4 * i + 1] = a.y, v[4 * i + 2] = b.x, v[4 * i + 3] = b.y;
+    } else {
+      v[2 * i] = __uint_as_float(q[i] << 16);
+      v[2 * i + 1] = __uint_as_float(q[i] & 0xFFFF0000u);
+    }
+  }
+}
+template <bool FP8>
+__device__ __forceinline__ float operand_value(const void *p, int64_t i) {
+  if (FP8) return e4m3_pair_value(reinterpret_cast<const uint8_t *>(p)[i]).x;
+  return load_f(reinterpret_cast<const __nv_bfloat16 *>(p), i);
+}
+
+// The epilogue of one value.
+__device__ __forceinline__ void scalar_epilogue(const TileEpilogue &e, float a, int64_t row,
+                                                int64_t col, int64_t N) {
+  if (e.col_scale) a = a * __ldg(e.row_scale + row) * __ldg(e.col_scale + col);
+  if (e.bias) a += load_f(e.bias, col);
+  const int64_t off = row * N + col;
+  if (e.pre) store_f(e.pre, off, a);
+  a = act_value(a, e.act);
+  if (e.residual) a += load_f(e.residual, off);
+  store_f(reinterpret_cast<__nv_bfloat16 *>(e.out), off, a);
+}
+
+// R rows of x against every weight row; a warp a column.
+template <bool FP8, int R, bool VEC>
+__global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs p) {
+  constexpr int E = FP8 ? 16 : 8, ES = FP8 ? 1 : 2;
+  constexpr int U = R <= 2 ? 4 : 2;
+  const int lane = threadIdx.x & 31;
+  const int64_t col = (int64_t)blockIdx.x * (kVectorThreads / 32) + (threadIdx.x >> 5);
+  if (col >= p.N) return;
+  float acc[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) acc[r] = 0.f;
+  if (VEC) {
+    const uint4 *w = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.w) +
+                                                     col * p.K * ES);
+    const uint4 *x = reinterpret_cast<const uint4 *>(p.x);
+    const int nc = (int)(p.K / E);
+    for (int c0 = lane; c0 < nc; c0 += 32 * U) {
+      uint4 wu[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        wu[u] = c0 + 32 * u < nc ? __ldg(w + c0 + 32 * u) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (c0 + 32 * u >= nc) break;
+        float wv[E];
+        operand_values<FP8>(wu[u], wv);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          if (r >= p.rows) break;
+          float xv[E];
+          operand_values<FP8>(__ldg(x + (int64_t)r * nc + c0 + 32 * u), xv);
+#pragma unroll
+          for (int i = 0; i < E; ++i) acc[r] = fmaf(xv[i], wv[i], acc[r]);
+        }
+      }
+    }
+  } else {
+    for (int64_t k = lane; k < p.K; k += 32) {
+      const float wv = operand_value<FP8>(p.w, col * p.K + k);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+        if (r < p.rows) acc[r] = fmaf(operand_value<FP8>(p.x, r * p.K + k), wv, acc[r]);
+    }
+  }
+  float mine = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const float s = group_reduce<32, SumOp>(acc[r], nullptr);
+    if (lane == r) mine = s;
+  }
+  if (lane < p.rows) scalar_epilogue(p.e, mine, lane, col, p.N);
+}
+
+// Rows copied to a padded pitch (elements of ES bytes; the padding is zero).
+template <int ES>
+__global__ void __launch_bounds__(kPackThreads)
+pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols,
+            uint8_t *__restrict__ dst, int64_t pitch) {
+  const int64_t total = rows * pitch;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / pitch, c = i - r * pitch;
+    if (ES == 2) {
+      uint16_t v = 0;
+      if (c < cols) v = reinterpret_cast<const uint16_t *>(src)[r * cols + c];
+      reinterpret_cast<uint16_t *>(dst)[i] = v;
+    } else {
+      dst[i] = c < cols ? src[r * cols + c] : 0;
+    }
+  }
+}
+
+// y from the splits' fp32 sums, added in split order.
+__global__ void __launch_bounds__(256)
+join_kernel(const float *__restrict__ partial, int splits, int64_t M, int64_t N, TileEpilogue e) {
+  const int64_t total = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += partial[k * total + i];
+    const int64_t row = i / N;
+    scalar_epilogue(e, s, row, i - row * N, N);
+  }
+}
+
+// da = dy f'(pre) in bf16 (pitch `pitch`, its padding zero; null: not wanted), and the blocks'
+// column sums of the unrounded da (null: not wanted).  A thread holds VEC columns of every
+// kSlopeLanes-th row of its block's rows.
+template <int VEC>
+__global__ void __launch_bounds__(32 * kSlopeLanes)
+slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restrict__ pre, int act,
+             int64_t M, int64_t N, __nv_bfloat16 *__restrict__ da, int64_t pitch,
+             float *__restrict__ partial) {
+  __shared__ float sums[kSlopeLanes][32 * VEC];
+  const int64_t col = ((int64_t)blockIdx.x * 32 + threadIdx.x) * VEC;
+  float s[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) s[i] = 0.f;
+  const int64_t r0 = M * blockIdx.y / gridDim.y, r1 = M * (blockIdx.y + 1) / gridDim.y;
+  if (col < N) {
+#pragma unroll 2
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += kSlopeLanes) {
+      RowChunk<__nv_bfloat16, VEC> c, q;
+      c.load(dy + r * N + col);
+      float g[VEC];
+      c.get(g);
+      if (pre) {
+        float a[VEC];
+        q.load(pre + r * N + col);
+        q.get(a);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[i] *= act_slope(a[i], act);
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[i] += g[i];
+      if (da) {
+        c.put(g);
+        c.store(da + r * pitch + col);
+      }
+    }
+  } else if (da && col < pitch) {
+    RowChunk<__nv_bfloat16, VEC> c;
+    c.zero();
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += kSlopeLanes) c.store(da + r * pitch + col);
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) sums[threadIdx.y][threadIdx.x * VEC + i] = s[i];
+  __syncthreads();
+  for (int c = threadIdx.y * 32 + threadIdx.x; c < 32 * VEC; c += 32 * kSlopeLanes) {
+    const int64_t out = (int64_t)blockIdx.x * 32 * VEC + c;
+    if (out >= N) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int l = 0; l < kSlopeLanes; ++l) t += sums[l][c];
+    partial[(int64_t)blockIdx.y * N + out] = t;
+  }
+}
+
+// dbias from the blocks' column sums, in block order (32 columns by 32 lanes).
+__global__ void __launch_bounds__(1024)
+column_sum_kernel(const float *__restrict__ partial, int blocks, int64_t N,
+                  __nv_bfloat16 *__restrict__ out) {
+  __shared__ float part[32][33];
+  const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < N)
+    for (int b = threadIdx.y; b < blocks; b += 32) s += partial[(int64_t)b * N + c];
+  part[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < N) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += part[i][threadIdx.x];
+    store_f(out, c, s);
+  }
+}
+
+// ---------------------------------------------------------------- plans
+enum TileKind { kPair256, kPair128, kOne128, kOne64 };
+
+struct ProductPlan {
+  TileKind kind;
+  int ctas, bn, m_tiles, n_tiles, splits, kblocks, grid;
+  int64_t partial_floats;
+};
+
+// Tile shape and split of an [M, N] product over `kblocks` blocks of 128 bytes.
+ProductPlan product_plan(int64_t M, int64_t N, int kblocks) {
+  const int sms = sm_count();
+  struct Shape {
+    TileKind kind;
+    int ctas, bn;
+    double cost;  // of a k block, in 128 x 64 tiles' time
+  };
+  static const Shape shapes[] = {
+      {kPair256, 2, 256, 4.0}, {kPair128, 2, 128, 2.2}, {kOne128, 1, 128, 2.4}, {kOne64, 1, 64, 1.4}};
+  ProductPlan best{};
+  double best_cost = 0;
+  for (const Shape &s : shapes) {
+    const int64_t mt = cdiv(M, (int64_t)kTileM * s.ctas), nt = cdiv(N, s.bn);
+    const int slots = sms / s.ctas;
+    int splits = 1;
+    if (mt * nt * 2 <= slots) {  // k split until the SMs are busy, 4 blocks a split at least
+      splits = (int)std::min<int64_t>(slots / (mt * nt), std::max(1, kblocks / 4));
+      splits = std::min(splits, 64);
+    }
+    const int64_t waves = cdiv(mt * nt * splits, slots);
+    // a tile costs its k blocks and about 6 blocks' time of fill and epilogue; a split is
+    // written and read once more
+    const double cost = (double)waves * s.cost * ((double)cdiv(kblocks, splits) + 6.0) +
+                        (splits > 1 ? 12.0 : 0.0);
+    if (best_cost == 0 || cost < best_cost) {
+      best_cost = cost;
+      best = ProductPlan{s.kind, s.ctas, s.bn, (int)mt, (int)nt, splits, kblocks,
+                         (int)std::min<int64_t>(mt * nt * splits, slots) * s.ctas,
+                         splits > 1 ? (int64_t)splits * M * N : 0};
+    }
+  }
+  return best;
+}
+
+template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
+int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
+                 cudaStream_t stream) {
+  using S = TileShape<CTAS, BN, FP8>;
+  auto *kernel = tile_gemm_kernel<CTAS, BN, A_MN, B_MN, FP8>;
+  static std::atomic<uint64_t> ready{0};  // devices whose shared memory limit is raised
+  int dev = 0;
+  LNET_TRY(cuda_check(cudaGetDevice(&dev), "cudaGetDevice"));
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (!(ready.load() & bit)) {
+    LNET_TRY(cuda_check(
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM),
+        "tile_gemm_kernel shared memory"));
+    ready.fetch_or(bit);
+  }
+  LNET_TRY(tile_tensor_map(&args.a, a, FP8, kTileM));
+  LNET_TRY(tile_tensor_map(&args.b, b, FP8, S::NB));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)q.grid);
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute cluster{};
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = CTAS;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  LNET_TRY(cuda_check(cudaLaunchKernelEx(&cfg, kernel, args), "tile_gemm_kernel"));
+  return after_launch("tile_gemm_kernel");
+}
+
+template <bool A_MN, bool B_MN, bool FP8>
+int launch_kind(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
+                cudaStream_t s) {
+  switch (q.kind) {
+    case kPair256: return launch_tiles<2, 256, A_MN, B_MN, FP8>(q, a, b, args, s);
+    case kPair128: return launch_tiles<2, 128, A_MN, B_MN, FP8>(q, a, b, args, s);
+    case kOne128: return launch_tiles<1, 128, A_MN, B_MN, FP8>(q, a, b, args, s);
+    default: return launch_tiles<1, 64, A_MN, B_MN, FP8>(q, a, b, args, s);
+  }
+}
+
+// C = A B^T through the epilogue; `partial` holds plan.partial_floats.
+template <bool A_MN, bool B_MN, bool FP8>
+int product(const TileOperand &a, const TileOperand &b, const TileEpilogue &e, float *partial,
+            cudaStream_t s) {
+  const int64_t M = a.mn, N = b.mn;
+  const int kblocks = (int)cdiv(a.k, FP8 ? 128 : 64);
+  const ProductPlan q = product_plan(M, N, kblocks);
+  TileArgs args{};
+  args.e = e;
+  args.M = M, args.N = N;
+  args.m_tiles = q.m_tiles, args.n_tiles = q.n_tiles, args.splits = q.splits;
+  args.kblocks = kblocks;
+  args.partial = q.splits > 1;
+  args.vec = N % 8 == 0 && aligned16(e.out) && aligned16(e.pre) && aligned16(e.bias) &&
+             aligned16(e.residual) && aligned16(e.col_scale);
+  if (args.partial) {
+    args.e = TileEpilogue{};
+    args.e.out = partial;
+    args.vec = N % 4 == 0;
+  }
+  LNET_TRY((launch_kind<A_MN, B_MN, FP8>(q, a, b, args, s)));
+  if (args.partial) {
+    const int64_t total = M * N;
+    const int blocks = (int)std::min<int64_t>(cdiv(total, 256), (int64_t)sm_count() * 16);
+    join_kernel<<<blocks, 256, 0, s>>>(partial, q.splits, M, N, e);
+    LNET_TRY(after_launch("linear_join_kernel"));
+  }
+  return LNET_OK;
+}
+
+bool tma_rows(const void *p, int64_t pitch_bytes) { return aligned16(p) && pitch_bytes % 16 == 0; }
+
+// `o` itself, or its copy with padded rows (element (i, j) of a rows x cols matrix).
+int packed(TileOperand &o, int64_t rows, int64_t cols, int elem, void *copy, cudaStream_t s) {
+  if (!copy) return LNET_OK;
+  const int64_t pitch = (int64_t)align_up((size_t)cols * elem, 16) / elem;
+  const int64_t total = rows * pitch;
+  const int blocks = (int)std::min<int64_t>(cdiv(total, kPackThreads * 4), (int64_t)sm_count() * 16);
+  if (elem == 2)
+    pack_kernel<2><<<blocks, kPackThreads, 0, s>>>(reinterpret_cast<const uint8_t *>(o.ptr), rows,
+                                                   cols, reinterpret_cast<uint8_t *>(copy), pitch);
+  else
+    pack_kernel<1><<<blocks, kPackThreads, 0, s>>>(reinterpret_cast<const uint8_t *>(o.ptr), rows,
+                                                   cols, reinterpret_cast<uint8_t *>(copy), pitch);
+  o.ptr = copy;
+  o.pitch = pitch;
+  return after_launch("linear_pack_kernel");
+}
+
+int check_linear(const char *what, const lnet_b200_linear_request *q) {
+  if (!q) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: request must not be NULL", what);
+  if (q->rows < 0 || q->inner < 1 || q->outer < 1)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: rows %lld, inner %lld, outer %lld", what,
+                (long long)q->rows, (long long)q->inner, (long long)q->outer);
+  const int64_t most = (int64_t)1 << 30;
+  if (q->rows > most || q->inner > most || q->outer > most)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: an extent is above 2^30", what);
+  if (cdiv(q->rows, 128) * cdiv(q->outer, 64) > most || cdiv(q->rows, 128) * cdiv(q->inner, 64) > most ||
+      cdiv(q->outer, 128) * cdiv(q->inner, 64) > most)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: a product has more than 2^30 tiles", what);
+  if (q->dtype != LNET_BF16 && q->dtype != LNET_E4M3)
+    return fail(LNET_ERR_UNSUPPORTED, "%s: operands must be bf16 or e4m3", what);
+  if (q->activation < kActNone || q->activation > kActGelu)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: activation must be 0 to 3", what);
+  if (q->rows > 0 && (!q->x || !q->weight))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: x and weight must not be NULL", what);
+  if (q->rows > 0 && q->dtype == LNET_E4M3 && (!q->x_scale || !q->weight_scale))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: 8-bit operands need x_scale and weight_scale",
+                what);
+  return LNET_OK;
+}
+
+// Workspace of the forward pass: operands that TMA cannot address, partial sums.
+struct ForwardWork {
+  void *x, *w;
+  float *partial;
+};
+ForwardWork forward_work(Arena &ar, const lnet_b200_linear_request *q) {
+  ForwardWork f{};
+  if (q->rows <= kVectorRows) return f;
+  const int elem = q->dtype == LNET_BF16 ? 2 : 1;
+  const size_t pitch = align_up((size_t)q->inner * elem, 16);
+  if (!tma_rows(q->x, q->inner * elem)) f.x = ar.take<uint8_t>(q->rows * pitch);
+  if (!tma_rows(q->weight, q->inner * elem)) f.w = ar.take<uint8_t>(q->outer * pitch);
+  const ProductPlan p = product_plan(q->rows, q->outer, (int)cdiv(q->inner * elem, 128));
+  if (p.partial_floats) f.partial = ar.take<float>(p.partial_floats);
+  return f;
+}
+
+int slope_row_blocks(int64_t M, int64_t N, int vec) {
+  const int64_t across = cdiv(N, 32 * vec);
+  const int64_t want = cdiv((int64_t)sm_count() * 6, across);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, cdiv(M, kSlopeLanes * 2)));
+}
+int slope_vec(const lnet_b200_linear_request *q, const void *pre, const void *dy) {
+  return q->outer % 8 == 0 && aligned16(pre) && aligned16(dy) ? 8 : 1;
+}
+
+// Workspace of the gradient.
+struct BackwardWork {
+  __nv_bfloat16 *da;  // null: dy itself serves
+  void *x, *w;
+  float *partial, *columns;
+};
+BackwardWork backward_work(Arena &ar, const lnet_b200_linear_request *q, const void *pre,
+                           const void *dy, bool want_dx, bool want_dw, bool want_db) {
+  BackwardWork b{};
+  const size_t pitch_in = align_up((size_t)q->inner * 2, 16);
+  const size_t pitch_out = align_up((size_t)q->outer * 2, 16);
+  if ((want_dx || want_dw) && (pre || !tma_rows(dy, q->outer * 2)))
+    b.da = ar.take<__nv_bfloat16>(q->rows * pitch_out / 2);
+  if (want_dw && !tma_rows(q->x, q->inner * 2)) b.x = ar.take<uint8_t>(q->rows * pitch_in);
+  if (want_dx && !tma_rows(q->weight, q->inner * 2)) b.w = ar.take<uint8_t>(q->outer * pitch_in);
+  int64_t partial = 0;
+  if (want_dx)
+    partial = product_plan(q->rows, q->inner, (int)cdiv(q->outer, 64)).partial_floats;
+  if (want_dw)
+    partial = std::max(partial,
+                       product_plan(q->outer, q->inner, (int)cdiv(q->rows, 64)).partial_floats);
+  if (partial) b.partial = ar.take<float>(partial);
+  if (want_db)
+    b.columns = ar.take<float>((size_t)slope_row_blocks(q->rows, q->outer, slope_vec(q, pre, dy)) *
+                               q->outer);
+  return b;
+}
+
+template <bool FP8, bool VEC>
+void launch_vector(const VectorArgs &v, cudaStream_t s) {
+  const unsigned blocks = (unsigned)cdiv(v.N, kVectorThreads / 32);
+  if (v.rows == 1)
+    vector_kernel<FP8, 1, VEC><<<blocks, kVectorThreads, 0, s>>>(v);
+  else if (v.rows == 2)
+    vector_kernel<FP8, 2, VEC><<<blocks, kVectorThreads, 0, s>>>(v);
+  else if (v.rows <= 4)
+    vector_kernel<FP8, 4, VEC><<<blocks, kVectorThreads, 0, s>>>(v);
+  else
+    vector_kernel<FP8, 8, VEC><<<blocks, kVectorThreads, 0, s>>>(v);
+}
+
+}  // namespace
+}  // namespace lnet
+
+using namespace lnet;
+
+extern "C" int lnet_b200_linear_workspace_size(const lnet_b200_linear_request *req,
+                                               size_t *bytes) {
+  const char *what = "linear_workspace_size";
+  LNET_TRY(check_linear(what, req));
+  if (!bytes) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: bytes must not be NULL", what);
+  Arena ar(nullptr, 0);
+  if (req->rows > 0) forward_work(ar, req);
+  *bytes = ar.used;
+  return LNET_OK;
+}
+
+extern "C" int lnet_b200_linear_forward(const lnet_b200_linear_request *req, void *workspace,
+                                        size_t workspace_bytes, void *y, void *preact,
+                                        lnet_stream_t stream) {
+  const char *what = "linear_forward";
+  LNET_TRY(check_linear(what, req));
+  reset_launches();
+  if (req->rows == 0) return LNET_OK;
+  if (!y) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: y must not be NULL", what);
+  Arena ar(workspace, workspace_bytes);
+  const ForwardWork f = forward_work(ar, req);
+  if (ar.used > workspace_bytes || (ar.used && !workspace))
+    return fail(LNET_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", what, ar.used,
+                workspace_bytes);
+  begin_entry(stream);
+  const bool fp8 = req->dtype == LNET_E4M3;
+  const int elem = fp8 ? 1 : 2;
+  TileEpilogue e{};
+  e.out = y;
+  e.pre = reinterpret_cast<__nv_bfloat16 *>(preact);
+  e.bias = reinterpret_cast<const __nv_bfloat16 *>(req->bias);
+  e.residual = reinterpret_cast<const __nv_bfloat16 *>(req->residual);
+  e.row_scale = fp8 ? req->x_scale : nullptr;
+  e.col_scale = fp8 ? req->weight_scale : nullptr;
+  e.act = req->activation;
+  if (req->rows <= kVectorRows) {
+    const VectorArgs v{req->x, req->weight, e, req->outer, req->inner, (int)req->rows};
+    const bool vec = tma_rows(req->x, req->inner * elem) && tma_rows(req->weight, req->inner * elem);
+    if (fp8)
+      vec ? launch_vector<true, true>(v, stream) : launch_vector<true, false>(v, stream);
+    else
+      vec ? launch_vector<false, true>(v, stream) : launch_vector<false, false>(v, stream);
+    return after_launch("linear_vector_kernel");
+  }
+  TileOperand a{req->x, req->rows, req->inner, req->inner, false};
+  TileOperand b{req->weight, req->outer, req->inner, req->inner, false};
+  LNET_TRY(packed(a, req->rows, req->inner, elem, f.x, stream));
+  LNET_TRY(packed(b, req->outer, req->inner, elem, f.w, stream));
+  return fp8 ? product<false, false, true>(a, b, e, f.partial, stream)
+             : product<false, false, false>(a, b, e, f.partial, stream);
+}
+
+static int check_backward(const char *what, const lnet_b200_linear_request *req,
+                          const void *preact, const void *dy) {
+  LNET_TRY(check_linear(what, req));
+  if (req->dtype != LNET_BF16)
+    return fail(LNET_ERR_UNSUPPORTED, "%s: the gradient wants bf16 operands", what);
+  if (req->rows > 0 && (!dy || (req->activation != kActNone && !preact)))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: dy%s must not be NULL", what,
+                req->activation != kActNone ? ", preact" : "");
+  return LNET_OK;
+}
+
+extern "C" int lnet_b200_linear_backward_workspace_size(const lnet_b200_linear_request *req,
+                                                        const void *preact, const void *dy,
+                                                        int32_t want_dx, int32_t want_dweight,
+                                                        int32_t want_dbias, size_t *bytes) {
+  const char *what = "linear_backward_workspace_size";
+  LNET_TRY(check_backward(what, req, preact, dy));
+  if (!bytes) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: bytes must not be NULL", what);
+  Arena ar(nullptr, 0);
+  if (req->rows > 0)
+    backward_work(ar, req, req->activation ? preact : nullptr, dy, want_dx, want_dweight,
+                  want_dbias);
+  *bytes = ar.used;
+  return LNET_OK;
+}
+
+extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, const void *preact,
+                                         const void *dy, void *workspace, size_t workspace_bytes,
+                                         void *dx, void *dweight, void *dbias,
+                                         lnet_stream_t stream) {
+  const char *what = "linear_backward";
+  LNET_TRY(check_backward(what, req, preact, dy));
+  reset_launches();
+  begin_entry(stream);
+  const int64_t M = req->rows, N = req->outer, K = req->inner;
+  if (M == 0) {
+    if (dweight) LNET_TRY(cuda_check(cudaMemsetAsync(dweight, 0, N * K * 2, stream), what));
+    if (dbias) LNET_TRY(cuda_check(cudaMemsetAsync(dbias, 0, N * 2, stream), what));
+    return LNET_OK;
+  }
+  if (!req->activation) preact = nullptr;
+  Arena ar(workspace, workspace_bytes);
+  const BackwardWork w = backward_work(ar, req, preact, dy, dx != nullptr, dweight != nullptr,
+                                       dbias != nullptr);
+  if (ar.used > workspace_bytes || (ar.used && !workspace))
+    return fail(LNET_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", what, ar.used,
+                workspace_bytes);
+  const auto *dyp = reinterpret_cast<const __nv_bfloat16 *>(dy);
+  const auto *pre = reinterpret_cast<const __nv_bfloat16 *>(preact);
+  const int64_t pitch = w.da ? (int64_t)align_up((size_t)N * 2, 16) / 2 : N;
+  if (w.da || w.columns) {
+    const int vec = slope_vec(req, preact, dy);
+    const int64_t width = w.da ? pitch : N;
+    const dim3 grid((unsigned)cdiv(width, 32 * vec), (unsigned)slope_row_blocks(M, N, vec));
+    const dim3 block(32, kSlopeLanes);
+    if (vec == 8)
+      slope_kernel<8><<<grid, block, 0, stream>>>(dyp, pre, req->activation, M, N, w.da, pitch,
+                                                  w.columns);
+    else
+      slope_kernel<1><<<grid, block, 0, stream>>>(dyp, pre, req->activation, M, N, w.da, pitch,
+                                                  w.columns);
+    LNET_TRY(after_launch("linear_slope_kernel"));
+    if (w.columns) {
+      column_sum_kernel<<<(unsigned)cdiv(N, 32), dim3(32, 32), 0, stream>>>(
+          w.columns, (int)grid.y, N, reinterpret_cast<__nv_bfloat16 *>(dbias));
+      LNET_TRY(after_launch("linear_column_sum_kernel"));
+    }
+  }
+  const void *da = w.da ? (const void *)w.da : dy;
+  if (dx) {
+    TileOperand a{da, M, N, pitch, false};
+    TileOperand b{req->weight, K, N, K, true};
+    LNET_TRY(packed(b, N, K, 2, w.w, stream));
+    TileEpilogue e{};
+    e.out = dx;
+    LNET_TRY((product<false, true, false>(a, b, e, w.partial, stream)));
+  }
+  if (dweight) {
+    TileOperand a{da, N, M, pitch, true};
+    TileOperand b{req->x, K, M, K, true};
+    LNET_TRY(packed(b, M, K, 2, w.x, stream));
+    TileEpilogue e{};
+    e.out = dweight;
+    LNET_TRY((product<true, true, false>(a, b, e, w.partial, stream)));
+  }
+  return LNET_OK;
+}

@@ -199,6 +199,27 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
   }
 }
 
+// A matrix's rows in e4m3 with the scale max|row| / 448: what a serving program does once to
+// its weights.  A block a row, the second sweep from L2.
+template <typename T>
+__global__ void __launch_bounds__(256)
+quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t *q,
+                     float *scales) {
+  __shared__ float scratch[33];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    float amax = 0.f;
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
+      amax = MaxNanOp::of(amax, fabsf(load_f(x, row * dim + c)));
+    amax = group_reduce<0, MaxNanOp>(amax, scratch);
+    const float scale = amax / kE4m3Max;
+    if (threadIdx.x == 0) scales[row] = scale;
+    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
+      const float v = load_f(x, row * dim + c);
+      store_e4m3<1>(q + row * dim + c, &v, scale);
+    }
+  }
+}
+
 struct NormGradArgs {
   const void *h, *w, *dy, *dh;
   const float *rstd;
@@ -492,6 +513,26 @@ extern "C" int lnet_b200_residual_rms_norm_fp8(const void *x, const void *residu
              weight_dtype == LNET_BF16};
   return dtype == LNET_BF16 ? forward_typed<__nv_bfloat16, true>(a, stream)
                             : forward_typed<float, true>(a, stream);
+}
+
+extern "C" int lnet_b200_quantize_rows_fp8(const void *x, int32_t dtype, int64_t rows,
+                                           int64_t dim, uint8_t *values, float *scales,
+                                           lnet_stream_t stream) {
+  const char *what = "quantize_rows_fp8";
+  LNET_TRY(check_norm(what, rows, dim, dtype, LNET_F32, 0.f));
+  reset_launches();
+  if (rows == 0) return LNET_OK;
+  if (!x || !values || !scales)
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: x, values, scales must not be NULL", what);
+  begin_entry(stream);
+  const int blocks = (int)std::min<int64_t>(rows, (int64_t)sm_count() * 8);
+  if (dtype == LNET_BF16)
+    quantize_rows_kernel<<<blocks, 256, 0, stream>>>(reinterpret_cast<const __nv_bfloat16 *>(x),
+                                                     rows, dim, values, scales);
+  else
+    quantize_rows_kernel<<<blocks, 256, 0, stream>>>(reinterpret_cast<const float *>(x), rows, dim,
+                                                     values, scales);
+  return after_launch("quantize_rows_kernel");
 }
 
 extern "C" int lnet_b200_residual_rms_norm_workspace_size(int32_t dtype, int64_t rows, int64_t dim,

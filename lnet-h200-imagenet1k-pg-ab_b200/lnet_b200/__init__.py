@@ -21,6 +21,8 @@ Laplace layer behind the reference ``lnet`` module API.
   the next batch with the current forward.
 * :mod:`lnet_b200.norm` — residual addition + RMSNorm, its gradient and an 8-bit
   output.
+* :mod:`lnet_b200.linear` — matrix product with bias, activation and residual in
+  its epilogue, its gradient, and its form on 8-bit operands.
 * :mod:`lnet_b200.distill` — distillation loss against a teacher's top logits.
 * :mod:`lnet_b200.graph` — CUDA-graph capture and replay of a prepared forward.
 
@@ -42,6 +44,7 @@ from .laplace import (
     LaplaceParameterError,
     LaplaceShapeError,
 )
+from .linear import linear_act, linear_act_fp8, quantize_rows_fp8
 from .norm import residual_rms_norm, residual_rms_norm_fp8
 
 __all__ = [
@@ -52,11 +55,14 @@ __all__ = [
     "LaplaceParameterError",
     "LaplaceShapeError",
     "distillation_loss",
+    "linear_act",
+    "linear_act_fp8",
     "ops",
     "prepare_aggressive_training",
     "prepare_compiled_inference",
     "prepare_exact_split_training",
     "prepare_maskless_inference",
+    "quantize_rows_fp8",
     "residual_rms_norm",
     "residual_rms_norm_fp8",
 ]

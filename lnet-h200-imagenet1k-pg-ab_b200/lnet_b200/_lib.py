@@ -23,6 +23,7 @@ LNET_ERR_CUDA = 4
 LNET_F32 = 0
 LNET_BF16 = 1
 LNET_F64 = 2
+LNET_E4M3 = 3
 
 _c_p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -77,6 +78,22 @@ class AlphabetRequest(ctypes.Structure):
 class AlphabetGrads(ctypes.Structure):
     """Output pointers of lnet_b200_alphabet_backward, in PARAM_POINTER_FIELDS order."""
     _fields_ = [(name, _c_p) for name in PARAM_POINTER_FIELDS]
+
+
+class LinearRequest(ctypes.Structure):
+    _fields_ = [
+        ("rows", _i64),
+        ("inner", _i64),
+        ("outer", _i64),
+        ("dtype", _i32),
+        ("activation", _i32),
+        ("x", _c_p),
+        ("weight", _c_p),
+        ("bias", _c_p),
+        ("residual", _c_p),
+        ("x_scale", _c_p),
+        ("weight_scale", _c_p),
+    ]
 
 
 class DistillRequest(ctypes.Structure):
@@ -229,6 +246,26 @@ SIGNATURES = {
     "lnet_b200_residual_rms_norm_backward": (
         ctypes.c_int,
         [_c_p, _c_p, _c_p, _c_p, _c_p, _i32, _i32, _i64, _i64, _c_p, _c_p, _c_p, ctypes.c_size_t,
+         _c_p],
+    ),
+    "lnet_b200_quantize_rows_fp8": (
+        ctypes.c_int, [_c_p, _i32, _i64, _i64, _c_p, _c_p, _c_p]
+    ),
+    "lnet_b200_linear_workspace_size": (
+        ctypes.c_int, [ctypes.POINTER(LinearRequest), ctypes.POINTER(ctypes.c_size_t)]
+    ),
+    "lnet_b200_linear_forward": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearRequest), _c_p, ctypes.c_size_t, _c_p, _c_p, _c_p],
+    ),
+    "lnet_b200_linear_backward_workspace_size": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearRequest), _c_p, _c_p, _i32, _i32, _i32,
+         ctypes.POINTER(ctypes.c_size_t)],
+    ),
+    "lnet_b200_linear_backward": (
+        ctypes.c_int,
+        [ctypes.POINTER(LinearRequest), _c_p, _c_p, _c_p, ctypes.c_size_t, _c_p, _c_p, _c_p,
          _c_p],
     ),
     "lnet_b200_distill_workspace_size": (

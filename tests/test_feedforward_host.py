@@ -7,7 +7,8 @@ import ctypes
 import pytest
 import torch
 
-from lnet_b200 import (_lib, distillation_loss, residual_rms_norm, residual_rms_norm_fp8)
+from lnet_b200 import (_lib, distillation_loss, linear_act, linear_act_fp8, quantize_rows_fp8,
+                       residual_rms_norm, residual_rms_norm_fp8)
 
 
 @pytest.mark.parametrize("norm", [residual_rms_norm, residual_rms_norm_fp8])
@@ -31,6 +32,45 @@ def test_norm_refusals(norm):
         norm(x, w, None, -1.0)
     with pytest.raises(ValueError, match="eps"):
         norm(x, w, None, float("nan"))
+
+
+def test_linear_refusals():
+    bf = torch.bfloat16
+    x, w, b = torch.zeros(3, 8, dtype=bf), torch.zeros(5, 8, dtype=bf), torch.zeros(5, dtype=bf)
+    r = torch.zeros(3, 5, dtype=bf)
+    with pytest.raises(RuntimeError, match="CUDA only"):
+        linear_act(x, w, b, r)
+    with pytest.raises(TypeError, match="x must be"):
+        linear_act(x.float(), w)
+    with pytest.raises(TypeError, match="weight must be"):
+        linear_act(x, w.float())
+    for bad in (w[:, :7], w[0], w[:0]):
+        with pytest.raises(ValueError, match="weight must have shape"):
+            linear_act(x, bad)
+    with pytest.raises(ValueError, match="bias must have shape"):
+        linear_act(x, w, b[:4])
+    with pytest.raises(TypeError, match="bias must be"):
+        linear_act(x, w, b.float())
+    with pytest.raises(ValueError, match="residual must have shape"):
+        linear_act(x, w, b, r[:2])
+    with pytest.raises(TypeError, match="residual must be"):
+        linear_act(x, w, b, r.float())
+    with pytest.raises(ValueError, match="activation"):
+        linear_act(x, w, b, activation="tanh")
+    e4 = torch.float8_e4m3fn
+    xs, ws = torch.ones(3), torch.ones(5)
+    with pytest.raises(TypeError, match="x must be"):
+        linear_act_fp8(x, xs, w.to(e4), ws)
+    with pytest.raises(ValueError, match="x_scale must have shape"):
+        linear_act_fp8(x.to(e4), ws, w.to(e4), ws)
+    with pytest.raises(TypeError, match="weight_scale must be"):
+        linear_act_fp8(x.to(e4), xs, w.to(e4), ws.double())
+    with pytest.raises(RuntimeError, match="CUDA only"):
+        linear_act_fp8(x.to(e4), xs, w.to(e4), ws)
+    with pytest.raises(TypeError, match="t must be"):
+        quantize_rows_fp8(torch.zeros(2, 2, dtype=torch.float16))
+    with pytest.raises(RuntimeError, match="CUDA only"):
+        quantize_rows_fp8(x)
 
 
 def test_distillation_refusals():
@@ -93,4 +133,23 @@ def test_c_entries_refuse_before_any_cuda_call():
         setattr(bad, field, value)
         assert lib.lnet_b200_distill_workspace_size(
             ctypes.byref(bad), ctypes.byref(n)) == _lib.LNET_ERR_INVALID_ARGUMENT, field
+    lin = _lib.LinearRequest(rows=100, inner=90, outer=64, dtype=_lib.LNET_BF16, activation=1,
+                             x=256, weight=256)
+    assert lib.lnet_b200_linear_workspace_size(ctypes.byref(lin), ctypes.byref(n)) == _lib.LNET_OK
+    assert n.value >= 164 * 96 * 2  # rows of 180 bytes are copied to rows of 192
+    assert lib.lnet_b200_linear_forward(ctypes.byref(lin), None, 0, p, None,
+                                        None) == _lib.LNET_ERR_WORKSPACE
+    assert lib.lnet_b200_linear_backward(ctypes.byref(lin), None, p, None, 0, p, p, p,
+                                         None) == _lib.LNET_ERR_INVALID_ARGUMENT
+    assert "preact" in _lib.last_error()
+    for field, value, status in (("dtype", _lib.LNET_F32, _lib.LNET_ERR_UNSUPPORTED),
+                                 ("dtype", _lib.LNET_E4M3, _lib.LNET_ERR_INVALID_ARGUMENT),
+                                 ("activation", 4, _lib.LNET_ERR_INVALID_ARGUMENT),
+                                 ("inner", 0, _lib.LNET_ERR_INVALID_ARGUMENT),
+                                 ("outer", 1 << 40, _lib.LNET_ERR_INVALID_ARGUMENT),
+                                 ("weight", None, _lib.LNET_ERR_INVALID_ARGUMENT)):
+        bad = _lib.LinearRequest.from_buffer_copy(lin)
+        setattr(bad, field, value)
+        assert lib.lnet_b200_linear_workspace_size(ctypes.byref(bad),
+                                                   ctypes.byref(n)) == status, field
     assert lib.lnet_b200_distill_scale(None, 0, 4, p, None) == _lib.LNET_ERR_INVALID_ARGUMENT
