@@ -10,18 +10,22 @@
 // everywhere.  An index or label past the classes makes the row's loss NaN and
 // touches nothing else.
 //
-// One sweep reads the row for its running maximum and exponential sums (one sum
-// for each of the temperatures tau and 1 that the loss needs), a second one
-// writes the gradient from the row in L2 or L1; the few entries of the teacher
-// and the label are then corrected in place, each from z again, so that every
-// value is rounded once.  A row belongs to a block, or, where there are few
-// rows, to a cluster of up to 8 blocks that join their sums through distributed
-// shared memory.
+// Two kernels.  With a gradient, and rows that 8 blocks hold, the row stays on
+// chip (distill_resident_kernel below).  The loss alone, longer rows, and a
+// gradient whose alignment differs from z's take distill_row_kernel: one sweep
+// reads the row for its running maximum and exponential sums (one sum for each
+// of the temperatures tau and 1 that the loss needs), a second one writes the
+// gradient from the row in L2 or L1.  In both the few entries of the teacher and
+// the label are then corrected in place, each from z again, so that every value
+// is rounded once.  A row belongs to a block, or to a cluster of up to 8 blocks
+// that join their sums through distributed shared memory.
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "rows.cuh"
+#include "sm100.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -51,6 +55,56 @@ __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// Two fp32 values in one register pair: one instruction for both.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v));
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
+__device__ __forceinline__ Pair exp2_fast(Pair x) {
+  float a, b;
+  unpair(x, a, b);
+  return pair(exp2_fast(a), exp2_fast(b));
+}
+
+// Largest element of a chunk (NaN only where every element is).
+__device__ __forceinline__ float chunk_max(const RowChunk<float, 4> &k) {
+  return fmaxf(fmaxf(k.raw.x, k.raw.y), fmaxf(k.raw.z, k.raw.w));
+}
+__device__ __forceinline__ float chunk_max(const RowChunk<__nv_bfloat16, 8> &k) {
+  const __nv_bfloat162 *w = reinterpret_cast<const __nv_bfloat162 *>(&k.raw);
+  const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+
+// Maximum over a warp (a NaN is passed over).
+__device__ __forceinline__ float warp_max(float v) {
+  float m;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
 }
 
 // Running maximum m and sums of exp((z - m) / tau), exp(z - m).
@@ -232,7 +286,9 @@ __global__ void distill_row_kernel(const DistillArgs a) {
   float scale = 1.f;
   if (a.counts) {
     int n = 0;
-    for (int i = 0; i < a.n_counts; ++i) n += a.counts[i];
+    for (int i = tid & 31; i < a.n_counts; i += 32) n += a.counts[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
     scale = 1.f / (float)(n > 0 ? n : 1);
   }
   if (a.upstream) scale *= a.upstream[a.upstream_rows ? row : 0];
@@ -305,19 +361,460 @@ __global__ void distill_row_kernel(const DistillArgs a) {
   if (has_l && label >= lo && label < hi && tid == nt - 1) corrected(label);
 }
 
+// ---------------------------------------------------------------- loss and gradient, row on chip
+// First, a warp a row, the teacher's side: the softmax p of the entries, an index named twice
+// merged into its first place, the sums that the loss needs, and how many rows count.
+constexpr int kEntries = 256;          // most entries of a row here; more take the other kernel
+constexpr int kPrepareThreads = 256;
+constexpr int kHasTeacher = 1, kHasLabel = 2, kBad = 4;
+
+struct alignas(16) Entry {
+  int index;  // -1: nothing to do
+  float p, z;
+};
+struct RowInfo {
+  float plogp, pz;  // sum p log p, sum p z
+  float z_label;
+  int flags;
+};
+
+// NQ: entries of a lane.
+template <typename T, int NQ>
+__global__ void __launch_bounds__(kPrepareThreads)
+distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *counts,
+                       unsigned *done) {
+  __shared__ int warp_counts[kPrepareThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, top = (int)a.top;
+  const float kt = kLog2e / a.tau;
+  const bool use_kl = a.alpha != 0.f, use_ce = a.labels != nullptr && a.alpha != 1.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *done = 0;
+  int counted = 0;
+  for (int64_t row = (int64_t)blockIdx.x * (kPrepareThreads / 32) + warp; row < a.rows;
+       row += (int64_t)gridDim.x * (kPrepareThreads / 32)) {
+    const T *z = reinterpret_cast<const T *>(a.z) + row * a.classes;
+    const int64_t label = a.labels ? a.labels[row] : -1;
+    int index[NQ];
+    float t[NQ], zq[NQ];
+    int flags = 0;
+    float m = kLowest;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      index[q] = -1, t[q] = 0.f, zq[q] = 0.f;
+      if (q * 32 + lane >= top) continue;
+      const int64_t ix = a.index[row * a.top + q * 32 + lane];
+      t[q] = a.teacher[row * a.top + q * 32 + lane];
+      if (ix < 0 || t[q] == -INFINITY) continue;
+      flags |= kHasTeacher;
+      if (ix >= a.classes) {
+        flags |= kBad;
+        continue;
+      }
+      index[q] = (int)ix;
+      zq[q] = load_f(z, ix);
+      m = fmaxf(m, t[q]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+      flags |= __shfl_xor_sync(0xFFFFFFFFu, flags, o);
+    }
+    if (label >= 0) flags |= kHasLabel;
+    counted += flags != 0;
+    if (!use_kl) flags &= ~(kHasTeacher | kBad);
+    if (!use_ce) flags &= ~kHasLabel;
+    if (use_ce && label >= a.classes) flags |= kBad;
+    float w[NQ], s = 0.f;
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      w[q] = index[q] < 0 ? 0.f : exp2f((t[q] - m) * kt);
+      s += w[q];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    const float log_s = logf(s);
+    float plogp = 0.f, pz = 0.f, merged[NQ];
+    bool later[NQ];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      w[q] = index[q] < 0 ? 0.f : w[q] / s;
+      if (w[q] != 0.f) {
+        plogp = fmaf(w[q], (t[q] - m) / a.tau - log_s, plogp);
+        pz = fmaf(w[q], zq[q], pz);
+      }
+      merged[q] = 0.f, later[q] = false;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      plogp += __shfl_xor_sync(0xFFFFFFFFu, plogp, o);
+      pz += __shfl_xor_sync(0xFFFFFFFFu, pz, o);
+    }
+    float p_label = 0.f;
+#pragma unroll
+    for (int src = 0; src < NQ; ++src) {
+      if (src * 32 >= top) break;
+      const int named = min(32, top - src * 32);
+      for (int l = 0; l < named; ++l) {
+        const int ix = __shfl_sync(0xFFFFFFFFu, index[src], l);
+        const float p = __shfl_sync(0xFFFFFFFFu, w[src], l);
+        p_label += ix >= 0 && ix == label ? p : 0.f;
+#pragma unroll
+        for (int q = 0; q < NQ; ++q) {  // places without an entry have p 0
+          merged[q] += index[q] == ix ? p : 0.f;
+          later[q] |= index[q] == ix && src * 32 + l < q * 32 + lane;
+        }
+      }
+    }
+    const bool teach = (flags & kHasTeacher) != 0, lab = (flags & kHasLabel) != 0;
+    Entry *out = entries + row * (a.top + 1);
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      if (q * 32 + lane >= top) continue;
+      // the label's place carries its own entry
+      const bool dead = !teach || index[q] < 0 || later[q] || (lab && index[q] == label);
+      out[q * 32 + lane] = Entry{dead ? -1 : index[q], merged[q], zq[q]};
+    }
+    if (lane == 0) {
+      const bool in = lab && label < a.classes;
+      const float zl = in ? load_f(z, label) : 0.f;
+      out[top] = Entry{in ? (int)label : -1, teach ? p_label : 0.f, zl};
+      info[row] = RowInfo{plogp, pz, zl, flags};
+    }
+  }
+  if (lane == 0) warp_counts[warp] = counted;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int n = 0;
+    for (int i = 0; i < kPrepareThreads / 32; ++i) n += warp_counts[i];
+    counts[blockIdx.x] = n;
+  }
+}
+
+// Then the row.  A persistent cluster of 1 to 8 blocks takes one at a time.  A thread holds up to
+// kResident chunks of 16 bytes of it and their exponentials in registers, both relative to the
+// largest of its own elements, so that z is read once and each exponential is computed once:
+//   dz = [at e^((m_t - m) / tau)] e^((z - m_t) / tau) + [a1 e^(m_t - m)] e^(z - m_t).
+// The next row is brought to L2 meanwhile.  The warps' maxima and sums are joined over the
+// cluster: each warp stores its own into every block's shared memory (st.async, two sets in turn)
+// and every block waits for all of them on an mbarrier of its own.  A cluster barrier in its place
+// also waited for the block's gradient stores.
+// An entry is handed to the thread that holds its element (a list a thread in shared memory),
+// which writes the corrected value over its own store: no second barrier.
+// The exponentials take 64 registers a thread, 128 with the rest, so 512 threads fill an SM.  The
+// joins leave a block idle for about half of a row's time: four blocks of 128 threads on an SM and
+// clusters of 8 took 339 us for 8192 rows of 32768 bf16 classes (two temperatures), two of 256 and
+// clusters of 4 398 us, five of 128 (96 registers, some spilled) 359 us.  Blocks of 512 serve the
+// rows that 8 of 128 do not hold.  Bound by instructions and the join's latency (0.53 instructions
+// a clock and scheduler), at 0.49 of the measured HBM rate.
+constexpr int kResident = 4;
+constexpr int kSmallThreads = 128, kSmallBlocks = 4;
+constexpr int kLargeThreads = 512;
+constexpr int kResidentParts = 8;
+
+struct HeldRow {
+  RowStats stats;
+  RowInfo info;
+  int64_t row;
+  bool bad;
+};
+
+struct ResidentArgs {
+  DistillArgs d;
+  const Entry *entries;
+  const RowInfo *info;
+  unsigned *done;
+  float *total;  // the reduced loss, or null
+  int divide;    // by the count
+};
+
+template <typename T, bool TWO, bool ALIGNED, int MAXT>
+__global__ void __launch_bounds__(MAXT, MAXT == kSmallThreads ? kSmallBlocks : 1)
+distill_resident_kernel(const ResidentArgs ra) {
+  constexpr int VEC = vec_of<T>(), NV = kResident;
+  const DistillArgs &a = ra.d;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  __shared__ float4 stats[2][kResidentParts * MAXT / 32];  // m, sum tau, sum 1
+  __shared__ uint64_t joined[2];
+  __shared__ int head[2][MAXT];   // a thread's first entry, or -1
+  __shared__ int next[2][kEntries + 1];
+  __shared__ Entry mine[2][kEntries + 1];
+  __shared__ HeldRow held_set[32];
+  __shared__ double loss_sums[MAXT / 32];
+  __shared__ int last;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  const float kt = kLog2e / a.tau, inv_tau = 1.f / a.tau;
+  const T *zb = reinterpret_cast<const T *>(a.z);
+  T *db = reinterpret_cast<T *>(a.dz);
+  const int classes = (int)a.classes, slots = (int)a.top + 1;
+  head[0][tid] = head[1][tid] = -1;
+  if (tid < 2) sm100::mbar_init(joined + tid, warps);
+  sm100::fence_barrier_init();
+  bool failed = false;  // a wait gave up: NaN from then on
+
+  int count = 0;
+  for (int i = lane; i < a.n_counts; i += 32) count += a.counts[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) count += __shfl_xor_sync(0xFFFFFFFFu, count, o);
+  float unit = ra.divide ? 1.f / (float)(count > 0 ? count : 1) : 1.f;
+  if (a.upstream && !a.upstream_rows) unit *= a.upstream[0];
+
+  // Chunk c of a row covers elements [c VEC - shift, (c + 1) VEC - shift): 16-byte aligned in z
+  // (and in dz, which the launch requires); the row's first and last may be cut.
+  const int chunk0 = part * nt * NV + tid;
+  auto shift_of = [&](int64_t row) {
+    return ALIGNED ? 0
+                   : (int)((reinterpret_cast<uintptr_t>(zb + row * a.classes) & 15) / sizeof(T));
+  };
+  RowChunk<T, VEC> cur[NV];
+  auto load_row = [&](RowChunk<T, VEC>(&k)[NV], int64_t row) {
+    const T *z = zb + row * a.classes;
+    const int shift = shift_of(row);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = (chunk0 + j * nt) * VEC - shift;
+      if (e0 >= 0 && e0 + VEC <= classes) {
+        k[j].load(z + e0);
+      } else {
+        float v[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          v[i] = !ALIGNED && e0 + i >= 0 && e0 + i < classes ? load_f(z, e0 + i) : -INFINITY;
+        k[j].put(v);
+      }
+    }
+  };
+
+  if (parts > 1)
+    cluster.sync();  // every block of the cluster runs before one writes to it
+  else
+    __syncthreads();
+  const int64_t first = blockIdx.x / parts, step = gridDim.x / parts;
+  // Losses wait until warp 0 of the first block has 32 rows, one a lane: their logarithms, taken a
+  // row at a time, made the other warps wait.
+  int held_rows = 0;
+  auto flush = [&]() {
+    __syncwarp();
+    if (a.loss && part == 0 && warp == 0 && lane < held_rows) {
+      const HeldRow held = held_set[lane];
+      const RowStats &s = held.stats;
+      const float s_one = TWO ? s.s1 : s.st;
+      float loss = 0.f;
+      if (held.info.flags & kHasTeacher) {
+        // sum p (log p - log q), log q = (z - m) / tau - log S
+        const float plogq = (held.info.pz - s.m) * inv_tau - logf(s.st);
+        loss = a.alpha * a.tau * a.tau * (s.st == 0.f ? INFINITY : held.info.plogp - plogq);
+      }
+      if (held.info.flags & kHasLabel)
+        loss += (1.f - a.alpha) * (held.info.z_label == -INFINITY
+                                       ? INFINITY
+                                       : logf(s_one) + (s.m - held.info.z_label));
+      a.loss[held.row] = held.bad ? NAN : loss;
+    }
+    __syncwarp();
+    held_rows = 0;
+  };
+  int set = 0;
+  uint32_t phase = 0;
+  for (int64_t row = first; row < a.rows; row += step, phase ^= set, set ^= 1) {
+    T *dz = db + row * a.classes;
+    const Entry *entries = ra.entries + row * slots;
+    Entry e = tid < slots ? entries[tid] : Entry{-1, 0.f, 0.f};
+    const RowInfo info = ra.info[row];
+    load_row(cur, row);
+    if (tid == 0 && row + step < a.rows) {  // whole chunks only: the copy's unit is 16 bytes
+      const T *next_row = zb + (row + step) * a.classes;
+      const int cut = shift_of(row + step);
+      const int c0 = part == 0 && cut ? 1 : part * nt * NV;
+      const int c1 = min(part * nt * NV + nt * NV, (classes + cut) / VEC);
+      if (c1 > c0) sm100::bulk_prefetch_l2(next_row + c0 * VEC - cut, (uint32_t)(c1 - c0) * 16);
+    }
+
+    // ---- exponentials relative to the thread's largest element
+    Pair et[NV][VEC / 2], e1[TWO ? NV : 1][VEC / 2];
+    RowStats st{kLowest, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) st.m = fmaxf(st.m, chunk_max(cur[j]));
+    const float m_own = st.m;
+    {
+      const Pair minus = pair(-st.m, -st.m), k2 = pair(kt, kt), l2 = pair(kLog2e, kLog2e);
+      Pair sum_t = pair(0.f, 0.f), sum_1 = sum_t;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float v[VEC];
+        cur[j].get(v);
+#pragma unroll
+        for (int i = 0; i < VEC / 2; ++i) {
+          const Pair d = pair(v[2 * i], v[2 * i + 1]) + minus;
+          et[j][i] = exp2_fast(d * k2);
+          sum_t = sum_t + et[j][i];
+          if (TWO) {
+            e1[j][i] = exp2_fast(d * l2);
+            sum_1 = sum_1 + e1[j][i];
+          }
+        }
+      }
+      float x, y;
+      unpair(sum_t, x, y);
+      st.st = x + y;
+      unpair(sum_1, x, y);
+      st.s1 = x + y;
+    }
+
+    // ---- entries of this block's classes, to the threads that hold them
+    const int shift = shift_of(row);
+    const int lo = part * nt * NV * VEC - shift, hi = lo + nt * NV * VEC;
+    for (int j = tid; j < slots; j += nt) {
+      if (j != tid) e = entries[j];
+      if (e.index >= 0 && e.index >= lo && e.index < hi) {
+        mine[set][j] = e;
+        next[set][j] = atomicExch(&head[set][((e.index - lo) / VEC) & (nt - 1)], j);
+      }
+    }
+
+    // ---- sums joined over warps and blocks
+    {
+      const float m = warp_max(st.m);
+      st.st *= exp2_fast((st.m - m) * kt);
+      if (TWO) st.s1 *= exp2_fast((st.m - m) * kLog2e);
+      st.m = m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        st.st += __shfl_xor_sync(0xFFFFFFFFu, st.st, o);
+        if (TWO) st.s1 += __shfl_xor_sync(0xFFFFFFFFu, st.s1, o);
+      }
+      if (parts == 1) {
+        if (lane == 0) stats[set][warp] = make_float4(st.m, st.st, st.s1, 0.f);
+        __syncthreads();
+      } else {
+        __syncwarp();  // the warp's entries are listed before its arrival
+        if (lane < parts)
+          sm100::store_async_rank(&stats[set][part * warps + warp], joined + set, lane, st.m,
+                                  st.st, st.s1, 0.f);
+        if (lane == 0) {
+          if (warp == 0)
+            sm100::mbar_arrive_expect_tx(joined + set, (uint32_t)(parts * warps * sizeof(float4)));
+          else
+            sm100::mbar_arrive(joined + set);
+        }
+        if (!failed) failed = !sm100::mbar_wait_cluster_bounded(joined + set, phase, 1000000u);
+      }
+    }
+    {
+      const int n = parts * warps;
+      RowStats own{kLowest, 0.f, 0.f};
+      if (lane < n) {
+        const float4 b = stats[set][lane];
+        own = RowStats{b.x, b.y, b.z};
+      }
+      for (int i = lane + 32; i < n; i += 32) {
+        const float4 b = stats[set][i];
+        stats_join<TWO>(own, RowStats{b.x, b.y, b.z}, kt);
+      }
+      const float m = warp_max(own.m);
+      st.st = own.st * exp2_fast((own.m - m) * kt);
+      if (TWO) st.s1 = own.s1 * exp2_fast((own.m - m) * kLog2e);
+      st.m = m;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        st.st += __shfl_xor_sync(0xFFFFFFFFu, st.st, o);
+        if (TWO) st.s1 += __shfl_xor_sync(0xFFFFFFFFu, st.s1, o);
+      }
+    }
+    // a row that is -inf throughout: q = 0, log q = -inf
+    const float s_one = TWO ? st.s1 : st.st;
+    const float inv_t = st.st == 0.f ? 0.f : __fdividef(1.f, st.st);  // sums lie in [1, classes]
+    const float inv_1 = s_one == 0.f ? 0.f : __fdividef(1.f, s_one);
+    const bool has_t = (info.flags & kHasTeacher) != 0, has_l = (info.flags & kHasLabel) != 0;
+    const bool bad = (info.flags & kBad) != 0 || failed;
+    if (tid == 0) held_set[held_rows] = HeldRow{st, info, row, bad};
+    if (++held_rows == 32) flush();
+
+    // ---- the gradient
+    float scale = a.upstream_rows && a.upstream ? unit * a.upstream[row] : unit;
+    if (bad) scale = NAN;
+    const float ct = has_t || bad ? a.alpha * a.tau * scale : 0.f;
+    const float c1 = has_l ? (1.f - a.alpha) * scale : 0.f;
+    float at = ct * inv_t, a1 = c1 * inv_1;
+    if (!TWO) at += a1;
+    const float ft = at * exp2_fast((m_own - st.m) * kt);
+    const float f1 = TWO ? a1 * exp2_fast((m_own - st.m) * kLog2e) : 0.f;
+    const Pair ft2 = pair(ft, ft), f12 = pair(f1, f1);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = (chunk0 + j * nt) * VEC - shift;
+      float v[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC / 2; ++i) {
+        Pair g = ft2 * et[j][i];
+        if (TWO) g = fma(f12, e1[j][i], g);
+        unpair(g, v[2 * i], v[2 * i + 1]);
+      }
+      if (e0 >= 0 && e0 + VEC <= classes) {
+        RowChunk<T, VEC> k;
+        k.put(v);
+        k.store(dz + e0);
+      } else if (!ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (e0 + i >= 0 && e0 + i < classes) store_f(dz, e0 + i, v[i]);
+      }
+    }
+    int j = head[set][tid];
+    if (j >= 0) {
+      head[set][tid] = -1;
+      if (!bad)
+        for (; j >= 0; j = next[set][j]) {
+          const Entry own = mine[set][j];
+          const float d = own.z - st.m;
+          float g = at * exp2_fast(d * kt);
+          if (TWO) g = fmaf(a1, exp2_fast(d * kLog2e), g);
+          g -= ct * own.p;
+          if (j == slots - 1) g -= c1;
+          store_f(dz, own.index, g);
+        }
+    }
+  }
+
+  flush();
+
+  // ---- the last block to finish adds the rows' losses, in a fixed order
+  if (ra.total) {
+    if (part == 0 && warp == 0) __threadfence();
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      last = atomicAdd(ra.done, 1u) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      double s = 0.0;
+      for (int64_t i = tid; i < a.rows; i += nt) s += (double)__ldcg(a.loss + i);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+      if (lane == 0) loss_sums[warp] = s;
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 1; w < warps; ++w) s += loss_sums[w];
+        *ra.total = (float)(ra.divide ? s / (double)(count > 0 ? count : 1) : s);
+      }
+    }
+  }
+  if (parts > 1) cluster.sync();  // no block leaves while another writes its sums here
+}
+
 // How many rows count: those with an entry of the teacher or a label (a warp a row).
 __global__ void __launch_bounds__(kCountThreads)
 distill_count_kernel(const int64_t *index, const float *teacher, const int64_t *labels,
-                     int64_t rows, int64_t top, int use_kl, int *counts) {
+                     int64_t rows, int64_t top, int *counts) {
   __shared__ int warp_counts[kCountThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int n = 0;
   for (int64_t row = (int64_t)blockIdx.x * (kCountThreads / 32) + warp; row < rows;
        row += (int64_t)gridDim.x * (kCountThreads / 32)) {
     bool any = labels && labels[row] >= 0;
-    if (use_kl)
-      for (int64_t j = lane; j < top && !any; j += 32)
-        any = index[row * top + j] >= 0 && teacher[row * top + j] != -INFINITY;
+    for (int64_t j = lane; j < top && !any; j += 32)
+      any = index[row * top + j] >= 0 && teacher[row * top + j] != -INFINITY;
     n += __any_sync(0xFFFFFFFFu, any) ? 1 : 0;
   }
   if (lane == 0) warp_counts[warp] = n;
@@ -387,24 +884,115 @@ int check_distill(const char *what, const lnet_b200_distill_request *q) {
 }
 
 int count_blocks(int64_t rows) {
-  return (int)std::min<int64_t>(cdiv(rows, kCountThreads / 32), 128);
+  return (int)std::min<int64_t>(cdiv(rows, kCountThreads / 32), 1024);
 }
 
 struct DistillWork {
   int *counts;
+  unsigned *done;
   float *row_loss;
+  Entry *entries;
+  RowInfo *info;
 };
 
 DistillWork distill_work(Arena &ar, const lnet_b200_distill_request *q) {
   DistillWork w{};
-  w.counts = ar.take<int>(count_blocks(std::max<int64_t>(q->rows, 1)));
-  w.row_loss = ar.take<float>(q->reduction == 0 ? 0 : q->rows);
+  const int64_t rows = std::max<int64_t>(q->rows, 1);
+  w.counts = ar.take<int>(count_blocks(rows));
+  w.done = ar.take<unsigned>(1);
+  w.row_loss = ar.take<float>(q->reduction == 0 ? 0 : rows);
+  if (q->top <= kEntries) {
+    w.entries = ar.take<Entry>(rows * (q->top + 1));
+    w.info = ar.take<RowInfo>(rows);
+  }
   return w;
+}
+
+// Where the resident kernel serves a request: threads and blocks of a cluster.
+struct ResidentPlan {
+  int threads, parts;
+  bool aligned;
+};
+
+template <typename T>
+bool resident_plan(const lnet_b200_distill_request *q, const void *dz, ResidentPlan &p) {
+  constexpr int VEC = vec_of<T>();
+  const uintptr_t zp = reinterpret_cast<uintptr_t>(q->logits), gp = reinterpret_cast<uintptr_t>(dz);
+  if (!dz || ((zp ^ gp) & 15) || q->top > kEntries) return false;
+  p.aligned = zp % 16 == 0 && q->classes % VEC == 0;
+  // one chunk more where a row may start inside a chunk
+  const int64_t chunks = cdiv(q->classes, VEC) + (p.aligned ? 0 : 1);
+  // The smallest blocks that 8 of hold the row: 64 or 128 threads, then 256 or 512.
+  p.threads = 64, p.parts = 1;
+  auto holds = [&] { return chunks <= (int64_t)p.parts * p.threads * kResident; };
+  while (p.threads < kSmallThreads && !holds()) p.threads *= 2;
+  while (p.parts < kResidentParts && !holds()) p.parts *= 2;
+  while (p.threads < kLargeThreads && !holds()) p.threads *= 2;
+  return holds();
+}
+
+template <typename T, bool TWO, bool ALIGNED, int MAXT>
+int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
+  auto *kernel = distill_resident_kernel<T, TWO, ALIGNED, MAXT>;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = p.parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.stream = s;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cfg.blockDim = dim3(p.threads);
+  cfg.gridDim = dim3(p.parts);
+  // Clusters that run at once: fewer than SMs / parts, since a cluster stays inside one group of
+  // SMs.  A waiting cluster would double the time of a persistent grid.
+  int clusters = 0;
+  if (p.parts == 1)
+    clusters = sm_count() * (MAXT == kSmallThreads ? kSmallBlocks * kSmallThreads : MAXT) / p.threads;
+  else
+    LNET_TRY(cuda_check(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg),
+                        "distill_resident_kernel occupancy"));
+  clusters = (int)std::max<int64_t>(1, std::min<int64_t>(a.d.rows, clusters));
+  cfg.gridDim = dim3((unsigned)(clusters * p.parts));
+  LNET_TRY(cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "distill_resident_kernel"));
+  return after_launch("distill_resident_kernel");
+}
+
+bool two_temperatures(const DistillArgs &a) {
+  return a.alpha != 0.f && a.labels && a.alpha != 1.f && a.tau != 1.f;
+}
+
+template <typename T>
+int launch_prepare(const DistillArgs &a, const DistillWork &w, int blocks, cudaStream_t s) {
+  if (a.top <= 32)
+    distill_prepare_kernel<T, 1><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
+                                                                    w.done);
+  else if (a.top <= 64)
+    distill_prepare_kernel<T, 2><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
+                                                                    w.done);
+  else
+    distill_prepare_kernel<T, kEntries / 32><<<blocks, kPrepareThreads, 0, s>>>(
+        a, w.entries, w.info, w.counts, w.done);
+  return after_launch("distill_prepare_kernel");
+}
+
+template <typename T>
+int launch_resident(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
+  auto sized = [&](auto two, auto aligned) {
+    constexpr bool TWO = decltype(two)::value, ALIGNED = decltype(aligned)::value;
+    return p.threads <= kSmallThreads
+               ? launch_resident_typed<T, TWO, ALIGNED, kSmallThreads>(p, a, s)
+               : launch_resident_typed<T, TWO, ALIGNED, kLargeThreads>(p, a, s);
+  };
+  if (two_temperatures(a.d))
+    return p.aligned ? sized(std::true_type{}, std::true_type{})
+                     : sized(std::true_type{}, std::false_type{});
+  return p.aligned ? sized(std::false_type{}, std::true_type{})
+                   : sized(std::false_type{}, std::false_type{});
 }
 
 template <typename T>
 int launch_rows(const lnet_b200_distill_request *q, const DistillArgs &a, cudaStream_t s) {
-  const bool two = a.alpha != 0.f && a.labels && a.alpha != 1.f && a.tau != 1.f;
   // Threads: 4 chunks of 16 bytes each, 64 to 512.
   const int64_t chunks = cdiv(q->classes, vec_of<T>());
   const int threads = (int)std::min<int64_t>(512, std::max<int64_t>(64, cdiv(chunks, 4 * 32) * 32));
@@ -413,16 +1001,17 @@ int launch_rows(const lnet_b200_distill_request *q, const DistillArgs &a, cudaSt
   while (parts < 8 && q->rows * parts * 2 <= 2 * sm_count() && chunks / (parts * 2) >= 4 * threads)
     parts *= 2;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(q->rows * parts));
-  cfg.blockDim = dim3(threads);
-  cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = parts;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.stream = s;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t err = two ? cudaLaunchKernelEx(&cfg, distill_row_kernel<T, true>, a)
+  cfg.gridDim = dim3((unsigned)(q->rows * parts));
+  cfg.blockDim = dim3(threads);
+  const cudaError_t err = two_temperatures(a)
+                              ? cudaLaunchKernelEx(&cfg, distill_row_kernel<T, true>, a)
                               : cudaLaunchKernelEx(&cfg, distill_row_kernel<T, false>, a);
   LNET_TRY(cuda_check(err, "distill_row_kernel"));
   return after_launch("distill_row_kernel");
@@ -446,26 +1035,35 @@ int run_distill(const char *what, const lnet_b200_distill_request *q, void *work
   }
   // labels without weight still make their rows count
   const bool mean = q->reduction == 2;
-  const int n_counts = mean ? count_blocks(q->rows) : 0;
-  if (mean) {
-    distill_count_kernel<<<n_counts, kCountThreads, 0, stream>>>(
-        q->teacher_indices, q->teacher_logits, q->labels, q->rows, q->top, 1, w.counts);
-    LNET_TRY(after_launch("distill_count_kernel"));
-  }
+  const int n_counts = count_blocks(q->rows);
   DistillArgs a{};
   a.z = q->logits;
   a.index = q->teacher_indices, a.teacher = q->teacher_logits, a.labels = q->labels;
-  a.counts = mean ? w.counts : nullptr, a.n_counts = n_counts;
   a.upstream = upstream, a.upstream_rows = reduce ? 0 : 1;
   a.loss = loss ? (reduce ? w.row_loss : loss) : nullptr;
   a.dz = dz;
   a.rows = q->rows, a.classes = q->classes, a.top = q->top;
   a.alpha = q->alpha;
   a.tau = a.alpha == 0.f ? 1.f : q->temperature;  // without the teacher only softmax(z) is needed
-  LNET_TRY(q->dtype == LNET_BF16 ? launch_rows<__nv_bfloat16>(q, a, stream)
-                                 : launch_rows<float>(q, a, stream));
+  const bool bf16 = q->dtype == LNET_BF16;
+  ResidentPlan plan{};
+  if (bf16 ? resident_plan<__nv_bfloat16>(q, dz, plan) : resident_plan<float>(q, dz, plan)) {
+    LNET_TRY(bf16 ? launch_prepare<__nv_bfloat16>(a, w, n_counts, stream)
+                  : launch_prepare<float>(a, w, n_counts, stream));
+    a.counts = w.counts, a.n_counts = n_counts;
+    const ResidentArgs ra{a, w.entries, w.info, w.done, loss && reduce ? loss : nullptr, mean};
+    return bf16 ? launch_resident<__nv_bfloat16>(plan, ra, stream)
+                : launch_resident<float>(plan, ra, stream);
+  }
+  if (mean) {
+    distill_count_kernel<<<n_counts, kCountThreads, 0, stream>>>(
+        q->teacher_indices, q->teacher_logits, q->labels, q->rows, q->top, w.counts);
+    LNET_TRY(after_launch("distill_count_kernel"));
+    a.counts = w.counts, a.n_counts = n_counts;
+  }
+  LNET_TRY(bf16 ? launch_rows<__nv_bfloat16>(q, a, stream) : launch_rows<float>(q, a, stream));
   if (loss && reduce) {
-    distill_sum_kernel<<<1, kSumThreads, 0, stream>>>(w.row_loss, q->rows, a.counts, n_counts,
+    distill_sum_kernel<<<1, kSumThreads, 0, stream>>>(w.row_loss, q->rows, a.counts, a.n_counts,
                                                       loss);
     LNET_TRY(after_launch("distill_sum_kernel"));
   }

@@ -40,21 +40,55 @@ __device__ __forceinline__ float weight_at(const void *w, bool w_bf16, int64_t i
                 : __ldg(reinterpret_cast<const float *>(w) + i);
 }
 
+// VEC weights from column c * VEC on, in fp32 (16-byte loads where the plan is vectorised).
+template <int VEC>
+__device__ __forceinline__ void weight_chunk(const void *w, bool w_bf16, int c, float *v) {
+  if (VEC == 1) {
+    v[0] = weight_at(w, w_bf16, c);
+  } else if (w_bf16) {
+    const uint16_t *p = reinterpret_cast<const uint16_t *>(w) + c * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p) + i);
+      v[4 * i] = __uint_as_float(u.x << 16);
+      v[4 * i + 1] = __uint_as_float(u.x & 0xFFFF0000u);
+      v[4 * i + 2] = __uint_as_float(u.y << 16);
+      v[4 * i + 3] = __uint_as_float(u.y & 0xFFFF0000u);
+    }
+  } else {
+    const float *p = reinterpret_cast<const float *>(w) + c * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 u = __ldg(reinterpret_cast<const float4 *>(p) + i);
+      v[4 * i] = u.x, v[4 * i + 1] = u.y, v[4 * i + 2] = u.z, v[4 * i + 3] = u.w;
+    }
+  }
+}
+
 // q = e4m3(y / s), saturating; s = 0 means that the row is zero.
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
+// The quotient is taken as a product with 1 / s where that is a normal number: two roundings of
+// fp32, 2^-20 of a code's step, so a code differs only where y / s lies that near to a tie.
 template <int VEC>
 __device__ __forceinline__ void store_e4m3(uint8_t *p, const float *v, float s) {
-  const float d = s == 0.f ? 1.f : s;
+  float d[VEC];
+  if (s == 0.f || s > 1e-30f) {
+    const float inv = s == 0.f ? 1.f : 1.f / s;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) d[i] = v[i] * inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) d[i] = v[i] / s;
+  }
   if (VEC == 1) {
-    *p = (uint8_t)(e4m3_pair(v[0] / d, 0.f) & 0xFF);
+    *p = (uint8_t)(e4m3_pair(d[0], 0.f) & 0xFF);
   } else {
     uint32_t w[VEC >= 4 ? VEC / 4 : 1];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
-      w[i] = e4m3_pair(v[4 * i] / d, v[4 * i + 1] / d) |
-             (e4m3_pair(v[4 * i + 2] / d, v[4 * i + 3] / d) << 16);
+      w[i] = e4m3_pair(d[4 * i], d[4 * i + 1]) | (e4m3_pair(d[4 * i + 2], d[4 * i + 3]) << 16);
     if (VEC == 8)
       *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[VEC == 8 ? 1 : 0]);
     else
@@ -81,6 +115,12 @@ norm_forward_kernel(const NormArgs a) {
   const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
   const int nvec = (int)(a.dim / VEC);
   const T *x = reinterpret_cast<const T *>(a.x), *r = reinterpret_cast<const T *>(a.r);
+  float w[NV][VEC];  // a thread's columns are the same in every row
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = lane + j * g;
+    if (c < nvec) weight_chunk<VEC>(a.w, a.w_bf16, c, w[j]);
+  }
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
        base += (int64_t)gridDim.x * per) {
     const int64_t row = base + sub;
@@ -132,8 +172,7 @@ norm_forward_kernel(const NormArgs a) {
         cx[j].get(v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
-          amax = MaxNanOp::of(
-              amax, fabsf(v[i] * rstd * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i)));
+          amax = MaxNanOp::of(amax, fabsf(v[i] * rstd * w[j][i]));
       }
       amax = group_reduce<G, MaxNanOp>(amax, scratch);
       scale = amax / kE4m3Max;
@@ -146,7 +185,7 @@ norm_forward_kernel(const NormArgs a) {
       float v[VEC];
       cx[j].get(v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] *= rstd * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i);
+      for (int i = 0; i < VEC; ++i) v[i] = v[i] * rstd * w[j][i];
       if (FP8) {
         store_e4m3<VEC>(a.q + off + (int64_t)c * VEC, v, scale);
       } else {
@@ -190,7 +229,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
       if (threadIdx.x == 0) a.scales[row] = scale;
     }
     for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
-      const float v = load_f(h, off + c) * (rstd * weight_at(a.w, a.w_bf16, c));
+      const float v = load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c);
       if (FP8)
         store_e4m3<1>(a.q + off + c, &v, scale);
       else
@@ -267,13 +306,14 @@ norm_backward_kernel(const NormGradArgs a) {
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       if (c >= nvec) continue;
-      float h[VEC], dy[VEC];
+      float h[VEC], dy[VEC], w[VEC];
       ch[j].get(h), cy[j].get(dy);
+      weight_chunk<VEC>(a.w, a.w_bf16, c, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         const float t = dy[i] * (h[i] * rstd);
         dw[j][i] += t;
-        dot = fmaf(t, weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i), dot);
+        dot = fmaf(t, w[i], dot);
       }
     }
     dot = group_reduce<G, SumOp>(dot, scratch);
@@ -282,13 +322,11 @@ norm_backward_kernel(const NormGradArgs a) {
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       if (!live || c >= nvec) continue;
-      float h[VEC], dy[VEC], s[VEC];
+      float h[VEC], dy[VEC], s[VEC], w[VEC];
       ch[j].get(h), cy[j].get(dy), cs[j].get(s);
+      weight_chunk<VEC>(a.w, a.w_bf16, c, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float gi = dy[i] * weight_at(a.w, a.w_bf16, (int64_t)c * VEC + i);
-        s[i] = fmaf(rstd, gi - h[i] * k, s[i]);
-      }
+      for (int i = 0; i < VEC; ++i) s[i] = fmaf(rstd, dy[i] * w[i] - h[i] * k, s[i]);
       cs[j].put(s);
       cs[j].store(reinterpret_cast<T *>(a.dx) + off + (int64_t)c * VEC);
     }
@@ -429,7 +467,7 @@ void launch_forward(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
 template <typename T, bool FP8>
 int forward_typed(const NormArgs &a, cudaStream_t s) {
   const bool aligned = aligned16(a.x) && aligned16(a.r) && aligned16(a.h) && aligned16(a.y) &&
-                       aligned16(a.q);
+                       aligned16(a.q) && aligned16(a.w);
   const NormPlan p = norm_plan(a.rows, a.dim, sizeof(T), aligned, kForwardBlocks);
   if (p.wide)
     norm_forward_wide_kernel<T, FP8><<<p.blocks, p.threads, 0, s>>>(a);
@@ -566,7 +604,8 @@ extern "C" int lnet_b200_residual_rms_norm_backward(
   }
   const int elem = dtype == LNET_BF16 ? 2 : 4;
   const bool aligned =
-      aligned16(stream_in) && aligned16(dy) && aligned16(dstream) && aligned16(dx);
+      aligned16(stream_in) && aligned16(dy) && aligned16(dstream) && aligned16(dx) &&
+      aligned16(weight);
   const NormPlan p = norm_plan(rows, dim, elem, aligned, kBackwardBlocks);
   const size_t need = dweight ? (size_t)p.blocks * (size_t)dim * sizeof(float) : 0;
   if (need > workspace_bytes || (need && !workspace))

@@ -350,6 +350,26 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+__device__ __forceinline__ bool mbar_wait_cluster_bounded(uint64_t *bar, uint32_t parity,
+                                                          uint32_t limit) {
+  for (uint32_t i = 0; i < limit; ++i)
+    if (mbar_try_wait_cluster(bar, parity, 1000u)) return true;
+  return false;
+}
+// Four floats into CTA `rank`'s copy of `dst` (16-byte aligned); completes 16 bytes on its copy of
+// `bar`.
+__device__ __forceinline__ void store_async_rank(void *dst, uint64_t *bar, uint32_t rank, float x,
+                                                 float y, float z, float w) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+      ::"r"(map_to_rank(dst, rank)),
+      "f"(x), "f"(y), "f"(z), "f"(w), "r"(map_to_rank(bar, rank))
+      : "memory");
+}
+// Brings `bytes` (a multiple of 16) from a 16-byte aligned address to L2.
+__device__ __forceinline__ void bulk_prefetch_l2(const void *src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(src), "r"(bytes) : "memory");
+}
 // 2-D tiled load into this CTA's shared memory; the barrier (an address in the
 // cluster's window) may be the pair's other CTA's where GROUP is 2.
 template <int GROUP>

@@ -4,20 +4,28 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _lib
+
+# The same values as torch.cuda.current_device() and torch.cuda.current_stream(i).cuda_stream,
+# without the 3 us that building a Stream object takes (a small kernel's own time).
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 DTYPES = {torch.float32: _lib.LNET_F32, torch.bfloat16: _lib.LNET_BF16}
 
 
 def call(device: torch.device, name: str, *args) -> None:
     """``name(*args, stream)`` with ``device`` current; raises on an error status."""
+    index = device.index
     fn = getattr(_lib.load(), name)
-    if torch.cuda.current_device() == device.index:
-        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if _current_device() == index:
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+            status = fn(*args, _raw_stream(index))
     if status:
         _lib.check(status, name)
 
@@ -32,4 +40,19 @@ def require_cuda(what: str, t: Tensor) -> None:
 
 
 def wants_grad(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def single_backward(fn):
+    """``once_differentiable`` for the passes that could be differentiated again
+    (``create_graph``), without its cost for all others."""
+    once = once_differentiable(fn)
+
+    def backward(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
+
+    return backward

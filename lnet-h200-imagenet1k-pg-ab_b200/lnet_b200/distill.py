@@ -10,13 +10,13 @@ pass over the student's logits.
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._launch import DTYPES, call, pointer, require_cuda, wants_grad
+from ._launch import DTYPES, call, pointer, require_cuda, single_backward, wants_grad
 
 REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 
@@ -58,6 +58,17 @@ def _check_distill_args(logits, teacher_indices, teacher_logits, labels, tempera
         raise ValueError(f"reduction must be one of {tuple(REDUCTIONS)}, got {reduction!r}")
 
 
+@lru_cache(maxsize=256)
+def _workspace_bytes(rows: int, top: int, reduction: int) -> int:
+    n = ctypes.c_size_t(0)
+    req = _lib.DistillRequest(rows=rows, classes=1, top=top, reduction=reduction, logits=1,
+                              teacher_indices=1, teacher_logits=1, temperature=1.0,
+                              alpha=1.0)  # the size depends on nothing else
+    _lib.check(_lib.load().lnet_b200_distill_workspace_size(ctypes.byref(req), ctypes.byref(n)),
+               "lnet_b200_distill_workspace_size")
+    return int(n.value)
+
+
 class _Request:
     """One call's request and workspace (the tensors are kept for its pointers)."""
 
@@ -70,15 +81,11 @@ class _Request:
             logits=logits.data_ptr(), teacher_indices=indices.data_ptr(),
             teacher_logits=teacher.data_ptr(), labels=pointer(labels), temperature=temperature,
             alpha=alpha)
-        n = ctypes.c_size_t(0)
-        _lib.check(_lib.load().lnet_b200_distill_workspace_size(ctypes.byref(self.req),
-                                                                ctypes.byref(n)),
-                   "lnet_b200_distill_workspace_size")
-        self.bytes = int(n.value)
 
     def run(self, name, *args):
-        ws = torch.empty(max(self.bytes, 1), dtype=torch.uint8, device=self.device)
-        call(self.device, name, ctypes.byref(self.req), ws.data_ptr(), self.bytes, *args)
+        nbytes = _workspace_bytes(self.req.rows, self.req.top, self.req.reduction)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        call(self.device, name, ctypes.byref(self.req), ws.data_ptr(), nbytes, *args)
 
 
 def _launch_distill(logits, indices, teacher, labels, temperature, alpha, reduction,
@@ -109,7 +116,7 @@ class _DistillationLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
+    @single_backward
     def backward(ctx, dloss):
         args = ctx.saved_tensors
         logits = args[0]

@@ -10,13 +10,13 @@ with its gradient, and its serving form on 8-bit operands
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._launch import DTYPES, call, pointer, require_cuda, wants_grad
+from ._launch import DTYPES, call, pointer, require_cuda, single_backward, wants_grad
 
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -55,41 +55,59 @@ def _request(x, weight, bias, residual, activation, x_scale=None,
         pointer(weight_scale))
 
 
+# Workspace sizes depend on the extents, the type and the alignment of the pointers alone.
+@lru_cache(maxsize=1024)
+def _forward_bytes(rows, inner, outer, dtype, x_align, w_align) -> int:
+    n = ctypes.c_size_t(0)
+    req = _lib.LinearRequest(rows, inner, outer, dtype, 0, 256 + x_align, 256 + w_align, None,
+                             None, 256, 256)
+    _lib.check(_lib.load().lnet_b200_linear_workspace_size(ctypes.byref(req), ctypes.byref(n)),
+               "lnet_b200_linear_workspace_size")
+    return int(n.value)
+
+
+@lru_cache(maxsize=1024)
+def _backward_bytes(rows, inner, outer, activation, x_align, w_align, pre_align, dy_align,
+                    want_dx, want_dw, want_db) -> int:
+    n = ctypes.c_size_t(0)
+    req = _lib.LinearRequest(rows, inner, outer, _lib.LNET_BF16, activation, 256 + x_align,
+                             256 + w_align)
+    _lib.check(_lib.load().lnet_b200_linear_backward_workspace_size(
+        ctypes.byref(req), 256 + pre_align if activation else None, 256 + dy_align, want_dx,
+        want_dw, want_db, ctypes.byref(n)), "lnet_b200_linear_backward_workspace_size")
+    return int(n.value)
+
+
 def _workspace(nbytes: int, device: torch.device) -> Tensor | None:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
 def _launch_linear(x, req, keep_preact: bool) -> tuple[Tensor, Tensor | None]:
     """(y, pre-activation or None) of a request of contiguous tensors."""
-    lib = _lib.load()
-    n = ctypes.c_size_t(0)
-    ref = ctypes.byref(req)
-    _lib.check(lib.lnet_b200_linear_workspace_size(ref, ctypes.byref(n)),
-               "lnet_b200_linear_workspace_size")
-    shape = (*x.shape[:-1], req.outer)
-    y = torch.empty(shape, dtype=torch.bfloat16, device=x.device)
+    device = x.device
+    nbytes = _forward_bytes(req.rows, req.inner, req.outer, req.dtype, (req.x or 0) & 15,
+                            req.weight & 15)
+    y = torch.empty((*x.shape[:-1], req.outer), dtype=torch.bfloat16, device=device)
     pre = torch.empty_like(y) if keep_preact else None
-    ws = _workspace(n.value, x.device)
-    call(x.device, "lnet_b200_linear_forward", ref, pointer(ws), n.value, y.data_ptr(),
+    ws = _workspace(nbytes, device)
+    call(device, "lnet_b200_linear_forward", ctypes.byref(req), pointer(ws), nbytes, y.data_ptr(),
          pointer(pre))
     return y, pre
 
 
 def _launch_linear_backward(x, weight, activation, pre, dy, want_dx, want_dw, want_db):
     """(dx, dweight, dbias), each None where it is not wanted."""
-    lib = _lib.load()
     req = _request(x, weight, None, None, activation)
-    n = ctypes.c_size_t(0)
-    ref = ctypes.byref(req)
-    _lib.check(lib.lnet_b200_linear_backward_workspace_size(
-        ref, pointer(pre), dy.data_ptr(), want_dx, want_dw, want_db, ctypes.byref(n)),
-        "lnet_b200_linear_backward_workspace_size")
+    pre_at, dy_at = pointer(pre), dy.data_ptr()
+    nbytes = _backward_bytes(req.rows, req.inner, req.outer, activation, (req.x or 0) & 15,
+                             req.weight & 15, (pre_at or 0) & 15, dy_at & 15, want_dx, want_dw,
+                             want_db)
     dx = torch.empty_like(x) if want_dx else None
     dw = torch.empty_like(weight) if want_dw else None
     db = torch.empty(req.outer, dtype=torch.bfloat16, device=x.device) if want_db else None
-    ws = _workspace(n.value, x.device)
-    call(x.device, "lnet_b200_linear_backward", ref, pointer(pre), dy.data_ptr(), pointer(ws),
-         n.value, pointer(dx), pointer(dw), pointer(db))
+    ws = _workspace(nbytes, x.device)
+    call(x.device, "lnet_b200_linear_backward", ctypes.byref(req), pre_at, dy_at, pointer(ws),
+         nbytes, pointer(dx), pointer(dw), pointer(db))
     return dx, dw, db
 
 
@@ -108,7 +126,7 @@ class _LinearAct(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @single_backward
     def backward(ctx, dy):
         x, weight, pre = ctx.saved_tensors
         need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad

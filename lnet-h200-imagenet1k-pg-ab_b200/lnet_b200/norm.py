@@ -14,10 +14,9 @@ from functools import lru_cache
 
 import torch
 from torch import Tensor
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from ._launch import DTYPES, call, pointer, require_cuda, wants_grad
+from ._launch import DTYPES, call, pointer, require_cuda, single_backward, wants_grad
 
 RMS_NORM_EPS = torch.finfo(torch.float32).eps  # nn.RMSNorm's default for fp32
 
@@ -97,7 +96,7 @@ class _ResidualRmsNorm(torch.autograd.Function):
         return y, x if stream is None else stream  # without a residual the stream is x itself
 
     @staticmethod
-    @once_differentiable
+    @single_backward
     def backward(ctx, dy, dstream):
         stream, weight, rstd = ctx.saved_tensors
         need_x, need_w, need_r, _ = ctx.needs_input_grad

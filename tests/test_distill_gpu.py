@@ -182,7 +182,7 @@ def test_rows_that_leave_nothing(cuda_device):
     z2 = z.detach().clone().requires_grad_()
     total = distillation_loss(z2, none, teacher)
     grad, = torch.autograd.grad(total, z2)
-    assert float(total) == 0 and bool((grad == 0).all())
+    assert float(total.detach()) == 0 and bool((grad == 0).all())
 
 
 def test_infinite_and_nan_logits(cuda_device):
