@@ -32,7 +32,6 @@ namespace cg = cooperative_groups;
 namespace lnet {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.402823466e+38f;
 constexpr int kCountThreads = 256;
 constexpr int kSumThreads = 1024;
@@ -49,46 +48,6 @@ struct DistillArgs {
   float tau, alpha;
   int n_counts, upstream_rows;
 };
-
-// ex2.approx (2 ulp), results below 2^-126 flushed to zero
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// Two fp32 values in one register pair: one instruction for both.
-struct Pair {
-  uint64_t v;
-};
-__device__ __forceinline__ Pair pair(float a, float b) {
-  Pair p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
-  return p;
-}
-__device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v));
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-  Pair p;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
-}
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-  Pair p;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
-  return p;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-  Pair p;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return p;
-}
-__device__ __forceinline__ Pair exp2_fast(Pair x) {
-  float a, b;
-  unpair(x, a, b);
-  return pair(exp2_fast(a), exp2_fast(b));
-}
 
 // Largest element of a chunk (NaN only where every element is).
 __device__ __forceinline__ float chunk_max(const RowChunk<float, 4> &k) {

@@ -14,6 +14,9 @@
 // bytes a clock, more than an SM's share of L2; the pair's 256 x 256 tile splits
 // B between the two SMs, 64 bytes a clock for the same work.
 //
+// A last wave that would leave SMs idle is split along k: those tiles' fp32 sums
+// go to memory and a second kernel joins them.
+//
 // Every wait is bounded: a role whose wait gives up marks the CTA as failed, all
 // roles leave their loops, and tiles that were not finished are written as NaN.
 #pragma once
@@ -21,7 +24,7 @@
 #include <cuda.h>
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "rows.cuh"
 #include "sm100.cuh"
 #include "tmap.cuh"
 
@@ -35,28 +38,95 @@ constexpr int kTileSmemLimit = 227 * 1024;
 
 enum LinearActivation { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
-// f(a); SiLU and GELU (0.5 a (1 + erf(a / sqrt 2))) in fp32.
-__device__ __forceinline__ float act_value(float a, int act) {
-  if (act == kActRelu) return a < 0.f ? 0.f : a;  // keeps NaN
-  if (act == kActSilu) return a / (1.f + __expf(-a));
-  if (act == kActGelu) return 0.5f * a * (1.f + erff(a * 0.70710678118654752f));
+// rcp.approx (1 ulp) of both values
+__device__ __forceinline__ Pair rcp_fast(Pair x) {
+  float a, b;
+  unpair(x, a, b);
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(a));
+  asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(b));
+  return pair(a, b);
+}
+__device__ __forceinline__ Pair pair_of(float v) { return pair(v, v); }
+
+// The normal distribution's tail Q(|a|) and the exponential e = e^(-a^2 / 2) that it shares with
+// the density: Q = p(t) e / 2, t = 1 / (1 + 0.3275911 |a| / sqrt 2), with the polynomial 7.1.26 of
+// Abramowitz and Stegun, Handbook of Mathematical Functions (absolute error of erf below 1.5e-7).
+// With erff and expf an epilogue took longer than the MMAs of K = 2048.
+__device__ __forceinline__ Pair normal_tail(Pair a, Pair &e) {
+  float x, y;
+  unpair(a, x, y);
+  e = exp2_fast(a * a * pair_of(-0.72134752f));
+  const Pair t = rcp_fast(fma(pair(fabsf(x), fabsf(y)), pair_of(0.23164190f), pair_of(1.f)));
+  Pair p = fma(pair_of(0.5307027145f), t, pair_of(-0.7265760135f));
+  p = fma(p, t, pair_of(0.7107068705f));
+  p = fma(p, t, pair_of(-0.142248368f));
+  p = fma(p, t, pair_of(0.127414796f));
+  return p * t * e;
+}
+
+// f(a): SiLU a / (1 + e^-a), GELU a Phi(a) = a (1 + erf(a / sqrt 2)) / 2, in fp32.
+template <int ACT>
+__device__ __forceinline__ Pair act_value(Pair a) {
+  float x, y;
+  if (ACT == kActRelu) {
+    unpair(a, x, y);
+    return pair(x < 0.f ? 0.f : x, y < 0.f ? 0.f : y);  // keeps NaN
+  }
+  if (ACT == kActSilu)
+    return a * rcp_fast(exp2_fast(a * pair_of(-kLog2e)) + pair_of(1.f));
+  if (ACT == kActGelu) {
+    Pair e;
+    const Pair q = normal_tail(a, e), above = fma(q, pair_of(-1.f), pair_of(1.f));
+    float q0, q1, u0, u1;
+    unpair(a, x, y), unpair(q, q0, q1), unpair(above, u0, u1);
+    return a * pair(x < 0.f ? q0 : u0, y < 0.f ? q1 : u1);
+  }
   return a;
 }
 // f'(a)
-__device__ __forceinline__ float act_slope(float a, int act) {
-  if (act == kActRelu) return a > 0.f ? 1.f : (a != a ? a : 0.f);
-  if (act == kActSilu) {
-    const float s = 1.f / (1.f + __expf(-a));
-    return s * (1.f + a * (1.f - s));
+template <int ACT>
+__device__ __forceinline__ Pair act_slope(Pair a) {
+  float x, y;
+  if (ACT == kActRelu) {
+    unpair(a, x, y);
+    return pair(x > 0.f ? 1.f : (x != x ? x : 0.f), y > 0.f ? 1.f : (y != y ? y : 0.f));
   }
-  if (act == kActGelu)
-    return 0.5f * (1.f + erff(a * 0.70710678118654752f)) +
-           a * __expf(-0.5f * a * a) * 0.39894228040143268f;
-  return 1.f;
+  if (ACT == kActSilu) {
+    const Pair s = rcp_fast(exp2_fast(a * pair_of(-kLog2e)) + pair_of(1.f));
+    return s * fma(a, fma(s, pair_of(-1.f), pair_of(1.f)), pair_of(1.f));
+  }
+  if (ACT == kActGelu) {
+    Pair e;
+    const Pair q = normal_tail(a, e), half = fma(q, pair_of(-1.f), pair_of(0.5f));
+    float h0, h1;
+    unpair(a, x, y), unpair(half, h0, h1);
+    const Pair phi = e * pair_of(0.39894228f);  // Phi = 1/2 +- (1/2 - Q)
+    return fma(a, phi, pair(copysignf(h0, x), copysignf(h1, y)) + pair_of(0.5f));
+  }
+  return pair_of(1.f);
+}
+
+// f of N values (N even): the choice of f is made once, outside the loop over them.
+template <int N, int ACT>
+__device__ __forceinline__ void act_each(float *v) {
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const Pair r = act_value<ACT>(pair(v[i], v[i + 1]));
+    unpair(r, v[i], v[i + 1]);
+  }
+}
+template <int N>
+__device__ __forceinline__ void act_values(float *v, int act) {
+  switch (act) {
+    case kActRelu: act_each<N, kActRelu>(v); break;
+    case kActSilu: act_each<N, kActSilu>(v); break;
+    case kActGelu: act_each<N, kActGelu>(v); break;
+    default: break;
+  }
 }
 
 struct TileEpilogue {
-  void *out;                      // bf16 [M, N], or fp32 partial sums [splits, M, N]
+  __nv_bfloat16 *out;             // [M, N]
   __nv_bfloat16 *pre;             // C * scales + bias in bf16, or null
   const __nv_bfloat16 *bias;      // [N] or null
   const __nv_bfloat16 *residual;  // [M, N] or null
@@ -68,9 +138,11 @@ struct TileArgs {
   CUtensorMap a, b;
   TileEpilogue e;
   int64_t M, N;
-  int m_tiles, n_tiles, splits, kblocks;
-  int partial;  // write fp32 sums of this split
-  int vec;      // 16-byte accesses to every [M, N] and [N] tensor
+  // Tiles 0 to full - 1 take all of k; the others are split into `splits` ranges of k each, whose
+  // fp32 sums go to `partial` [tile - full][split][CTA][BN / 4][128 rows][4].
+  int m_tiles, n_tiles, full, splits, kblocks;
+  float *partial;
+  int vec;  // N is a multiple of 8 and every [M, N] tensor 16-byte aligned
 };
 
 template <int CTAS, int BN, bool FP8>
@@ -78,105 +150,137 @@ struct TileShape {
   static constexpr int NB = BN / CTAS;  // rows of B a CTA holds
   static constexpr int A_BYTES = kTileM * 128, B_BYTES = NB * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (kTileSmemLimit - 2048) / STAGE > 8 ? 8
-                                                                   : (kTileSmemLimit - 2048) / STAGE;
-  static constexpr int SMEM = STAGES * STAGE + 1024 /* alignment */ + 512 /* barriers */;
+  // a warp's 32 x 32 bf16 block on its way to memory, and its columns' bias and scale (fp32)
+  static constexpr int WARP_COLS = BN / 2 >= 32 ? BN / 2 : 32;
+  static constexpr int WARP_BYTES = 2048 + 2 * WARP_COLS * 4;
+  static constexpr int OTHER = 1024 /* alignment */ + 512 /* barriers */ + kEpiWarps * WARP_BYTES;
+  static constexpr int STAGES =
+      (kTileSmemLimit - OTHER) / STAGE > 8 ? 8 : (kTileSmemLimit - OTHER) / STAGE;
+  static constexpr int SMEM = STAGES * STAGE + OTHER;
   static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
-// 32 columns of one row through the epilogue.  Loads bias, scales and residual
-// 16 bytes at a time where the row's columns are all there and aligned.
-__device__ __forceinline__ void tile_epilogue(const TileArgs &p, float *v, int64_t row,
-                                              int64_t col, float row_scale, int64_t split) {
-  const TileEpilogue &e = p.e;
-  const bool full = col + 32 <= p.N;
-  if (p.partial) {
-    float *out = reinterpret_cast<float *>(e.out) + (split * p.M + row) * p.N + col;
-    if (full && p.vec) {
+// ---------------------------------------------------------------- epilogue
+// A warp holds a 32 x 32 block of a, a lane a row.  Rows of a block lie N elements apart, so a lane
+// that moved its own row would touch 32 lines an instruction; the block goes through shared memory
+// (64-byte rows, 16-byte units exchanged so that neither side has bank conflicts) and moves as 4
+// lanes a row.
+__device__ __forceinline__ uint4 *block_unit(uint8_t *block, int row, int unit) {
+  return reinterpret_cast<uint4 *>(block + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
+}
+__device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv_bfloat16 *dst,
+                                            int64_t row0, int64_t col, int64_t M, int64_t N) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-      for (int j = 0; j < 32; j += 4)
-        *reinterpret_cast<float4 *>(out + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-    } else {
-      for (int j = 0; j < 32; ++j)
-        if (col + j < p.N) out[j] = v[j];
+  for (int u = 0; u < 4; ++u) {
+    RowChunk<__nv_bfloat16, 8> c;
+    c.put(v + 8 * u);
+    *block_unit(block, lane, u) = c.raw;
+  }
+  __syncwarp();
+  const int64_t at = col + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2);
+    if (row0 + r < M && at < N)
+      *reinterpret_cast<uint4 *>(dst + (row0 + r) * N + at) = *block_unit(block, r, lane & 3);
+  }
+  __syncwarp();
+}
+// 16-byte units of a block of `src`: issued early, used by block_add.
+__device__ __forceinline__ void block_fetch(const __nv_bfloat16 *src, uint4 *u, int64_t row0,
+                                            int64_t col, int64_t M, int64_t N) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = col + (lane & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = row0 + i * 8 + (lane >> 2);
+    u[i] = make_uint4(0, 0, 0, 0);
+    if (r < M && at < N) u[i] = __ldg(reinterpret_cast<const uint4 *>(src + r * N + at));
+  }
+}
+__device__ __forceinline__ void block_add(uint8_t *block, const uint4 *u, float *v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *block_unit(block, i * 8 + (lane >> 2), lane & 3) = u[i];
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    RowChunk<__nv_bfloat16, 8> c;
+    c.raw = *block_unit(block, lane, k);
+    float w[8];
+    c.get(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[8 * k + i] += w[i];
+  }
+  __syncwarp();
+}
+
+// The block's 32 columns of bias and scale come from shared memory (`bias`, `scale`; scale only
+// with row scales); `res` holds the residual's units.  Every lane of the warp takes part.
+__device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, int64_t M, int64_t N, bool vec,
+                                              float *v, int64_t row0, int64_t col, float row_scale,
+                                              const float *bias, const float *scale,
+                                              uint8_t *block, const uint4 *res) {
+  const int lane = threadIdx.x & 31;
+  if (e.col_scale) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 s = *reinterpret_cast<const float4 *>(scale + j);
+      v[j] *= row_scale * s.x, v[j + 1] *= row_scale * s.y;
+      v[j + 2] *= row_scale * s.z, v[j + 3] *= row_scale * s.w;
     }
+  }
+  if (e.bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+      const float4 b = *reinterpret_cast<const float4 *>(bias + j);
+      v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+    }
+  }
+  if (vec) {
+    if (e.pre) block_store(block, v, e.pre, row0, col, M, N);
+    act_values<32>(v, e.act);
+    if (e.residual) block_add(block, res, v);
+    block_store(block, v, e.out, row0, col, M, N);
     return;
   }
-  const int64_t off = row * p.N + col;
-  __nv_bfloat16 *out = reinterpret_cast<__nv_bfloat16 *>(e.out) + off;
-  if (full && p.vec) {
+  const int64_t row = row0 + lane, off = row * N + col;
+  if (row >= M) return;
+  if (e.pre) {
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-      float w[8];
-      if (e.col_scale) {
-        const float4 s0 = __ldg(reinterpret_cast<const float4 *>(e.col_scale + col + j));
-        const float4 s1 = __ldg(reinterpret_cast<const float4 *>(e.col_scale + col + j + 4));
-        const float s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j + i] = v[j + i] * row_scale * s[i];
-      }
-      auto unpack = [&](const __nv_bfloat16 *src) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src));
-        const uint32_t q[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[2 * i] = __uint_as_float(q[i] << 16);
-          w[2 * i + 1] = __uint_as_float(q[i] & 0xFFFF0000u);
-        }
-      };
-      auto pack = [&](__nv_bfloat16 *dst) {
-        uint32_t q[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __nv_bfloat162 b = __floats2bfloat162_rn(v[j + 2 * i], v[j + 2 * i + 1]);
-          q[i] = *reinterpret_cast<const uint32_t *>(&b);
-        }
-        *reinterpret_cast<uint4 *>(dst) = make_uint4(q[0], q[1], q[2], q[3]);
-      };
-      if (e.bias) {
-        unpack(e.bias + col + j);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j + i] += w[i];
-      }
-      if (e.pre) pack(e.pre + off + j);
-      if (e.act != kActNone) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j + i] = act_value(v[j + i], e.act);
-      }
-      if (e.residual) {
-        unpack(e.residual + off + j);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[j + i] += w[i];
-      }
-      pack(out + j);
-    }
-    return;
+    for (int j = 0; j < 32; ++j)
+      if (col + j < N) store_f(e.pre, off + j, v[j]);
   }
+  act_values<32>(v, e.act);
 #pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    if (col + j >= p.N) break;
-    float a = v[j];
-    if (e.col_scale) a = a * row_scale * __ldg(e.col_scale + col + j);
-    if (e.bias) a += load_f(e.bias, col + j);
-    if (e.pre) store_f(e.pre, off + j, a);
-    a = act_value(a, e.act);
-    if (e.residual) a += load_f(e.residual, off + j);
-    store_f(out, j, a);
+  for (int j = 0; j < 32; ++j)
+    if (col + j < N) store_f(e.out, off + j, v[j] + (e.residual ? load_f(e.residual, off + j) : 0.f));
+}
+
+// Bias and scale of `n` columns from `col` on into a warp's shared memory (0 past N).
+__device__ __forceinline__ void stage_columns(const TileEpilogue &e, int64_t N, int64_t col, int n,
+                                              float *bias, float *scale) {
+  for (int c = threadIdx.x & 31; c < n; c += 32) {
+    if (e.bias) bias[c] = col + c < N ? load_f(e.bias, col + c) : 0.f;
+    if (e.col_scale) scale[c] = col + c < N ? __ldg(e.col_scale + col + c) : 0.f;
   }
 }
 
-// The k blocks of one split: [k0, k1).
-__device__ __forceinline__ void split_range(const TileArgs &p, int split, int &k0, int &k1) {
-  k0 = (int)((int64_t)p.kblocks * split / p.splits);
-  k1 = (int)((int64_t)p.kblocks * (split + 1) / p.splits);
+// Unit t of the work: tile, and its k blocks [k0, k1) (split < 0: all of them).
+struct TileUnit {
+  int tile, split, k0, k1;
+};
+__device__ __forceinline__ TileUnit unit_at(const TileArgs &p, int t) {
+  if (t < p.full) return TileUnit{t, -1, 0, p.kblocks};
+  const int u = t - p.full, tile = u / p.splits, split = u - tile * p.splits;
+  return TileUnit{p.full + tile, split, (int)((int64_t)p.kblocks * split / p.splits),
+                  (int)((int64_t)p.kblocks * (split + 1) / p.splits)};
 }
 
 // Tile order: bands of 8 row tiles, down the rows inside a column, so that a
 // wave of CTAs shares few operand tiles in L2.
-__device__ __forceinline__ void tile_at(const TileArgs &p, int t, int &m, int &n, int &split) {
-  const int per = p.m_tiles * p.n_tiles;
-  split = t / per;
-  t -= split * per;
+__device__ __forceinline__ void tile_at(const TileArgs &p, int t, int &m, int &n) {
   constexpr int kBand = 8;
   const int band = t / (kBand * p.n_tiles);
   const int height = min(kBand, p.m_tiles - band * kBand);
@@ -199,6 +303,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
   uint64_t *full = bars, *empty = bars + STAGES, *acc_full = bars + 2 * STAGES,
            *acc_empty = acc_full + 2, *drain = acc_empty + 2;
   uint32_t *tslot = reinterpret_cast<uint32_t *>(drain + 1);
+  uint8_t *warp_smem = smem + STAGES * S::STAGE + 512;
   volatile uint32_t *failed = tslot + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CTAS == 2 ? sm100::cluster_rank() : 0;
@@ -231,7 +336,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = *tslot;
-  const int tiles = p.m_tiles * p.n_tiles * p.splits;
+  const int units = p.full + (p.m_tiles * p.n_tiles - p.full) * p.splits;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   auto wait = [&](uint64_t *bar, uint32_t parity) {
     bool ok = sm100::mbar_try_wait_cluster(bar, parity, 1000u);
@@ -245,12 +350,12 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
-      int m, n, split, k0, k1;
-      tile_at(p, t, m, n, split);
-      split_range(p, split, k0, k1);
+    for (int t = first; t < units && ok; t += step) {
+      const TileUnit w = unit_at(p, t);
+      int m, n;
+      tile_at(p, w.tile, m, n);
       const int am = (m * CTAS + (int)rank) * kTileM, bn = n * BN + (int)rank * NB;
-      for (int k = k0; k < k1; ++k) {
+      for (int k = w.k0; k < w.k1; ++k) {
         if (issued >= STAGES && !(ok = wait(empty + stage, phase ^ 1))) break;
         if (leader) sm100::mbar_arrive_expect_tx(full + stage, CTAS * S::STAGE);
         const uint32_t bar = CTAS == 2 ? sm100::map_to_rank(full + stage, 0)
@@ -291,13 +396,11 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += step) {
-      int m, n, split, k0, k1;
-      tile_at(p, t, m, n, split);
-      split_range(p, split, k0, k1);
+    for (int t = first; t < units && ok; t += step) {
+      const TileUnit w = unit_at(p, t);
       if (!(ok = wait(acc_empty + acc, acc_phase ^ 1))) break;
       sm100::tc_fence_after();
-      for (int k = k0; k < k1; ++k) {
+      for (int k = w.k0; k < w.k1; ++k) {
         if (!(ok = wait(full + stage, phase))) break;
         sm100::tc_fence_after();
         const uint32_t da = sm100::smem_u32(smem + stage * S::STAGE), db = da + S::A_BYTES;
@@ -306,7 +409,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
 #pragma unroll
         for (int s = 0; s < 4; ++s)  // 32 bytes of k, or 16 k rows of 128 bytes
           sm100::mma_group<CTAS, FP8>(tmem + acc * BN, ad + s * (A_MN ? 128 : 2),
-                                      bd + s * (B_MN ? 128 : 2), idesc, k > k0 || s > 0);
+                                      bd + s * (B_MN ? 128 : 2), idesc, k > w.k0 || s > 0);
         sm100::mma_commit_group<CTAS>(empty + stage);
         if (++stage == STAGES) stage = 0, phase ^= 1;
       }
@@ -320,23 +423,36 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     }
   } else if (warp >= 2) {  // ----------------------------------------------- epilogue
     const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
-    constexpr int COLS = BN / 2 >= 32 ? BN / 2 : 32;  // columns of a warp
+    constexpr int COLS = S::WARP_COLS;
     const bool mine = half * COLS < BN;
+    uint8_t *block = warp_smem + ew * S::WARP_BYTES;
+    float *bias = reinterpret_cast<float *>(block + 2048), *scale = bias + COLS;
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    for (int t = first; t < tiles; t += step) {
-      int m, n, split;
-      tile_at(p, t, m, n, split);
+    for (int t = first; t < units; t += step) {
+      const TileUnit w = unit_at(p, t);
+      int m, n;
+      tile_at(p, w.tile, m, n);
+      const int64_t row0 = (int64_t)(m * CTAS + (int)rank) * kTileM + quad * 32;
+      const int64_t col0 = (int64_t)n * BN + half * COLS;
+      const bool in = mine && row0 < p.M && col0 < p.N;
+      float rs = 1.f;
+      if (in && w.split < 0) {  // while the accumulators are not there yet
+        stage_columns(p.e, p.N, col0, COLS, bias, scale);
+        if (p.e.row_scale && row0 + lane < p.M) rs = __ldg(p.e.row_scale + row0 + lane);
+      }
+      __syncwarp();
       if (ok) ok = wait(acc_full + acc, acc_phase);
       ok = __all_sync(0xFFFFFFFFu, ok);
       sm100::tc_fence_after();
-      const int64_t row = (int64_t)(m * CTAS + (int)rank) * kTileM + quad * 32 + lane;
-      const float rs = p.e.row_scale && row < p.M ? __ldg(p.e.row_scale + row) : 1.f;
 #pragma unroll 1
-      for (int c = 0; mine && c < COLS; c += 32) {
-        const int64_t col = (int64_t)n * BN + half * COLS + c;
+      for (int c = 0; in && c < COLS && col0 + c < p.N; c += 32) {
+        const bool res = w.split < 0 && p.e.residual && p.vec;
+        uint4 ru[4];
+        if (res) block_fetch(p.e.residual, ru, row0, col0 + c, p.M, p.N);
         float v[32];
+        __syncwarp();
         if (ok) {
           sm100::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS + c, v);
           sm100::tmem_ld_wait();
@@ -344,7 +460,17 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
-        if (row < p.M && col < p.N) tile_epilogue(p, v, row, col, rs, split);
+        if (w.split < 0) {
+          tile_epilogue(p.e, p.M, p.N, p.vec, v, row0, col0 + c, rs, bias + c, scale + c, block, ru);
+        } else {
+          float4 *out = reinterpret_cast<float4 *>(p.partial) +
+                        (((int64_t)(w.tile - p.full) * p.splits + w.split) * CTAS + rank) *
+                            (BN / 4 * kTileM) +
+                        (half * COLS + c) / 4 * kTileM + quad * 32 + lane;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            out[j * kTileM] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
       }
       sm100::tc_fence_before();
       __syncwarp();
@@ -368,6 +494,47 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     else
       sm100::tmem_dealloc(tmem, S::TMEM);
   }
+}
+
+// The tiles whose k was split: their sums, added in split order, through the epilogue.  A warp takes
+// a 32 x 32 block.
+constexpr int kJoinThreads = 128;
+template <int CTAS, int BN>
+__global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_constant__ TileArgs p) {
+  constexpr int BLOCKS = CTAS * 4 * (BN / 32);  // of a tile
+  __shared__ __align__(16) uint8_t smem[kJoinThreads / 32][2048 + 2 * 32 * 4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int id = blockIdx.x * (kJoinThreads / 32) + warp;
+  const int tile = id / BLOCKS, b = id - tile * BLOCKS;
+  if (p.full + tile >= p.m_tiles * p.n_tiles) return;
+  const int cta = b / (4 * (BN / 32)), quad = b / (BN / 32) % 4, c = b % (BN / 32) * 32;
+  int m, n;
+  tile_at(p, p.full + tile, m, n);
+  const int64_t row0 = (int64_t)(m * CTAS + cta) * kTileM + quad * 32;
+  const int64_t col = (int64_t)n * BN + c;
+  if (row0 >= p.M || col >= p.N) return;
+  uint8_t *block = smem[warp];
+  float *bias = reinterpret_cast<float *>(block + 2048), *scale = bias + 32;
+  stage_columns(p.e, p.N, col, 32, bias, scale);
+  __syncwarp();
+  uint4 ru[4];
+  if (p.e.residual && p.vec) block_fetch(p.e.residual, ru, row0, col, p.M, p.N);
+  const float rs = p.e.row_scale && row0 + lane < p.M ? __ldg(p.e.row_scale + row0 + lane) : 1.f;
+  float v[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) v[j] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 *in = reinterpret_cast<const float4 *>(p.partial) +
+                       (((int64_t)tile * p.splits + s) * CTAS + cta) * (BN / 4 * kTileM) +
+                       c / 4 * kTileM + quad * 32 + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float4 u = __ldg(in + j * kTileM);
+      v[4 * j] += u.x, v[4 * j + 1] += u.y, v[4 * j + 2] += u.z, v[4 * j + 3] += u.w;
+    }
+  }
+  tile_epilogue(p.e, p.M, p.N, p.vec, v, row0, col, rs, bias, scale, block, ru);
 }
 
 // ---------------------------------------------------------------- host side

@@ -70,9 +70,11 @@ __device__ __forceinline__ void scalar_epilogue(const TileEpilogue &e, float a, 
   if (e.bias) a += load_f(e.bias, col);
   const int64_t off = row * N + col;
   if (e.pre) store_f(e.pre, off, a);
-  a = act_value(a, e.act);
+  float v[2] = {a, 0.f};
+  act_values<2>(v, e.act);
+  a = v[0];
   if (e.residual) a += load_f(e.residual, off);
-  store_f(reinterpret_cast<__nv_bfloat16 *>(e.out), off, a);
+  store_f(e.out, off, a);
 }
 
 // R rows of x against every weight row; a warp a column.
@@ -147,52 +149,50 @@ pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols,
   }
 }
 
-// y from the splits' fp32 sums, added in split order.
-__global__ void __launch_bounds__(256)
-join_kernel(const float *__restrict__ partial, int splits, int64_t M, int64_t N, TileEpilogue e) {
-  const int64_t total = M * N;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += partial[k * total + i];
-    const int64_t row = i / N;
-    scalar_epilogue(e, s, row, i - row * N, N);
-  }
-}
-
 // da = dy f'(pre) in bf16 (pitch `pitch`, its padding zero; null: not wanted), and the blocks'
 // column sums of the unrounded da (null: not wanted).  A thread holds VEC columns of every
 // kSlopeLanes-th row of its block's rows.
-template <int VEC>
+template <int VEC, int ACT>
 __global__ void __launch_bounds__(32 * kSlopeLanes)
-slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restrict__ pre, int act,
-             int64_t M, int64_t N, __nv_bfloat16 *__restrict__ da, int64_t pitch,
+slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restrict__ pre, int64_t M,
+             int64_t N, __nv_bfloat16 *__restrict__ da, int64_t pitch,
              float *__restrict__ partial) {
   __shared__ float sums[kSlopeLanes][32 * VEC];
+  constexpr int R = 4;  // rows in flight
   const int64_t col = ((int64_t)blockIdx.x * 32 + threadIdx.x) * VEC;
   float s[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) s[i] = 0.f;
   const int64_t r0 = M * blockIdx.y / gridDim.y, r1 = M * (blockIdx.y + 1) / gridDim.y;
   if (col < N) {
-#pragma unroll 2
-    for (int64_t r = r0 + threadIdx.y; r < r1; r += kSlopeLanes) {
-      RowChunk<__nv_bfloat16, VEC> c, q;
-      c.load(dy + r * N + col);
-      float g[VEC];
-      c.get(g);
-      if (pre) {
-        float a[VEC];
-        q.load(pre + r * N + col);
-        q.get(a);
+    for (int64_t r = r0 + threadIdx.y; r < r1; r += kSlopeLanes * R) {
+      RowChunk<__nv_bfloat16, VEC> c[R], q[R];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) g[i] *= act_slope(a[i], act);
+      for (int k = 0; k < R; ++k) {
+        c[k].zero(), q[k].zero();
+        if (r + k * kSlopeLanes >= r1) continue;
+        c[k].load(dy + (r + k * kSlopeLanes) * N + col);
+        if (ACT != kActNone) q[k].load(pre + (r + k * kSlopeLanes) * N + col);
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[i] += g[i];
-      if (da) {
-        c.put(g);
-        c.store(da + r * pitch + col);
+      for (int k = 0; k < R; ++k) {
+        float g[VEC + 1], a[VEC + 1];
+        c[k].get(g), q[k].get(a);
+        if (VEC == 1) g[1] = 0.f, a[1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; i += 2) {
+          const Pair d = pair(g[i], g[i + 1]) * act_slope<ACT>(pair(a[i], a[i + 1]));
+          unpair(d, g[i], g[i + 1]);
+        }
+        const bool live = r + k * kSlopeLanes < r1;
+        if (live) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) s[i] += g[i];
+        }
+        if (da && live) {
+          c[k].put(g);
+          c[k].store(da + (r + k * kSlopeLanes) * pitch + col);
+        }
       }
     }
   } else if (da && col < pitch) {
@@ -211,6 +211,25 @@ slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restri
 #pragma unroll
     for (int l = 0; l < kSlopeLanes; ++l) t += sums[l][c];
     partial[(int64_t)blockIdx.y * N + out] = t;
+  }
+}
+
+template <int VEC>
+void launch_slope(dim3 grid, dim3 block, int act, const __nv_bfloat16 *dy, const __nv_bfloat16 *pre,
+                  int64_t M, int64_t N, __nv_bfloat16 *da, int64_t pitch, float *columns,
+                  cudaStream_t s) {
+  switch (act) {
+    case kActRelu:
+      slope_kernel<VEC, kActRelu><<<grid, block, 0, s>>>(dy, pre, M, N, da, pitch, columns);
+      break;
+    case kActSilu:
+      slope_kernel<VEC, kActSilu><<<grid, block, 0, s>>>(dy, pre, M, N, da, pitch, columns);
+      break;
+    case kActGelu:
+      slope_kernel<VEC, kActGelu><<<grid, block, 0, s>>>(dy, pre, M, N, da, pitch, columns);
+      break;
+    default:
+      slope_kernel<VEC, kActNone><<<grid, block, 0, s>>>(dy, pre, M, N, da, pitch, columns);
   }
 }
 
@@ -238,40 +257,44 @@ enum TileKind { kPair256, kPair128, kOne128, kOne64 };
 
 struct ProductPlan {
   TileKind kind;
-  int ctas, bn, m_tiles, n_tiles, splits, kblocks, grid;
+  int m_tiles, n_tiles, full, splits, grid;
   int64_t partial_floats;
 };
 
-// Tile shape and split of an [M, N] product over `kblocks` blocks of 128 bytes.
+// Tile shape and split of an [M, N] product over `kblocks` blocks of 128 bytes.  Time in units of
+// 128 clocks, about 70 ns: a k block of a 128 x 64 tile's MMAs.
 ProductPlan product_plan(int64_t M, int64_t N, int kblocks) {
   const int sms = sm_count();
   struct Shape {
     TileKind kind;
     int ctas, bn;
-    double cost;  // of a k block, in 128 x 64 tiles' time
+    double block;  // a k block, measured at 16384 x 8192 x 2048 and its gradient's products
   };
   static const Shape shapes[] = {
-      {kPair256, 2, 256, 4.0}, {kPair128, 2, 128, 2.2}, {kOne128, 1, 128, 2.4}, {kOne64, 1, 64, 1.4}};
+      {kPair256, 2, 256, 4.0}, {kPair128, 2, 128, 2.8}, {kOne128, 1, 128, 2.85}, {kOne64, 1, 64, 1.8}};
   ProductPlan best{};
   double best_cost = 0;
   for (const Shape &s : shapes) {
-    const int64_t mt = cdiv(M, (int64_t)kTileM * s.ctas), nt = cdiv(N, s.bn);
+    const int64_t mt = cdiv(M, (int64_t)kTileM * s.ctas), nt = cdiv(N, s.bn), tiles = mt * nt;
     const int slots = sms / s.ctas;
-    int splits = 1;
-    if (mt * nt * 2 <= slots) {  // k split until the SMs are busy, 4 blocks a split at least
-      splits = (int)std::min<int64_t>(slots / (mt * nt), std::max(1, kblocks / 4));
-      splits = std::min(splits, 64);
-    }
-    const int64_t waves = cdiv(mt * nt * splits, slots);
-    // a tile costs its k blocks and about 6 blocks' time of fill and epilogue; a split is
-    // written and read once more
-    const double cost = (double)waves * s.cost * ((double)cdiv(kblocks, splits) + 6.0) +
-                        (splits > 1 ? 12.0 : 0.0);
-    if (best_cost == 0 || cost < best_cost) {
-      best_cost = cost;
-      best = ProductPlan{s.kind, s.ctas, s.bn, (int)mt, (int)nt, splits, kblocks,
-                         (int)std::min<int64_t>(mt * nt * splits, slots) * s.ctas,
-                         splits > 1 ? (int64_t)splits * M * N : 0};
+    const int64_t waves = tiles / slots, tail = tiles % slots;
+    constexpr double kFill = 24;  // pipeline fill and the last epilogue, once
+    const double whole = s.block * kblocks + 6;
+    for (int splits = 1; splits <= 64; ++splits) {
+      // every split keeps 4 k blocks, and all splits run at once
+      if (splits > 1 && (tail == 0 || tail * splits > slots || kblocks / splits < 4)) break;
+      double cost = kFill + waves * whole;
+      if (tail) cost += s.block * cdiv(kblocks, splits) + 6;
+      // the sums are written and read once (about 6 TB/s), and one more kernel runs
+      const int64_t floats = splits > 1 ? tail * splits * s.ctas * kTileM * s.bn : 0;
+      if (splits > 1) cost += 45 + floats * 8 / 4.2e5;
+      if (best_cost == 0 || cost < best_cost) {
+        best_cost = cost;
+        const int64_t full = splits > 1 ? waves * slots : tiles;
+        const int64_t units = full + (tiles - full) * splits;
+        best = ProductPlan{s.kind, (int)mt, (int)nt, (int)full, splits,
+                           (int)std::min<int64_t>(units, slots) * s.ctas, floats};
+      }
     }
   }
   return best;
@@ -306,7 +329,12 @@ int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
   LNET_TRY(cuda_check(cudaLaunchKernelEx(&cfg, kernel, args), "tile_gemm_kernel"));
-  return after_launch("tile_gemm_kernel");
+  LNET_TRY(after_launch("tile_gemm_kernel"));
+  if (q.splits == 1) return LNET_OK;
+  const int blocks = (q.m_tiles * q.n_tiles - q.full) * CTAS * 4 * (BN / 32);
+  tile_join_kernel<CTAS, BN><<<(unsigned)cdiv(blocks, kJoinThreads / 32), kJoinThreads, 0, stream>>>(
+      args);
+  return after_launch("tile_join_kernel");
 }
 
 template <bool A_MN, bool B_MN, bool FP8>
@@ -330,24 +358,11 @@ int product(const TileOperand &a, const TileOperand &b, const TileEpilogue &e, f
   TileArgs args{};
   args.e = e;
   args.M = M, args.N = N;
-  args.m_tiles = q.m_tiles, args.n_tiles = q.n_tiles, args.splits = q.splits;
-  args.kblocks = kblocks;
-  args.partial = q.splits > 1;
-  args.vec = N % 8 == 0 && aligned16(e.out) && aligned16(e.pre) && aligned16(e.bias) &&
-             aligned16(e.residual) && aligned16(e.col_scale);
-  if (args.partial) {
-    args.e = TileEpilogue{};
-    args.e.out = partial;
-    args.vec = N % 4 == 0;
-  }
-  LNET_TRY((launch_kind<A_MN, B_MN, FP8>(q, a, b, args, s)));
-  if (args.partial) {
-    const int64_t total = M * N;
-    const int blocks = (int)std::min<int64_t>(cdiv(total, 256), (int64_t)sm_count() * 16);
-    join_kernel<<<blocks, 256, 0, s>>>(partial, q.splits, M, N, e);
-    LNET_TRY(after_launch("linear_join_kernel"));
-  }
-  return LNET_OK;
+  args.m_tiles = q.m_tiles, args.n_tiles = q.n_tiles, args.full = q.full;
+  args.splits = q.splits, args.kblocks = kblocks;
+  args.partial = partial;
+  args.vec = N % 8 == 0 && aligned16(e.out) && aligned16(e.pre) && aligned16(e.residual);
+  return launch_kind<A_MN, B_MN, FP8>(q, a, b, args, s);
 }
 
 bool tma_rows(const void *p, int64_t pitch_bytes) { return aligned16(p) && pitch_bytes % 16 == 0; }
@@ -492,7 +507,7 @@ extern "C" int lnet_b200_linear_forward(const lnet_b200_linear_request *req, voi
   const bool fp8 = req->dtype == LNET_E4M3;
   const int elem = fp8 ? 1 : 2;
   TileEpilogue e{};
-  e.out = y;
+  e.out = reinterpret_cast<__nv_bfloat16 *>(y);
   e.pre = reinterpret_cast<__nv_bfloat16 *>(preact);
   e.bias = reinterpret_cast<const __nv_bfloat16 *>(req->bias);
   e.residual = reinterpret_cast<const __nv_bfloat16 *>(req->residual);
@@ -572,11 +587,9 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
     const dim3 grid((unsigned)cdiv(width, 32 * vec), (unsigned)slope_row_blocks(M, N, vec));
     const dim3 block(32, kSlopeLanes);
     if (vec == 8)
-      slope_kernel<8><<<grid, block, 0, stream>>>(dyp, pre, req->activation, M, N, w.da, pitch,
-                                                  w.columns);
+      launch_slope<8>(grid, block, req->activation, dyp, pre, M, N, w.da, pitch, w.columns, stream);
     else
-      slope_kernel<1><<<grid, block, 0, stream>>>(dyp, pre, req->activation, M, N, w.da, pitch,
-                                                  w.columns);
+      launch_slope<1>(grid, block, req->activation, dyp, pre, M, N, w.da, pitch, w.columns, stream);
     LNET_TRY(after_launch("linear_slope_kernel"));
     if (w.columns) {
       column_sum_kernel<<<(unsigned)cdiv(N, 32), dim3(32, 32), 0, stream>>>(
@@ -590,7 +603,7 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
     TileOperand b{req->weight, K, N, K, true};
     LNET_TRY(packed(b, N, K, 2, w.w, stream));
     TileEpilogue e{};
-    e.out = dx;
+    e.out = reinterpret_cast<__nv_bfloat16 *>(dx);
     LNET_TRY((product<false, true, false>(a, b, e, w.partial, stream)));
   }
   if (dweight) {
@@ -598,7 +611,7 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
     TileOperand b{req->x, K, M, K, true};
     LNET_TRY(packed(b, M, K, 2, w.x, stream));
     TileEpilogue e{};
-    e.out = dweight;
+    e.out = reinterpret_cast<__nv_bfloat16 *>(dweight);
     LNET_TRY((product<true, true, false>(a, b, e, w.partial, stream)));
   }
   return LNET_OK;

@@ -17,8 +17,10 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "rows.cuh"
+#include "sm100.cuh"
 
 namespace lnet {
 namespace {
@@ -106,6 +108,16 @@ struct NormArgs {
   int w_bf16;
 };
 
+// Brings the rows of a block's next turn, which lie together, to L2: one instruction a tensor, and
+// the next turn waits for L2 in place of HBM.
+template <typename T, int VEC>
+__device__ __forceinline__ void prefetch_rows(const T *p, int64_t base, int per, int64_t rows,
+                                              int64_t dim) {
+  if (VEC == 1 || p == nullptr || base >= rows) return;
+  const int64_t n = min((int64_t)per, rows - base) * dim * (int64_t)sizeof(T);
+  sm100::bulk_prefetch_l2(p + base * dim, (uint32_t)n);
+}
+
 template <typename T, int VEC, int G, bool FP8>
 __global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
 norm_forward_kernel(const NormArgs a) {
@@ -126,6 +138,10 @@ norm_forward_kernel(const NormArgs a) {
     const int64_t row = base + sub;
     const bool live = row < a.rows;
     const int64_t off = row * a.dim;
+    const int64_t next = base + (int64_t)gridDim.x * per;
+    // (with several rows a block the loads in flight suffice, and the copies cost a sixth)
+    if (G == 0 && threadIdx.x == 0) prefetch_rows<T, VEC>(x, next, per, a.rows, a.dim);
+    if (G == 0 && threadIdx.x == blockDim.x - 1) prefetch_rows<T, VEC>(r, next, per, a.rows, a.dim);
     RowChunk<T, VEC> cx[NV], cr[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -289,6 +305,10 @@ norm_backward_kernel(const NormGradArgs a) {
     const int64_t row = base + sub;
     const bool live = row < a.rows;
     const int64_t off = row * a.dim;
+    const int64_t next = base + (int64_t)gridDim.x * per;
+    if (threadIdx.x == 0) prefetch_rows<T, VEC>(hp, next, per, a.rows, a.dim);
+    if (threadIdx.x == 32) prefetch_rows<T, VEC>(dyp, next, per, a.rows, a.dim);
+    if (threadIdx.x == blockDim.x - 1) prefetch_rows<T, VEC>(dhp, next, per, a.rows, a.dim);
     RowChunk<T, VEC> ch[NV], cy[NV], cs[NV];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -421,9 +441,10 @@ norm_columns_kernel(const float *__restrict__ partial, int blocks, int64_t dim, 
   }
 }
 
-// Threads, lanes a row and blocks of a call (lanes 0: a block a row; wide: see above).
+// Threads, lanes a row, row groups and blocks (at most) of a call (lanes 0: a block a row).
 struct NormPlan {
   int lanes, threads, blocks;
+  int64_t groups;
   bool vec, wide;
 };
 
@@ -445,22 +466,45 @@ NormPlan norm_plan(int64_t rows, int64_t dim, int elem, bool aligned, int blocks
     p.wide = true;
     p.threads = kWideThreads;
   }
-  p.blocks = (int)std::min<int64_t>(cdiv(rows, per), (int64_t)sm_count() * blocks_per_sm);
+  p.groups = cdiv(rows, per);
+  p.blocks = (int)std::min<int64_t>(p.groups, (int64_t)sm_count() * blocks_per_sm);
   return p;
 }
 
-// blocks of an SM: forward blocks of 256 threads fill it; the gradient's hold more registers,
-// and each writes its column sums
-constexpr int kForwardBlocks = 8, kBackwardBlocks = 4;
+// The grid of a persistent kernel: as many blocks as run at once (a second, shorter wave would
+// leave most of the GPU idle), at most p.blocks.
+template <auto KERNEL>
+int resident_blocks(const NormPlan &p) {
+  static std::atomic<int> known[kWideThreads / 32 + 1];  // by threads
+  std::atomic<int> &k = known[p.threads / 32];
+  int n = k.load();
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, p.threads, 0) != cudaSuccess ||
+        n < 1)
+      n = 1;
+    k.store(n);
+  }
+  return (int)std::min<int64_t>(p.blocks, (int64_t)sm_count() * n);
+}
+
+// most blocks of an SM; each of the gradient's writes its column sums
+constexpr int kForwardBlocks = 32, kBackwardBlocks = 4;
+
+template <auto KERNEL, typename A>
+int launch_rows(const NormPlan &p, const A &a, cudaStream_t s) {
+  const int blocks = resident_blocks<KERNEL>(p);
+  KERNEL<<<blocks, p.threads, 0, s>>>(a);
+  return blocks;
+}
 
 template <typename T, int VEC, bool FP8>
 void launch_forward(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
   switch (p.lanes) {
-    case 4: norm_forward_kernel<T, VEC, 4, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 8: norm_forward_kernel<T, VEC, 8, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 16: norm_forward_kernel<T, VEC, 16, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 32: norm_forward_kernel<T, VEC, 32, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
-    default: norm_forward_kernel<T, VEC, 0, FP8><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 4: launch_rows<norm_forward_kernel<T, VEC, 4, FP8>>(p, a, s); break;
+    case 8: launch_rows<norm_forward_kernel<T, VEC, 8, FP8>>(p, a, s); break;
+    case 16: launch_rows<norm_forward_kernel<T, VEC, 16, FP8>>(p, a, s); break;
+    case 32: launch_rows<norm_forward_kernel<T, VEC, 32, FP8>>(p, a, s); break;
+    default: launch_rows<norm_forward_kernel<T, VEC, 0, FP8>>(p, a, s); break;
   }
 }
 
@@ -470,7 +514,7 @@ int forward_typed(const NormArgs &a, cudaStream_t s) {
                        aligned16(a.q) && aligned16(a.w);
   const NormPlan p = norm_plan(a.rows, a.dim, sizeof(T), aligned, kForwardBlocks);
   if (p.wide)
-    norm_forward_wide_kernel<T, FP8><<<p.blocks, p.threads, 0, s>>>(a);
+    launch_rows<norm_forward_wide_kernel<T, FP8>>(p, a, s);
   else if (p.vec)
     launch_forward<T, vec_of<T>(), FP8>(p, a, s);
   else
@@ -478,15 +522,22 @@ int forward_typed(const NormArgs &a, cudaStream_t s) {
   return after_launch("norm_forward_kernel");
 }
 
+// The gradient's kernel; returns its blocks.
 template <typename T, int VEC>
-void launch_backward(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
+int launch_backward(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
   switch (p.lanes) {
-    case 4: norm_backward_kernel<T, VEC, 4><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 8: norm_backward_kernel<T, VEC, 8><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 16: norm_backward_kernel<T, VEC, 16><<<p.blocks, p.threads, 0, s>>>(a); break;
-    case 32: norm_backward_kernel<T, VEC, 32><<<p.blocks, p.threads, 0, s>>>(a); break;
-    default: norm_backward_kernel<T, VEC, 0><<<p.blocks, p.threads, 0, s>>>(a); break;
+    case 4: return launch_rows<norm_backward_kernel<T, VEC, 4>>(p, a, s);
+    case 8: return launch_rows<norm_backward_kernel<T, VEC, 8>>(p, a, s);
+    case 16: return launch_rows<norm_backward_kernel<T, VEC, 16>>(p, a, s);
+    case 32: return launch_rows<norm_backward_kernel<T, VEC, 32>>(p, a, s);
+    default: return launch_rows<norm_backward_kernel<T, VEC, 0>>(p, a, s);
   }
+}
+
+template <typename T>
+int backward_typed(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
+  if (p.wide) return launch_rows<norm_backward_wide_kernel<T>>(p, a, s);
+  return p.vec ? launch_backward<T, vec_of<T>()>(p, a, s) : launch_backward<T, 1>(p, a, s);
 }
 
 int check_norm(const char *what, int64_t rows, int64_t dim, int dtype, int weight_dtype,
@@ -614,25 +665,12 @@ extern "C" int lnet_b200_residual_rms_norm_backward(
   NormGradArgs a{stream_in, weight, dy, dstream, rstd, dx,
                  dweight ? reinterpret_cast<float *>(workspace) : nullptr, rows, dim,
                  weight_dtype == LNET_BF16};
-  if (dtype == LNET_BF16) {
-    if (p.wide)
-      norm_backward_wide_kernel<__nv_bfloat16><<<p.blocks, p.threads, 0, stream>>>(a);
-    else if (p.vec)
-      launch_backward<__nv_bfloat16, 8>(p, a, stream);
-    else
-      launch_backward<__nv_bfloat16, 1>(p, a, stream);
-  } else {
-    if (p.wide)
-      norm_backward_wide_kernel<float><<<p.blocks, p.threads, 0, stream>>>(a);
-    else if (p.vec)
-      launch_backward<float, 4>(p, a, stream);
-    else
-      launch_backward<float, 1>(p, a, stream);
-  }
+  const int blocks = dtype == LNET_BF16 ? backward_typed<__nv_bfloat16>(p, a, stream)
+                                        : backward_typed<float>(p, a, stream);
   LNET_TRY(after_launch("norm_backward_kernel"));
   if (dweight) {
     norm_columns_kernel<<<(unsigned)cdiv(dim, 32), dim3(32, kReduceLanes), 0, stream>>>(
-        a.partial, p.blocks, dim, dweight, a.w_bf16);
+        a.partial, blocks, dim, dweight, a.w_bf16);
     LNET_TRY(after_launch("norm_columns_kernel"));
   }
   return LNET_OK;

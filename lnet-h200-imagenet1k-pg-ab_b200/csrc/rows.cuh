@@ -6,6 +6,8 @@
 
 namespace lnet {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 // VEC consecutive elements of a row: 16 bytes, or one element where the row's
 // pitch or base does not keep 16-byte alignment.
 template <typename T, int VEC>
@@ -119,6 +121,46 @@ __device__ __forceinline__ float group_reduce(float v, float *scratch) {
     for (int o = 16; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
   }
   return v;
+}
+
+// ex2.approx (2 ulp), results below 2^-126 flushed to zero
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two fp32 values in one register pair: one instruction for both.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ void unpair(Pair p, float &a, float &b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v));
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
+__device__ __forceinline__ Pair exp2_fast(Pair x) {
+  float a, b;
+  unpair(x, a, b);
+  return pair(exp2_fast(a), exp2_fast(b));
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
