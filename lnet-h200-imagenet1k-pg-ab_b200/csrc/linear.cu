@@ -27,7 +27,7 @@ namespace {
 constexpr int kVectorRows = 8;
 constexpr int kVectorThreads = 256;
 constexpr int kPackThreads = 256;
-constexpr int kSlopeLanes = 8;  // row lanes of a block of the slope kernel
+constexpr int kSlopeLanes = 8, kSlopeBlocks = 4;  // row lanes and resident blocks of the slope kernel
 
 struct VectorArgs {
   const void *x, *w;
@@ -153,12 +153,12 @@ pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols,
 // column sums of the unrounded da (null: not wanted).  A thread holds VEC columns of every
 // kSlopeLanes-th row of its block's rows.
 template <int VEC, int ACT>
-__global__ void __launch_bounds__(32 * kSlopeLanes)
+__global__ void __launch_bounds__(32 * kSlopeLanes, kSlopeBlocks)
 slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restrict__ pre, int64_t M,
              int64_t N, __nv_bfloat16 *__restrict__ da, int64_t pitch,
              float *__restrict__ partial) {
   __shared__ float sums[kSlopeLanes][32 * VEC];
-  constexpr int R = 4;  // rows in flight
+  constexpr int R = 2;  // rows in flight; four held registers that a fourth block needs
   const int64_t col = ((int64_t)blockIdx.x * 32 + threadIdx.x) * VEC;
   float s[VEC];
 #pragma unroll
@@ -426,7 +426,7 @@ ForwardWork forward_work(Arena &ar, const lnet_b200_linear_request *q) {
 
 int slope_row_blocks(int64_t M, int64_t N, int vec) {
   const int64_t across = cdiv(N, 32 * vec);
-  const int64_t want = cdiv((int64_t)sm_count() * 6, across);
+  const int64_t want = (int64_t)sm_count() * kSlopeBlocks / across;  // all of them at once
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, cdiv(M, kSlopeLanes * 2)));
 }
 int slope_vec(const lnet_b200_linear_request *q, const void *pre, const void *dy) {

@@ -67,35 +67,54 @@ __device__ __forceinline__ void weight_chunk(const void *w, bool w_bf16, int c, 
   }
 }
 
-// q = e4m3(y / s), saturating; s = 0 means that the row is zero.
+template <int VEC>
+__device__ __forceinline__ void weight_lanes(const void *w, bool w_bf16, int c, Lanes<VEC> *p) {
+  float v[VEC];
+  weight_chunk<VEC>(w, w_bf16, c, v);
+  to_lanes<VEC>(v, p);
+}
+
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-// The quotient is taken as a product with 1 / s where that is a normal number: two roundings of
-// fp32, 2^-20 of a code's step, so a code differs only where y / s lies that near to a tie.
+// e4m3(v k) of a chunk, saturating.
 template <int VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t *p, const float *v, float s) {
-  float d[VEC];
-  if (s == 0.f || s > 1e-30f) {
-    const float inv = s == 0.f ? 1.f : 1.f / s;
+__device__ __forceinline__ void store_e4m3(uint8_t *p, const Lanes<VEC> *l, float k) {
+  Lanes<VEC> s[lanes_of<VEC>()];
+  float v[VEC];
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) d[i] = v[i] * inv;
+  for (int i = 0; i < lanes_of<VEC>(); ++i) s[i] = l[i] * splat<VEC>(k);
+  from_lanes<VEC>(s, v);
+  if constexpr (VEC == 1) {
+    *p = (uint8_t)e4m3_pair(v[0], 0.f);
   } else {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) d[i] = v[i] / s;
-  }
-  if (VEC == 1) {
-    *p = (uint8_t)(e4m3_pair(d[0], 0.f) & 0xFF);
-  } else {
-    uint32_t w[VEC >= 4 ? VEC / 4 : 1];
+    uint32_t q[VEC / 4];
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
-      w[i] = e4m3_pair(d[4 * i], d[4 * i + 1]) | (e4m3_pair(d[4 * i + 2], d[4 * i + 3]) << 16);
-    if (VEC == 8)
-      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[VEC == 8 ? 1 : 0]);
+      q[i] = e4m3_pair(v[4 * i], v[4 * i + 1]) | (e4m3_pair(v[4 * i + 2], v[4 * i + 3]) << 16);
+    if constexpr (VEC == 8)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(q[0], q[1]);
     else
-      *reinterpret_cast<uint32_t *>(p) = w[0];
+      *reinterpret_cast<uint32_t *>(p) = q[0];
   }
+}
+// Scale of a row whose y is f t, and the factor k that takes t to its codes: with m = max|t|,
+// s = f m / 448 and y / s = t (448 / m), two fp32 roundings from the quotient, 2^-20 of a code's
+// step.  A zero row has s = 0 and codes 0; a scale that is not finite takes its row along.
+__device__ __forceinline__ float e4m3_scale(float m, float f, float &k) {
+  const float s = f * m / kE4m3Max;
+  k = s == 0.f ? 0.f : kE4m3Max / m;
+  if (!(s < INFINITY)) k = s == s ? 0.f : s;
+  return s;
+}
+// Largest magnitude of a chunk so far.
+template <int VEC>
+__device__ __forceinline__ float chunk_magnitude(float m, const Lanes<VEC> *l) {
+  float v[VEC];
+  from_lanes<VEC>(l, v);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) m = MaxMagnitudeOp::of(m, fabsf(v[i]));
+  return m;
 }
 
 struct NormArgs {
@@ -127,11 +146,13 @@ norm_forward_kernel(const NormArgs a) {
   const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
   const int nvec = (int)(a.dim / VEC);
   const T *x = reinterpret_cast<const T *>(a.x), *r = reinterpret_cast<const T *>(a.r);
-  float w[NV][VEC];  // a thread's columns are the same in every row
+  constexpr int NP = lanes_of<VEC>();
+  using L = Lanes<VEC>;
+  L w[NV][NP];  // a thread's columns are the same in every row
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + j * g;
-    if (c < nvec) weight_chunk<VEC>(a.w, a.w_bf16, c, w[j]);
+    if (c < nvec) weight_lanes<VEC>(a.w, a.w_bf16, c, w[j]);
   }
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
        base += (int64_t)gridDim.x * per) {
@@ -157,55 +178,58 @@ norm_forward_kernel(const NormArgs a) {
         if (live && c < nvec) cr[j].load(r + off + (int64_t)c * VEC);
       }
     }
-    float ss = 0.f;
+    L sum = splat<VEC>(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
-      float v[VEC];
-      cx[j].get(v);
+      L v[NP];
+      get_lanes(cx[j], v);
       if (r) {
-        float u[VEC];
-        cr[j].get(u);
+        L u[NP];
+        get_lanes(cr[j], u);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] += u[i];
-        cx[j].put(v);  // the stream, rounded to its type
+        for (int i = 0; i < NP; ++i) v[i] = v[i] + u[i];
+        put_lanes(cx[j], v);  // the stream, rounded to its type
         if (live && c < nvec) cx[j].store(reinterpret_cast<T *>(a.h) + off + (int64_t)c * VEC);
-        cx[j].get(v);
+        get_lanes(cx[j], v);
       }
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) ss = fmaf(v[i], v[i], ss);
+      for (int i = 0; i < NP; ++i) sum = fma(v[i], v[i], sum);
     }
-    ss = group_reduce<G, SumOp>(ss, scratch);
+    const float ss = group_reduce<G, SumOp>(lane_sum(sum), scratch);
     const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
     if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
-    float amax = 0.f, scale = 0.f;
-    if (FP8) {
+    if (FP8) {  // y = rstd t, t = h w
+      L t[NV][NP];
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        if (lane + j * g >= nvec) continue;
+        get_lanes(cx[j], t[j]);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) t[j][i] = t[j][i] * w[j][i];
+        m = chunk_magnitude<VEC>(m, t[j]);
+      }
+      m = group_reduce<G, MaxMagnitudeOp>(m, scratch);
+      float k;
+      const float scale = e4m3_scale(m, rstd, k);
+      if (live && lane == 0) a.scales[row] = scale;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = lane + j * g;
-        if (c >= nvec) continue;
-        float v[VEC];
-        cx[j].get(v);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          amax = MaxNanOp::of(amax, fabsf(v[i] * rstd * w[j][i]));
+        if (live && c < nvec) store_e4m3<VEC>(a.q + off + (int64_t)c * VEC, t[j], k);
       }
-      amax = group_reduce<G, MaxNanOp>(amax, scratch);
-      scale = amax / kE4m3Max;
-      if (live && lane == 0) a.scales[row] = scale;
-    }
+    } else {
+      const L f = splat<VEC>(rstd);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = lane + j * g;
-      if (!live || c >= nvec) continue;
-      float v[VEC];
-      cx[j].get(v);
+      for (int j = 0; j < NV; ++j) {
+        const int c = lane + j * g;
+        if (!live || c >= nvec) continue;
+        L v[NP];
+        get_lanes(cx[j], v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = v[i] * rstd * w[j][i];
-      if (FP8) {
-        store_e4m3<VEC>(a.q + off + (int64_t)c * VEC, v, scale);
-      } else {
-        cx[j].put(v);
+        for (int i = 0; i < NP; ++i) v[i] = v[i] * f * w[j][i];
+        put_lanes(cx[j], v);
         cx[j].store(reinterpret_cast<T *>(a.y) + off + (int64_t)c * VEC);
       }
     }
@@ -235,21 +259,23 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
     ss = group_reduce<0, SumOp>(ss, scratch);
     const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
-    float scale = 0.f;
+    float k = 0.f;
     if (FP8) {
-      float amax = 0.f;
+      float m = 0.f;
       for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x)
-        amax = MaxNanOp::of(amax, fabsf(load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c)));
-      amax = group_reduce<0, MaxNanOp>(amax, scratch);
-      scale = amax / kE4m3Max;
+        m = MaxMagnitudeOp::of(m, fabsf(load_f(h, off + c) * weight_at(a.w, a.w_bf16, c)));
+      m = group_reduce<0, MaxMagnitudeOp>(m, scratch);
+      const float scale = e4m3_scale(m, rstd, k);
       if (threadIdx.x == 0) a.scales[row] = scale;
     }
     for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
-      const float v = load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c);
-      if (FP8)
-        store_e4m3<1>(a.q + off + c, &v, scale);
-      else
-        store_f(reinterpret_cast<T *>(a.y), off + c, v);
+      const float v = load_f(h, off + c), w = weight_at(a.w, a.w_bf16, c);
+      if (FP8) {
+        const Single t{v * w};
+        store_e4m3<1>(a.q + off + c, &t, k);
+      } else {
+        store_f(reinterpret_cast<T *>(a.y), off + c, v * rstd * w);
+      }
     }
   }
 }
@@ -262,15 +288,15 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t
                      float *scales) {
   __shared__ float scratch[33];
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    float amax = 0.f;
+    float m = 0.f, k;
     for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
-      amax = MaxNanOp::of(amax, fabsf(load_f(x, row * dim + c)));
-    amax = group_reduce<0, MaxNanOp>(amax, scratch);
-    const float scale = amax / kE4m3Max;
+      m = MaxMagnitudeOp::of(m, fabsf(load_f(x, row * dim + c)));
+    m = group_reduce<0, MaxMagnitudeOp>(m, scratch);
+    const float scale = e4m3_scale(m, 1.f, k);
     if (threadIdx.x == 0) scales[row] = scale;
     for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
-      const float v = load_f(x, row * dim + c);
-      store_e4m3<1>(q + row * dim + c, &v, scale);
+      const Single v{load_f(x, row * dim + c)};
+      store_e4m3<1>(q + row * dim + c, &v, k);
     }
   }
 }
@@ -295,11 +321,13 @@ norm_backward_kernel(const NormGradArgs a) {
   const int nvec = (int)(a.dim / VEC);
   const T *hp = reinterpret_cast<const T *>(a.h), *dyp = reinterpret_cast<const T *>(a.dy);
   const T *dhp = reinterpret_cast<const T *>(a.dh);
-  float dw[NV][VEC];
+  constexpr int NP = lanes_of<VEC>();
+  using L = Lanes<VEC>;
+  L dwp[NV][NP];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
+    for (int i = 0; i < NP; ++i) dwp[j][i] = splat<VEC>(0.f);
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
        base += (int64_t)gridDim.x * per) {
     const int64_t row = base + sub;
@@ -321,37 +349,42 @@ norm_backward_kernel(const NormGradArgs a) {
       }
     }
     const float rstd = live ? __ldg(a.rstd + row) : 0.f;
-    float dot = 0.f;
+    const L f = splat<VEC>(rstd);
+    L sum = splat<VEC>(0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       if (c >= nvec) continue;
-      float h[VEC], dy[VEC], w[VEC];
-      ch[j].get(h), cy[j].get(dy);
-      weight_chunk<VEC>(a.w, a.w_bf16, c, w);
+      L h[NP], dy[NP], w[NP];
+      get_lanes(ch[j], h), get_lanes(cy[j], dy);
+      weight_lanes<VEC>(a.w, a.w_bf16, c, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float t = dy[i] * (h[i] * rstd);
-        dw[j][i] += t;
-        dot = fmaf(t, w[i], dot);
+      for (int i = 0; i < NP; ++i) {
+        const L t = dy[i] * (h[i] * f);
+        dwp[j][i] = dwp[j][i] + t;
+        sum = fma(t, w[i], sum);
       }
     }
-    dot = group_reduce<G, SumOp>(dot, scratch);
-    const float k = dot / (float)a.dim * rstd;
+    const float dot = group_reduce<G, SumOp>(lane_sum(sum), scratch);
+    const float k = -dot / (float)a.dim * rstd;
+    const L minus = splat<VEC>(k);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       if (!live || c >= nvec) continue;
-      float h[VEC], dy[VEC], s[VEC], w[VEC];
-      ch[j].get(h), cy[j].get(dy), cs[j].get(s);
-      weight_chunk<VEC>(a.w, a.w_bf16, c, w);
+      L h[NP], dy[NP], s[NP], w[NP];
+      get_lanes(ch[j], h), get_lanes(cy[j], dy), get_lanes(cs[j], s);
+      weight_lanes<VEC>(a.w, a.w_bf16, c, w);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[i] = fmaf(rstd, dy[i] * w[i] - h[i] * k, s[i]);
-      cs[j].put(s);
+      for (int i = 0; i < NP; ++i) s[i] = fma(f, fma(h[i], minus, dy[i] * w[i]), s[i]);
+      put_lanes(cs[j], s);
       cs[j].store(reinterpret_cast<T *>(a.dx) + off + (int64_t)c * VEC);
     }
   }
   if (!a.partial) return;
+  float dw[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) from_lanes<VEC>(dwp[j], dw[j]);
   float *out = a.partial + (int64_t)blockIdx.x * a.dim;
   if (G == 0) {
 #pragma unroll
@@ -467,7 +500,9 @@ NormPlan norm_plan(int64_t rows, int64_t dim, int elem, bool aligned, int blocks
     p.threads = kWideThreads;
   }
   p.groups = cdiv(rows, per);
-  p.blocks = (int)std::min<int64_t>(p.groups, (int64_t)sm_count() * blocks_per_sm);
+  // more blocks of few threads
+  const int most = blocks_per_sm * std::max(1, 256 / p.threads);
+  p.blocks = (int)std::min<int64_t>(p.groups, (int64_t)sm_count() * most);
   return p;
 }
 

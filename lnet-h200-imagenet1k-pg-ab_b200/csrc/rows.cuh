@@ -2,6 +2,8 @@
 // scalar chunks of a row in fp32, reductions over a group of lanes or a block.
 #pragma once
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace lnet {
@@ -94,11 +96,11 @@ struct SumOp {
   static __device__ __forceinline__ float id() { return 0.f; }
   static __device__ __forceinline__ float of(float a, float b) { return a + b; }
 };
-// Maximum that keeps a NaN of either side.
-struct MaxNanOp {
-  static __device__ __forceinline__ float id() { return 0.f; }  // of absolute values
+// Of magnitudes, as the integers that their bits are: a NaN is above infinity and stays.
+struct MaxMagnitudeOp {
+  static __device__ __forceinline__ float id() { return 0.f; }
   static __device__ __forceinline__ float of(float a, float b) {
-    return (a != a || a > b) ? a : b;
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
   }
 };
 
@@ -108,8 +110,12 @@ struct MaxNanOp {
 template <int G, typename Op>
 __device__ __forceinline__ float group_reduce(float v, float *scratch) {
   constexpr int W = G == 0 ? 32 : G;
+  if (W == 32 && std::is_same<Op, MaxMagnitudeOp>::value) {
+    v = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(v)));
+  } else {
 #pragma unroll
-  for (int o = W / 2; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+    for (int o = W / 2; o > 0; o >>= 1) v = Op::of(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  }
   if (G == 0) {
     const int warps = blockDim.x >> 5;
     if (warps == 1) return v;
@@ -161,6 +167,63 @@ __device__ __forceinline__ Pair exp2_fast(Pair x) {
   float a, b;
   unpair(x, a, b);
   return pair(exp2_fast(a), exp2_fast(b));
+}
+
+// A chunk in the form that is computed with: pairs, or its one element.
+struct Single {
+  float v;
+};
+__device__ __forceinline__ Single operator+(Single a, Single b) { return {a.v + b.v}; }
+__device__ __forceinline__ Single operator*(Single a, Single b) { return {a.v * b.v}; }
+__device__ __forceinline__ Single fma(Single a, Single b, Single c) { return {fmaf(a.v, b.v, c.v)}; }
+template <int VEC>
+using Lanes = std::conditional_t<VEC == 1, Single, Pair>;
+template <int VEC>
+__host__ __device__ constexpr int lanes_of() {
+  return VEC == 1 ? 1 : VEC / 2;
+}
+template <int VEC>
+__device__ __forceinline__ Lanes<VEC> splat(float v) {
+  if constexpr (VEC == 1)
+    return Single{v};
+  else
+    return pair(v, v);
+}
+template <int VEC>
+__device__ __forceinline__ void to_lanes(const float *v, Lanes<VEC> *p) {
+  if constexpr (VEC == 1) {
+    p[0].v = v[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) p[i] = pair(v[2 * i], v[2 * i + 1]);
+  }
+}
+template <int VEC>
+__device__ __forceinline__ void from_lanes(const Lanes<VEC> *p, float *v) {
+  if constexpr (VEC == 1) {
+    v[0] = p[0].v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC / 2; ++i) unpair(p[i], v[2 * i], v[2 * i + 1]);
+  }
+}
+__device__ __forceinline__ float lane_sum(Single a) { return a.v; }
+__device__ __forceinline__ float lane_sum(Pair a) {
+  float x, y;
+  unpair(a, x, y);
+  return x + y;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void get_lanes(const RowChunk<T, VEC> &c, Lanes<VEC> *p) {
+  float v[VEC];
+  c.get(v);
+  to_lanes<VEC>(v, p);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void put_lanes(RowChunk<T, VEC> &c, const Lanes<VEC> *p) {
+  float v[VEC];
+  from_lanes<VEC>(p, v);
+  c.put(v);
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

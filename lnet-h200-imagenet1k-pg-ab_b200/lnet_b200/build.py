@@ -2,7 +2,10 @@
 
 ``build()`` compiles every ``csrc/*.cu`` with nvcc into
 ``lnet_b200/_lib/liblnet_b200.so`` (a C-ABI shared library loaded with
-ctypes).  Rebuilds only when a source or header is newer than the library.
+ctypes), and ``csrc/torch_ops.cpp`` (the host path of the feed-forward and
+distillation operators) with g++ against torch's headers into
+``lnet_b200/_lib/_torch_ops.so``.  Rebuilds only what a source or header is
+newer than.
 """
 
 from __future__ import annotations
@@ -10,6 +13,7 @@ from __future__ import annotations
 import os
 import shutil
 import subprocess
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -19,6 +23,8 @@ CSRC = ROOT / "csrc"
 INCLUDE = REPO / "include"
 LIB_DIR = PKG / "_lib"
 LIB = LIB_DIR / "liblnet_b200.so"
+TORCH_OPS_SOURCE = CSRC / "torch_ops.cpp"
+TORCH_OPS = LIB_DIR / "_torch_ops.so"
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
 
 
@@ -44,7 +50,43 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > mtime for p in _deps())
 
 
+def torch_ops_stale() -> bool:
+    if not TORCH_OPS.exists():
+        return True
+    mtime = TORCH_OPS.stat().st_mtime
+    return any(p.stat().st_mtime > mtime for p in (TORCH_OPS_SOURCE, *INCLUDE.glob("*.h")))
+
+
+def _torch_ops_command(out: Path) -> list[str]:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc_path()).resolve().parents[1]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+            f"-I{root / 'include'}", f"-I{root / 'include/torch/csrc/api/include'}",
+            f"-I{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}",
+            str(TORCH_OPS_SOURCE), "-o", str(out), f"-L{root / 'lib'}", "-ltorch", "-ltorch_cpu",
+            "-ltorch_python", "-lc10", "-lc10_cuda"]
+
+
+def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
+    if not force and not torch_ops_stale():
+        return TORCH_OPS
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = TORCH_OPS.with_suffix(f".so.{os.getpid()}.tmp")
+    cmd = _torch_ops_command(tmp)
+    if verbose:
+        print(" ".join(cmd))
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed: {' '.join(cmd)}\n{res.stdout}{res.stderr}")
+    os.replace(tmp, TORCH_OPS)
+    return TORCH_OPS
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
+    build_torch_ops(force, verbose)
     if not force and not needs_build():
         return LIB
     LIB_DIR.mkdir(parents=True, exist_ok=True)

@@ -9,14 +9,10 @@ rounded to the inputs' type (it is the stream that the next block reads) and
 
 from __future__ import annotations
 
-import ctypes
-from functools import lru_cache
-
 import torch
 from torch import Tensor
 
-from . import _lib
-from ._launch import DTYPES, call, pointer, require_cuda, single_backward, wants_grad
+from ._native import DTYPES, native, refuse_grad, require_cuda
 
 RMS_NORM_EPS = torch.finfo(torch.float32).eps  # nn.RMSNorm's default for fp32
 
@@ -44,71 +40,6 @@ def _check_norm_args(x: Tensor, weight: Tensor, residual: Tensor | None, eps: fl
         raise ValueError(f"eps must be >= 0, got {eps}")
 
 
-def _rows(x: Tensor) -> int:
-    return x.numel() // x.shape[-1]
-
-
-def _launch_norm(x: Tensor, weight: Tensor, residual: Tensor | None, eps: float,
-                 keep_rstd: bool) -> tuple[Tensor, Tensor | None, Tensor | None]:
-    """(y, stream or None without a residual, rstd or None) of contiguous tensors."""
-    y = torch.empty_like(x)
-    stream = None if residual is None else torch.empty_like(x)
-    rstd = (torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if keep_rstd
-            else None)
-    call(x.device, "lnet_b200_residual_rms_norm", x.data_ptr(), pointer(residual),
-         weight.data_ptr(), DTYPES[x.dtype], DTYPES[weight.dtype], _rows(x), x.shape[-1], eps,
-         y.data_ptr(), pointer(stream), pointer(rstd))
-    return y, stream, rstd
-
-
-@lru_cache(maxsize=256)
-def _workspace_bytes(dtype: int, rows: int, dim: int) -> int:
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.load().lnet_b200_residual_rms_norm_workspace_size(dtype, rows, dim,
-                                                                      ctypes.byref(n)),
-               "lnet_b200_residual_rms_norm_workspace_size")
-    return int(n.value)
-
-
-def _launch_norm_backward(stream: Tensor, rstd: Tensor, weight: Tensor, dy: Tensor,
-                          dstream: Tensor | None, want_weight: bool
-                          ) -> tuple[Tensor, Tensor | None]:
-    dx = torch.empty_like(stream)
-    dweight = torch.empty_like(weight) if want_weight else None
-    code = DTYPES[stream.dtype]
-    nbytes = _workspace_bytes(code, _rows(stream), stream.shape[-1]) if want_weight else 0
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=stream.device) if nbytes else None
-    call(stream.device, "lnet_b200_residual_rms_norm_backward", stream.data_ptr(),
-         rstd.data_ptr(), weight.data_ptr(), dy.data_ptr(), pointer(dstream), code,
-         DTYPES[weight.dtype], _rows(stream), stream.shape[-1], dx.data_ptr(), pointer(dweight),
-         pointer(ws), nbytes)
-    return dx, dweight
-
-
-class _ResidualRmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        xc, wc = x.contiguous(), weight.contiguous()
-        rc = None if residual is None else residual.contiguous()
-        y, stream, rstd = _launch_norm(xc, wc, rc, eps, True)
-        ctx.save_for_backward(xc if stream is None else stream, wc, rstd)
-        ctx.set_materialize_grads(False)
-        return y, x if stream is None else stream  # without a residual the stream is x itself
-
-    @staticmethod
-    @single_backward
-    def backward(ctx, dy, dstream):
-        stream, weight, rstd = ctx.saved_tensors
-        need_x, need_w, need_r, _ = ctx.needs_input_grad
-        if dy is None:
-            return (dstream if need_x else None, torch.zeros_like(weight) if need_w else None,
-                    dstream if need_r else None, None)
-        dx, dweight = _launch_norm_backward(
-            stream, rstd, weight, dy.contiguous(),
-            None if dstream is None else dstream.contiguous(), need_w)
-        return dx if need_x else None, dweight, dx if need_r else None, None
-
-
 def residual_rms_norm(x: Tensor, weight: Tensor, residual: Tensor | None = None,
                       eps: float = RMS_NORM_EPS) -> tuple[Tensor, Tensor]:
     """``(y, stream)``: ``stream = x + residual`` (``x`` itself without one) and its RMSNorm
@@ -119,11 +50,7 @@ def residual_rms_norm(x: Tensor, weight: Tensor, residual: Tensor | None = None,
     """
     _check_norm_args(x, weight, residual, eps)
     require_cuda("residual_rms_norm", x)
-    if wants_grad(x, weight, residual):
-        return _ResidualRmsNorm.apply(x, weight, residual, eps)
-    y, stream, _ = _launch_norm(x.contiguous(), weight.contiguous(),
-                                None if residual is None else residual.contiguous(), eps, False)
-    return y, x if stream is None else stream
+    return native().norm(x, weight, residual, eps)
 
 
 def residual_rms_norm_fp8(x: Tensor, weight: Tensor, residual: Tensor | None = None,
@@ -137,17 +64,8 @@ def residual_rms_norm_fp8(x: Tensor, weight: Tensor, residual: Tensor | None = N
     """
     _check_norm_args(x, weight, residual, eps)
     require_cuda("residual_rms_norm_fp8", x)
-    if wants_grad(x, weight, residual):
-        raise RuntimeError("residual_rms_norm_fp8 has no gradient: call it under torch.no_grad()")
-    x, weight = x.contiguous(), weight.contiguous()
-    residual = None if residual is None else residual.contiguous()
-    values = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    stream = None if residual is None else torch.empty_like(x)
-    call(x.device, "lnet_b200_residual_rms_norm_fp8", x.data_ptr(), pointer(residual),
-         weight.data_ptr(), DTYPES[x.dtype], DTYPES[weight.dtype], _rows(x), x.shape[-1], eps,
-         values.data_ptr(), scales.data_ptr(), pointer(stream))
-    return values, scales, x if stream is None else stream
+    refuse_grad("residual_rms_norm_fp8", x, weight, residual)
+    return native().norm_fp8(x, weight, residual, eps)
 
 
 __all__ = ["RMS_NORM_EPS", "residual_rms_norm", "residual_rms_norm_fp8"]

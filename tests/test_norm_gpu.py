@@ -22,9 +22,11 @@ pytestmark = pytest.mark.gpu
 FP32 = 4e-6
 HALF_ULP = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2}
 DTYPES = [torch.float32, torch.bfloat16]
-# one element, a lane group of each size, odd widths, a block a row, and rows that no block holds
+# one element, a lane group of each size, odd widths, a block a row, rows that no block holds, and
+# enough rows for a warp a row
 SHAPES = [(1, 1), (1, 96), (7, 64), (300, 96), (5, 3, 128), (33, 257), (19, 1001), (64, 1024),
-          (9, 4096), (3, 8200), (2, 8193), (2, 16392), (2, 20001)]
+          (9, 4096), (3, 8200), (2, 8193), (2, 16392), (2, 20001), (1300, 2048), (1201, 4096),
+          (1211, 1544)]
 
 
 def make(shape, dtype, seed, device, std=1.0):
@@ -223,3 +225,12 @@ def test_fp8_refuses_a_gradient(cuda_device):
     x = make((4, 96), torch.bfloat16, 1, cuda_device).requires_grad_()
     with pytest.raises(RuntimeError, match="no gradient"):
         residual_rms_norm_fp8(x, torch.ones(96, device=cuda_device))
+
+
+def test_a_second_derivative_is_refused(cuda_device):
+    x = make((4, 96), torch.float32, 1, cuda_device).requires_grad_()
+    w = torch.ones(96, device=cuda_device, requires_grad=True)
+    y, _ = residual_rms_norm(x, w)
+    dx, = torch.autograd.grad(y.square().sum(), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="once"):
+        dx.sum().backward()
