@@ -23,6 +23,8 @@ Laplace layer behind the reference ``lnet`` module API.
   output.
 * :mod:`lnet_b200.linear` — matrix product with bias, activation and residual in
   its epilogue, its gradient, and its form on 8-bit operands.
+* :class:`B200FeedForward` — a feed-forward block of these, trained in bf16 and
+  served in 8 bits.
 * :mod:`lnet_b200.distill` — distillation loss against a teacher's top logits.
 * :mod:`lnet_b200.graph` — CUDA-graph capture and replay of a prepared forward.
 
@@ -33,6 +35,7 @@ All compute runs in the C-ABI CUDA library ``_lib/liblnet_b200.so`` built by
 from . import ops  # registers the lnet_b200:: custom ops
 from .alphabet import AlphabetConfig, B200Alphabet
 from .distill import distillation_loss
+from .feedforward import B200FeedForward
 from .inference import prepare_compiled_inference, prepare_maskless_inference
 from .train_runtime import (
     AlphabetTrainingRuntime,
@@ -51,6 +54,7 @@ __all__ = [
     "AlphabetConfig",
     "AlphabetTrainingRuntime",
     "B200Alphabet",
+    "B200FeedForward",
     "B200PoleResidueTemporalMixing",
     "LaplaceParameterError",
     "LaplaceShapeError",

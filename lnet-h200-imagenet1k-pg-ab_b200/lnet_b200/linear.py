@@ -42,6 +42,18 @@ def _check_linear_args(x, weight, bias, residual, activation, operand) -> None:
         raise ValueError(f"activation must be one of {tuple(ACTIVATIONS)}, got {activation!r}")
 
 
+def _check_linear_fp8_args(x, x_scale, weight, weight_scale, bias, residual, activation) -> None:
+    _check_linear_args(x, weight, bias, residual, activation, torch.float8_e4m3fn)
+    for name, t, shape in (("x_scale", x_scale, tuple(x.shape[:-1])),
+                           ("weight_scale", weight_scale, (weight.shape[0],))):
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be torch.float32, got {t.dtype}")
+        if t.device != x.device:
+            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+
+
 def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None,
                residual: Tensor | None = None, *, activation: str = "none") -> Tensor:
     """``f(x @ weight.T + bias) + residual`` for bfloat16 ``x`` [..., K] and ``weight`` [N, K].
@@ -63,15 +75,7 @@ def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Ten
     (:func:`lnet_b200.residual_rms_norm_fp8`, :func:`quantize_rows_fp8`); bias, residual and the
     result are bfloat16.  A serving form: it has no gradient and refuses inputs that want one.
     """
-    _check_linear_args(x, weight, bias, residual, activation, torch.float8_e4m3fn)
-    for name, t, shape in (("x_scale", x_scale, tuple(x.shape[:-1])),
-                           ("weight_scale", weight_scale, (weight.shape[0],))):
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
-        if t.dtype != torch.float32:
-            raise TypeError(f"{name} must be torch.float32, got {t.dtype}")
-        if t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, x on {x.device}")
+    _check_linear_fp8_args(x, x_scale, weight, weight_scale, bias, residual, activation)
     require_cuda("linear_act_fp8", x)
     refuse_grad("linear_act_fp8", x, x_scale, weight, weight_scale, bias, residual)
     return native().linear_fp8(x, x_scale, weight, weight_scale, bias, residual,

@@ -20,6 +20,12 @@ known output shape.  This module gives the B200 path the same surface:
   min_decay) -> y [B, T, D]`` — ``lnet_b200_laplace_forward``.
 * ``lnet_b200::patchify_images(images, mean, std, patch, dtype) -> tokens`` —
   ``lnet_b200_patchify_images``.
+* ``lnet_b200::residual_rms_norm``, ``linear_act``, ``distillation_loss`` and the
+  8-bit ``residual_rms_norm_fp8`` and ``linear_act_fp8`` — the calls of
+  :mod:`lnet_b200.norm`, :mod:`lnet_b200.linear` and :mod:`lnet_b200.distill`, the
+  first three with their gradients.  An op returns no input: without a residual
+  the norm's stream is an empty tensor (it is ``x``), and without an activation
+  the linear's pre-activation is.
 
 ``lnet_b200::alphabet_forward`` also carries ``register_autograd`` (the
 reference's ops register their VJPs the same way,
@@ -40,8 +46,12 @@ import torch
 from torch import Tensor
 
 from . import _lib
+from . import distill as _distill
 from . import images as _images
 from . import laplace as _laplace
+from . import linear as _linear
+from . import norm as _norm
+from ._native import native, require_cuda
 
 ALPHABET_WEIGHTS = tuple(_lib.PARAM_POINTER_FIELDS)
 ALPHABET_DIMS = ("raw_input_dim", "model_dim", "modes", "output_dim", "conv_kernel",
@@ -233,5 +243,192 @@ def _patchify_images_fake(images, mean, std, patch, dtype):
     return images.new_empty((b, (h // patch) * (w // patch), 3 * patch * patch), dtype=dtype)
 
 
-__all__ = ["ALPHABET_DIMS", "ALPHABET_WEIGHTS", "alphabet_forward", "laplace_forward",
-           "patchify_images"]
+def _none(t: Tensor) -> Tensor:
+    return t.new_empty(0)
+
+
+@torch.library.custom_op("lnet_b200::residual_rms_norm", mutates_args=())
+def residual_rms_norm(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None,
+                      eps: float = _norm.RMS_NORM_EPS) -> tuple[Tensor, Tensor, Tensor]:
+    """``(y, stream, rstd)`` of :func:`lnet_b200.residual_rms_norm` (``rstd`` [...] fp32)."""
+    _norm._check_norm_args(x, weight, residual, eps)
+    require_cuda("lnet_b200::residual_rms_norm", x)
+    y, stream, rstd = native().norm_forward(x, weight, residual, eps)
+    return y, _none(x) if stream is None else stream, rstd
+
+
+@residual_rms_norm.register_fake
+def _residual_rms_norm_fake(x, weight, residual=None, eps=_norm.RMS_NORM_EPS):
+    _norm._check_norm_args(x, weight, residual, eps)
+    stream = _none(x) if residual is None else x.new_empty(x.shape)
+    return x.new_empty(x.shape), stream, x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@torch.library.custom_op("lnet_b200::residual_rms_norm_backward", mutates_args=())
+def _residual_rms_norm_backward_op(stream: Tensor, rstd: Tensor, weight: Tensor, dy: Tensor,
+                                   dstream: Optional[Tensor]) -> tuple[Tensor, Tensor]:
+    dx, dweight = native().norm_backward(stream, rstd, weight, dy, dstream)
+    return dx, dweight
+
+
+@_residual_rms_norm_backward_op.register_fake
+def _residual_rms_norm_backward_fake(stream, rstd, weight, dy, dstream):
+    return stream.new_empty(stream.shape), weight.new_empty(weight.shape)
+
+
+def _residual_rms_norm_context(ctx, inputs, output):
+    x, weight, residual, _ = inputs
+    _, stream, rstd = output
+    ctx.residual = residual is not None
+    ctx.save_for_backward(stream if ctx.residual else x, rstd, weight)
+
+
+def _residual_rms_norm_gradient(ctx, dy, dstream, _):
+    stream, rstd, weight = ctx.saved_tensors
+    dx, dweight = torch.ops.lnet_b200.residual_rms_norm_backward(
+        stream, rstd, weight, dy, dstream if ctx.residual else None)
+    return dx, dweight, dx.clone() if ctx.residual else None, None
+
+
+residual_rms_norm.register_autograd(_residual_rms_norm_gradient,
+                                    setup_context=_residual_rms_norm_context)
+
+
+@torch.library.custom_op("lnet_b200::residual_rms_norm_fp8", mutates_args=())
+def residual_rms_norm_fp8(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None,
+                          eps: float = _norm.RMS_NORM_EPS) -> tuple[Tensor, Tensor, Tensor]:
+    """``(values, scales, stream)`` of :func:`lnet_b200.residual_rms_norm_fp8`."""
+    _norm._check_norm_args(x, weight, residual, eps)
+    require_cuda("lnet_b200::residual_rms_norm_fp8", x)
+    values, scales, stream = native().norm_fp8(x, weight, residual, eps)
+    return values, scales, _none(x) if residual is None else stream
+
+
+@residual_rms_norm_fp8.register_fake
+def _residual_rms_norm_fp8_fake(x, weight, residual=None, eps=_norm.RMS_NORM_EPS):
+    _norm._check_norm_args(x, weight, residual, eps)
+    stream = _none(x) if residual is None else x.new_empty(x.shape)
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            x.new_empty(x.shape[:-1], dtype=torch.float32), stream)
+
+
+@torch.library.custom_op("lnet_b200::linear_act", mutates_args=())
+def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
+               residual: Optional[Tensor] = None,
+               activation: str = "none") -> tuple[Tensor, Tensor]:
+    """``(y, pre-activation)`` of :func:`lnet_b200.linear_act`."""
+    _linear._check_linear_args(x, weight, bias, residual, activation, torch.bfloat16)
+    require_cuda("lnet_b200::linear_act", x)
+    y, pre = native().linear_forward(x, weight, bias, residual, _linear.ACTIVATIONS[activation])
+    return y, _none(x) if pre is None else pre
+
+
+@linear_act.register_fake
+def _linear_act_fake(x, weight, bias=None, residual=None, activation="none"):
+    _linear._check_linear_args(x, weight, bias, residual, activation, torch.bfloat16)
+    y = x.new_empty((*x.shape[:-1], weight.shape[0]))
+    return y, _none(x) if activation == "none" else x.new_empty(y.shape)
+
+
+@torch.library.custom_op("lnet_b200::linear_act_backward", mutates_args=())
+def _linear_act_backward_op(x: Tensor, weight: Tensor, activation: str, preact: Tensor,
+                            dy: Tensor) -> tuple[Tensor, Tensor, Tensor]:
+    code = _linear.ACTIVATIONS[activation]
+    dx, dweight, dbias = native().linear_backward(x, weight, code, preact if code else None, dy)
+    return dx, dweight, dbias
+
+
+@_linear_act_backward_op.register_fake
+def _linear_act_backward_fake(x, weight, activation, preact, dy):
+    return (x.new_empty(x.shape), weight.new_empty(weight.shape),
+            weight.new_empty(weight.shape[:1]))
+
+
+def _linear_act_context(ctx, inputs, output):
+    x, weight, bias, residual, ctx.activation = inputs
+    ctx.has = (bias is not None, residual is not None)
+    ctx.save_for_backward(x, weight, output[1])
+
+
+def _linear_act_gradient(ctx, dy, _):
+    x, weight, pre = ctx.saved_tensors
+    dx, dweight, dbias = torch.ops.lnet_b200.linear_act_backward(x, weight, ctx.activation, pre,
+                                                                 dy)
+    return dx, dweight, dbias if ctx.has[0] else None, dy if ctx.has[1] else None, None
+
+
+linear_act.register_autograd(_linear_act_gradient, setup_context=_linear_act_context)
+
+
+@torch.library.custom_op("lnet_b200::linear_act_fp8", mutates_args=())
+def linear_act_fp8(x: Tensor, x_scale: Tensor, weight: Tensor, weight_scale: Tensor,
+                   bias: Optional[Tensor] = None, residual: Optional[Tensor] = None,
+                   activation: str = "none") -> Tensor:
+    """:func:`lnet_b200.linear_act_fp8`."""
+    _linear._check_linear_fp8_args(x, x_scale, weight, weight_scale, bias, residual, activation)
+    require_cuda("lnet_b200::linear_act_fp8", x)
+    return native().linear_fp8(x, x_scale, weight, weight_scale, bias, residual,
+                               _linear.ACTIVATIONS[activation])
+
+
+@linear_act_fp8.register_fake
+def _linear_act_fp8_fake(x, x_scale, weight, weight_scale, bias=None, residual=None,
+                         activation="none"):
+    _linear._check_linear_fp8_args(x, x_scale, weight, weight_scale, bias, residual, activation)
+    return x.new_empty((*x.shape[:-1], weight.shape[0]), dtype=torch.bfloat16)
+
+
+@torch.library.custom_op("lnet_b200::distillation_loss", mutates_args=())
+def distillation_loss(logits: Tensor, teacher_indices: Tensor, teacher_logits: Tensor,
+                      labels: Optional[Tensor] = None, temperature: float = 1.0,
+                      alpha: float = 1.0, reduction: str = "mean") -> Tensor:
+    """:func:`lnet_b200.distillation_loss`; its gradient reads the logits again."""
+    _distill._check_distill_args(logits, teacher_indices, teacher_logits, labels, temperature,
+                                 alpha, reduction)
+    require_cuda("lnet_b200::distillation_loss", logits)
+    return native().distill(logits.detach(), teacher_indices, teacher_logits, labels, temperature,
+                            alpha, _distill.REDUCTIONS[reduction])
+
+
+@distillation_loss.register_fake
+def _distillation_loss_fake(logits, teacher_indices, teacher_logits, labels=None,
+                            temperature=1.0, alpha=1.0, reduction="mean"):
+    _distill._check_distill_args(logits, teacher_indices, teacher_logits, labels, temperature,
+                                 alpha, reduction)
+    shape = logits.shape[:-1] if reduction == "none" else ()
+    return logits.new_empty(shape, dtype=torch.float32)
+
+
+@torch.library.custom_op("lnet_b200::distillation_loss_backward", mutates_args=())
+def _distillation_loss_backward_op(logits: Tensor, teacher_indices: Tensor,
+                                   teacher_logits: Tensor, labels: Optional[Tensor],
+                                   temperature: float, alpha: float, reduction: str,
+                                   dloss: Tensor) -> Tensor:
+    return native().distill_backward(logits, teacher_indices, teacher_logits, labels, temperature,
+                                     alpha, _distill.REDUCTIONS[reduction], dloss)
+
+
+@_distillation_loss_backward_op.register_fake
+def _distillation_loss_backward_fake(logits, teacher_indices, teacher_logits, labels, temperature,
+                                     alpha, reduction, dloss):
+    return logits.new_empty(logits.shape)
+
+
+def _distillation_loss_context(ctx, inputs, output):
+    logits, indices, teacher, labels, *ctx.scalars = inputs
+    ctx.save_for_backward(logits, indices, teacher, labels)
+
+
+def _distillation_loss_gradient(ctx, dloss):
+    dlogits = torch.ops.lnet_b200.distillation_loss_backward(*ctx.saved_tensors, *ctx.scalars,
+                                                             dloss)
+    return dlogits, None, None, None, None, None, None
+
+
+distillation_loss.register_autograd(_distillation_loss_gradient,
+                                    setup_context=_distillation_loss_context)
+
+
+__all__ = ["ALPHABET_DIMS", "ALPHABET_WEIGHTS", "alphabet_forward", "distillation_loss",
+           "laplace_forward", "linear_act", "linear_act_fp8", "patchify_images",
+           "residual_rms_norm", "residual_rms_norm_fp8"]

@@ -7,7 +7,9 @@ import ctypes
 import pytest
 import torch
 
-from lnet_b200 import (_lib, distillation_loss, linear_act, linear_act_fp8, quantize_rows_fp8,
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from lnet_b200 import (B200FeedForward, _lib, distillation_loss, linear_act, linear_act_fp8, quantize_rows_fp8,
                        residual_rms_norm, residual_rms_norm_fp8)
 
 
@@ -153,3 +155,52 @@ def test_c_entries_refuse_before_any_cuda_call():
         assert lib.lnet_b200_linear_workspace_size(ctypes.byref(bad),
                                                    ctypes.byref(n)) == status, field
     assert lib.lnet_b200_distill_scale(None, 0, 4, p, None) == _lib.LNET_ERR_INVALID_ARGUMENT
+
+
+def test_ops_are_registered_and_functional():
+    for name in ("residual_rms_norm", "residual_rms_norm_fp8", "linear_act", "linear_act_fp8",
+                 "distillation_loss"):
+        schema = str(getattr(torch.ops.lnet_b200, name).default._schema)
+        assert "!" not in schema.split("->")[0], schema
+
+
+def test_fake_shapes_and_errors():
+    bf, e4 = torch.bfloat16, torch.float8_e4m3fn
+    ops = torch.ops.lnet_b200
+    with FakeTensorMode():
+        x, w = torch.empty(2, 5, 96, dtype=bf), torch.empty(96)
+        y, h, rstd = ops.residual_rms_norm(x, w, x)
+        assert y.shape == h.shape == x.shape and y.dtype == bf
+        assert rstd.shape == (2, 5) and rstd.dtype == torch.float32
+        assert ops.residual_rms_norm(x, w)[1].shape == (0,)
+        q, s, h = ops.residual_rms_norm_fp8(x, w, x)
+        assert q.dtype == e4 and s.shape == (2, 5) and h.shape == x.shape
+        up = torch.empty(384, 96, dtype=bf)
+        y, pre = ops.linear_act(x, up, activation="gelu")
+        assert y.shape == pre.shape == (2, 5, 384) and y.dtype == bf
+        assert ops.linear_act(x, up)[1].shape == (0,)
+        y = ops.linear_act_fp8(q, s, torch.empty(384, 96, dtype=e4), torch.empty(384))
+        assert y.shape == (2, 5, 384) and y.dtype == bf
+        z, ix = torch.empty(2, 5, 1000), torch.empty(2, 5, 8, dtype=torch.int64)
+        t = torch.empty(2, 5, 8)
+        assert ops.distillation_loss(z, ix, t).shape == ()
+        assert ops.distillation_loss(z, ix, t, None, 1.0, 1.0, "none").shape == (2, 5)
+        with pytest.raises(ValueError):
+            ops.residual_rms_norm(x, torch.empty(95))
+        with pytest.raises(TypeError):
+            ops.linear_act(x.float(), up)
+        with pytest.raises(ValueError):
+            ops.distillation_loss(z, ix, t[..., :7])
+
+
+def test_feedforward_module_on_cpu():
+    block = B200FeedForward(96, 384)
+    assert {n: tuple(p.shape) for n, p in block.named_parameters()} == {
+        "norm_weight": (96,), "up.weight": (384, 96), "up.bias": (384,),
+        "down.weight": (96, 384), "down.bias": (96,)}
+    with pytest.raises(RuntimeError, match="CUDA only"):
+        block(torch.zeros(2, 96, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        B200FeedForward(96, 0)
+    with pytest.raises(ValueError):
+        B200FeedForward(96, 384, activation="tanh")
