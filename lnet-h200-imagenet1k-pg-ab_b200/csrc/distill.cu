@@ -21,6 +21,8 @@
 // that join their sums through distributed shared memory.
 #include <cooperative_groups.h>
 
+#include <string.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -485,28 +487,33 @@ struct ResidentArgs {
   int divide;    // by the count
 };
 
-template <typename T, bool TWO, bool ALIGNED, int MAXT>
-__global__ void __launch_bounds__(MAXT, MAXT == kSmallThreads ? kSmallBlocks : 1)
+// NT: the block's threads where they are known, else 0.
+template <typename T, bool TWO, bool ALIGNED, int MAXT, int NV, int NT>
+__global__ void __launch_bounds__(MAXT, MAXT == kLargeThreads ? 1 : NV == 4 ? 4 : 3)
 distill_resident_kernel(const ResidentArgs ra) {
-  constexpr int VEC = vec_of<T>(), NV = kResident;
+  constexpr int VEC = vec_of<T>();
   const DistillArgs &a = ra.d;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   __shared__ float4 stats[2][kResidentParts * MAXT / 32];  // m, sum tau, sum 1
-  __shared__ uint64_t joined[2];
+  __shared__ uint64_t joined[2], landed[2];
+  extern __shared__ __align__(16) uint4 row_smem[];  // two parts of a row, in turn
   __shared__ int head[2][MAXT];   // a thread's first entry, or -1
   __shared__ int next[2][kEntries + 1];
   __shared__ Entry mine[2][kEntries + 1];
   __shared__ HeldRow held_set[32];
   __shared__ double loss_sums[MAXT / 32];
   __shared__ int last;
-  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
+  const int tid = threadIdx.x, nt = NT ? NT : blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
   const float kt = kLog2e / a.tau, inv_tau = 1.f / a.tau;
   const T *zb = reinterpret_cast<const T *>(a.z);
   T *db = reinterpret_cast<T *>(a.dz);
   const int classes = (int)a.classes, slots = (int)a.top + 1;
   head[0][tid] = head[1][tid] = -1;
-  if (tid < 2) sm100::mbar_init(joined + tid, warps);
+  if (tid < 2) {
+    sm100::mbar_init(joined + tid, warps);
+    sm100::mbar_init(landed + tid, 1);
+  }
   sm100::fence_barrier_init();
   bool failed = false;  // a wait gave up: NaN from then on
 
@@ -524,21 +531,36 @@ distill_resident_kernel(const ResidentArgs ra) {
     return ALIGNED ? 0
                    : (int)((reinterpret_cast<uintptr_t>(zb + row * a.classes) & 15) / sizeof(T));
   };
+  // Thread 0 asks for the whole chunks of a row's part: a bulk copy's unit is 16 bytes.
+  auto fetch_row = [&](int64_t row, int buffer) {
+    const int cut = shift_of(row);
+    const int c0 = part == 0 && cut ? 1 : part * nt * NV;
+    const int c1 = min(part * nt * NV + nt * NV, (classes + cut) / VEC);
+    if (c1 > c0) {
+      sm100::mbar_arrive_expect_tx(landed + buffer, (uint32_t)(c1 - c0) * 16);
+      sm100::bulk_load(sm100::smem_u32(row_smem + buffer * nt * NV + c0 - part * nt * NV),
+                       zb + row * a.classes + c0 * VEC - cut, (uint32_t)(c1 - c0) * 16,
+                       landed + buffer);
+    } else {
+      sm100::mbar_arrive(landed + buffer);
+    }
+  };
   RowChunk<T, VEC> cur[NV];
-  auto load_row = [&](RowChunk<T, VEC>(&k)[NV], int64_t row) {
+  auto load_row = [&](int64_t row, int buffer, int shift, bool whole) {
+    const uint4 *part_smem = row_smem + buffer * nt * NV + tid;
     const T *z = zb + row * a.classes;
-    const int shift = shift_of(row);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int e0 = (chunk0 + j * nt) * VEC - shift;
-      if (e0 >= 0 && e0 + VEC <= classes) {
-        k[j].load(z + e0);
+      if (whole || (e0 >= 0 && e0 + VEC <= classes)) {
+        const uint4 u = part_smem[j * nt];
+        memcpy(&cur[j].raw, &u, 16);
       } else {
         float v[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i)
           v[i] = !ALIGNED && e0 + i >= 0 && e0 + i < classes ? load_f(z, e0 + i) : -INFINITY;
-        k[j].put(v);
+        cur[j].put(v);
       }
     }
   };
@@ -572,6 +594,7 @@ distill_resident_kernel(const ResidentArgs ra) {
     __syncwarp();
     held_rows = 0;
   };
+  if (tid == 0 && first < a.rows) fetch_row(first, 0);
   int set = 0;
   uint32_t phase = 0;
   for (int64_t row = first; row < a.rows; row += step, phase ^= set, set ^= 1) {
@@ -579,14 +602,17 @@ distill_resident_kernel(const ResidentArgs ra) {
     const Entry *entries = ra.entries + row * slots;
     Entry e = tid < slots ? entries[tid] : Entry{-1, 0.f, 0.f};
     const RowInfo info = ra.info[row];
-    load_row(cur, row);
-    if (tid == 0 && row + step < a.rows) {  // whole chunks only: the copy's unit is 16 bytes
-      const T *next_row = zb + (row + step) * a.classes;
-      const int cut = shift_of(row + step);
-      const int c0 = part == 0 && cut ? 1 : part * nt * NV;
-      const int c1 = min(part * nt * NV + nt * NV, (classes + cut) / VEC);
-      if (c1 > c0) sm100::bulk_prefetch_l2(next_row + c0 * VEC - cut, (uint32_t)(c1 - c0) * 16);
-    }
+    if (tid == 0 && row + step < a.rows) fetch_row(row + step, set ^ 1);
+    if (!failed) failed = !sm100::mbar_wait_bounded(landed + set, phase, 1000000u);
+    // Most parts lie inside their row: without a check a chunk their loads and stores are one
+    // instruction each.
+    const int shift = shift_of(row);
+    const int lo = part * nt * NV * VEC - shift, hi = lo + nt * NV * VEC;
+    const bool whole = lo >= 0 && hi <= classes;
+    if (whole)
+      load_row(row, set, shift, true);
+    else
+      load_row(row, set, shift, false);
 
     // ---- exponentials relative to the thread's largest element
     Pair et[NV][VEC / 2], e1[TWO ? NV : 1][VEC / 2];
@@ -620,8 +646,6 @@ distill_resident_kernel(const ResidentArgs ra) {
     }
 
     // ---- entries of this block's classes, to the threads that hold them
-    const int shift = shift_of(row);
-    const int lo = part * nt * NV * VEC - shift, hi = lo + nt * NV * VEC;
     for (int j = tid; j < slots; j += nt) {
       if (j != tid) e = entries[j];
       if (e.index >= 0 && e.index >= lo && e.index < hi) {
@@ -698,26 +722,33 @@ distill_resident_kernel(const ResidentArgs ra) {
     const float ft = at * exp2_fast((m_own - st.m) * kt);
     const float f1 = TWO ? a1 * exp2_fast((m_own - st.m) * kLog2e) : 0.f;
     const Pair ft2 = pair(ft, ft), f12 = pair(f1, f1);
+    auto store_row = [&](bool whole_part) {
+      T *dpart = dz + chunk0 * VEC - shift;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e0 = (chunk0 + j * nt) * VEC - shift;
-      float v[VEC];
+      for (int j = 0; j < NV; ++j) {
+        float v[VEC];
 #pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) {
-        Pair g = ft2 * et[j][i];
-        if (TWO) g = fma(f12, e1[j][i], g);
-        unpair(g, v[2 * i], v[2 * i + 1]);
+        for (int i = 0; i < VEC / 2; ++i) {
+          Pair g = ft2 * et[j][i];
+          if (TWO) g = fma(f12, e1[j][i], g);
+          unpair(g, v[2 * i], v[2 * i + 1]);
+        }
+        const int e0 = (chunk0 + j * nt) * VEC - shift;
+        if (whole_part || (e0 >= 0 && e0 + VEC <= classes)) {
+          RowChunk<T, VEC> k;
+          k.put(v);
+          k.store(dpart + j * nt * VEC);
+        } else if (!ALIGNED) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (e0 + i >= 0 && e0 + i < classes) store_f(dz, e0 + i, v[i]);
+        }
       }
-      if (e0 >= 0 && e0 + VEC <= classes) {
-        RowChunk<T, VEC> k;
-        k.put(v);
-        k.store(dz + e0);
-      } else if (!ALIGNED) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          if (e0 + i >= 0 && e0 + i < classes) store_f(dz, e0 + i, v[i]);
-      }
-    }
+    };
+    if (whole)
+      store_row(true);
+    else
+      store_row(false);
     int j = head[set][tid];
     if (j >= 0) {
       head[set][tid] = -1;
@@ -869,7 +900,7 @@ DistillWork distill_work(Arena &ar, const lnet_b200_distill_request *q) {
 
 // Where the resident kernel serves a request: threads and blocks of a cluster.
 struct ResidentPlan {
-  int threads, parts;
+  int threads, parts, nv;
   bool aligned;
 };
 
@@ -882,17 +913,20 @@ bool resident_plan(const lnet_b200_distill_request *q, const void *dz, ResidentP
   // one chunk more where a row may start inside a chunk
   const int64_t chunks = cdiv(q->classes, VEC) + (p.aligned ? 0 : 1);
   // The smallest blocks that 8 of hold the row: 64 or 128 threads, then 256 or 512.
-  p.threads = 64, p.parts = 1;
-  auto holds = [&] { return chunks <= (int64_t)p.parts * p.threads * kResident; };
+  p.threads = 64, p.parts = 1, p.nv = 4;
+  auto holds = [&] { return chunks <= (int64_t)p.parts * p.threads * p.nv; };
   while (p.threads < kSmallThreads && !holds()) p.threads *= 2;
+  if (!holds()) p.nv = 8;
   while (p.parts < kResidentParts && !holds()) p.parts *= 2;
+  if (!holds()) p.nv = 4;
   while (p.threads < kLargeThreads && !holds()) p.threads *= 2;
   return holds();
 }
 
-template <typename T, bool TWO, bool ALIGNED, int MAXT>
+template <typename T, bool TWO, bool ALIGNED, int MAXT, int NV, int NT>
 int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
-  auto *kernel = distill_resident_kernel<T, TWO, ALIGNED, MAXT>;
+  constexpr auto kernel = &distill_resident_kernel<T, TWO, ALIGNED, MAXT, NV, NT>;
+  LNET_TRY(raise_shared_memory<kernel>(2 * MAXT * NV * 16, "distill_resident_kernel"));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -903,6 +937,7 @@ int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStre
   cfg.numAttrs = 1;
   cfg.blockDim = dim3(p.threads);
   cfg.gridDim = dim3(p.parts);
+  cfg.dynamicSmemBytes = 2 * p.threads * NV * 16;
   // Clusters that run at once: fewer than SMs / parts, since a cluster stays inside one group of
   // SMs.  A waiting cluster would double the time of a persistent grid.
   int clusters = 0;
@@ -939,9 +974,10 @@ template <typename T>
 int launch_resident(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
   auto sized = [&](auto two, auto aligned) {
     constexpr bool TWO = decltype(two)::value, ALIGNED = decltype(aligned)::value;
-    return p.threads <= kSmallThreads
-               ? launch_resident_typed<T, TWO, ALIGNED, kSmallThreads>(p, a, s)
-               : launch_resident_typed<T, TWO, ALIGNED, kLargeThreads>(p, a, s);
+    if (p.threads > kSmallThreads)
+      return launch_resident_typed<T, TWO, ALIGNED, kLargeThreads, 4, 0>(p, a, s);
+    return p.nv == 4 ? launch_resident_typed<T, TWO, ALIGNED, kSmallThreads, 4, 0>(p, a, s)
+                     : launch_resident_typed<T, TWO, ALIGNED, kSmallThreads, 8, kSmallThreads>(p, a, s);
   };
   if (two_temperatures(a.d))
     return p.aligned ? sized(std::true_type{}, std::true_type{})

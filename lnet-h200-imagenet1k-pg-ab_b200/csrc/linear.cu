@@ -16,7 +16,6 @@
 // TMA wants 16-byte aligned rows: an operand with other rows is first copied to
 // the workspace with its rows padded.
 #include <algorithm>
-#include <atomic>
 
 #include "gemm_tiles.cuh"
 #include "rows.cuh"
@@ -304,17 +303,8 @@ template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
 int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
                  cudaStream_t stream) {
   using S = TileShape<CTAS, BN, FP8>;
-  auto *kernel = tile_gemm_kernel<CTAS, BN, A_MN, B_MN, FP8>;
-  static std::atomic<uint64_t> ready{0};  // devices whose shared memory limit is raised
-  int dev = 0;
-  LNET_TRY(cuda_check(cudaGetDevice(&dev), "cudaGetDevice"));
-  const uint64_t bit = (uint64_t)1 << (dev & 63);
-  if (!(ready.load() & bit)) {
-    LNET_TRY(cuda_check(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM),
-        "tile_gemm_kernel shared memory"));
-    ready.fetch_or(bit);
-  }
+  constexpr auto kernel = &tile_gemm_kernel<CTAS, BN, A_MN, B_MN, FP8>;
+  LNET_TRY(raise_shared_memory<kernel>(S::SMEM, "tile_gemm_kernel shared memory"));
   LNET_TRY(tile_tensor_map(&args.a, a, FP8, kTileM));
   LNET_TRY(tile_tensor_map(&args.b, b, FP8, S::NB));
   cudaLaunchConfig_t cfg{};

@@ -2,6 +2,7 @@
 // scalar chunks of a row in fp32, reductions over a group of lanes or a block.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "common.cuh"
@@ -227,6 +228,20 @@ __device__ __forceinline__ void put_lanes(RowChunk<T, VEC> &c, const Lanes<VEC> 
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Raises a kernel's limit of dynamic shared memory on the current device, once a device.
+template <auto KERNEL>
+int raise_shared_memory(int bytes, const char *what) {
+  static std::atomic<uint64_t> ready{0};
+  int dev = 0;
+  LNET_TRY(cuda_check(cudaGetDevice(&dev), what));
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (ready.load() & bit) return LNET_OK;
+  LNET_TRY(cuda_check(
+      cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what));
+  ready.fetch_or(bit);
+  return LNET_OK;
+}
 
 // SMs of the current device (queried once per process; every GPU of a box is
 // the same part).
