@@ -329,18 +329,17 @@ constexpr int kEntries = 256;          // most entries of a row here; more take 
 constexpr int kPrepareThreads = 256;
 constexpr int kHasTeacher = 1, kHasLabel = 2, kBad = 4;
 
-struct alignas(16) Entry {
+struct Entry {
   int index;  // -1: nothing to do
-  float p, z;
+  float p;
 };
 struct RowInfo {
-  float plogp, pz;  // sum p log p, sum p z
-  float z_label;
+  float plogp;  // sum p log p
   int flags;
 };
 
 // NQ: entries of a lane.
-template <typename T, int NQ>
+template <int NQ>
 __global__ void __launch_bounds__(kPrepareThreads)
 distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *counts,
                        unsigned *done) {
@@ -352,15 +351,14 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
   int counted = 0;
   for (int64_t row = (int64_t)blockIdx.x * (kPrepareThreads / 32) + warp; row < a.rows;
        row += (int64_t)gridDim.x * (kPrepareThreads / 32)) {
-    const T *z = reinterpret_cast<const T *>(a.z) + row * a.classes;
     const int64_t label = a.labels ? a.labels[row] : -1;
     int index[NQ];
-    float t[NQ], zq[NQ];
+    float t[NQ];
     int flags = 0;
     float m = kLowest;
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-      index[q] = -1, t[q] = 0.f, zq[q] = 0.f;
+      index[q] = -1, t[q] = 0.f;
       if (q * 32 + lane >= top) continue;
       const int64_t ix = a.index[row * a.top + q * 32 + lane];
       t[q] = a.teacher[row * a.top + q * 32 + lane];
@@ -371,7 +369,6 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
         continue;
       }
       index[q] = (int)ix;
-      zq[q] = load_f(z, ix);
       m = fmaxf(m, t[q]);
     }
 #pragma unroll
@@ -393,22 +390,16 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
     const float log_s = logf(s);
-    float plogp = 0.f, pz = 0.f, merged[NQ];
+    float plogp = 0.f, merged[NQ];
     bool later[NQ];
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
       w[q] = index[q] < 0 ? 0.f : w[q] / s;
-      if (w[q] != 0.f) {
-        plogp = fmaf(w[q], (t[q] - m) / a.tau - log_s, plogp);
-        pz = fmaf(w[q], zq[q], pz);
-      }
+      if (w[q] != 0.f) plogp = fmaf(w[q], (t[q] - m) / a.tau - log_s, plogp);
       merged[q] = 0.f, later[q] = false;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      plogp += __shfl_xor_sync(0xFFFFFFFFu, plogp, o);
-      pz += __shfl_xor_sync(0xFFFFFFFFu, pz, o);
-    }
+    for (int o = 16; o > 0; o >>= 1) plogp += __shfl_xor_sync(0xFFFFFFFFu, plogp, o);
     float p_label = 0.f;
 #pragma unroll
     for (int src = 0; src < NQ; ++src) {
@@ -432,13 +423,12 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
       if (q * 32 + lane >= top) continue;
       // the label's place carries its own entry
       const bool dead = !teach || index[q] < 0 || later[q] || (lab && index[q] == label);
-      out[q * 32 + lane] = Entry{dead ? -1 : index[q], merged[q], zq[q]};
+      out[q * 32 + lane] = Entry{dead ? -1 : index[q], merged[q]};
     }
     if (lane == 0) {
       const bool in = lab && label < a.classes;
-      const float zl = in ? load_f(z, label) : 0.f;
-      out[top] = Entry{in ? (int)label : -1, teach ? p_label : 0.f, zl};
-      info[row] = RowInfo{plogp, pz, zl, flags};
+      out[top] = Entry{in ? (int)label : -1, teach ? p_label : 0.f};
+      info[row] = RowInfo{plogp, flags};
     }
   }
   if (lane == 0) warp_counts[warp] = counted;
@@ -471,11 +461,16 @@ constexpr int kSmallThreads = 128, kSmallBlocks = 4;
 constexpr int kLargeThreads = 512;
 constexpr int kResidentParts = 8;
 
+struct Listed {
+  int index;
+  float p, z;
+};
 struct HeldRow {
   RowStats stats;
   RowInfo info;
-  int64_t row;
+  float in_z;
   bool bad;
+  int64_t row;
 };
 
 struct ResidentArgs {
@@ -496,11 +491,13 @@ distill_resident_kernel(const ResidentArgs ra) {
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   __shared__ float4 stats[2][kResidentParts * MAXT / 32];  // m, sum tau, sum 1
+  // in block 0, of every warp's entries: sum of c (r - z), sum of c, r
+  __shared__ float4 shares[2][kResidentParts * MAXT / 32];
   __shared__ uint64_t joined[2], landed[2];
   extern __shared__ __align__(16) uint4 row_smem[];  // two parts of a row, in turn
   __shared__ int head[2][MAXT];   // a thread's first entry, or -1
   __shared__ int next[2][kEntries + 1];
-  __shared__ Entry mine[2][kEntries + 1];
+  __shared__ Listed mine[2][kEntries + 1];
   __shared__ HeldRow held_set[32];
   __shared__ double loss_sums[MAXT / 32];
   __shared__ int last;
@@ -580,15 +577,12 @@ distill_resident_kernel(const ResidentArgs ra) {
       const RowStats &s = held.stats;
       const float s_one = TWO ? s.s1 : s.st;
       float loss = 0.f;
-      if (held.info.flags & kHasTeacher) {
-        // sum p (log p - log q), log q = (z - m) / tau - log S
-        const float plogq = (held.info.pz - s.m) * inv_tau - logf(s.st);
-        loss = a.alpha * a.tau * a.tau * (s.st == 0.f ? INFINITY : held.info.plogp - plogq);
-      }
-      if (held.info.flags & kHasLabel)
-        loss += (1.f - a.alpha) * (held.info.z_label == -INFINITY
-                                       ? INFINITY
-                                       : logf(s_one) + (s.m - held.info.z_label));
+      if (held.info.flags & kHasTeacher)
+        loss = a.alpha * a.tau * a.tau * (held.info.plogp + logf(s.st));
+      if (held.info.flags & kHasLabel) loss += (1.f - a.alpha) * logf(s_one);
+      loss += held.in_z;
+      // nothing left of the row: log q = -inf
+      if (s.st == 0.f && (held.info.flags & (kHasTeacher | kHasLabel))) loss = INFINITY;
       a.loss[held.row] = held.bad ? NAN : loss;
     }
     __syncwarp();
@@ -600,7 +594,7 @@ distill_resident_kernel(const ResidentArgs ra) {
   for (int64_t row = first; row < a.rows; row += step, phase ^= set, set ^= 1) {
     T *dz = db + row * a.classes;
     const Entry *entries = ra.entries + row * slots;
-    Entry e = tid < slots ? entries[tid] : Entry{-1, 0.f, 0.f};
+    Entry e = tid < slots ? entries[tid] : Entry{-1, 0.f};
     const RowInfo info = ra.info[row];
     if (tid == 0 && row + step < a.rows) fetch_row(row + step, set ^ 1);
     if (!failed) failed = !sm100::mbar_wait_bounded(landed + set, phase, 1000000u);
@@ -646,11 +640,30 @@ distill_resident_kernel(const ResidentArgs ra) {
     }
 
     // ---- entries of this block's classes, to the threads that hold them
+    // With sum p = 1 the loss is alpha tau^2 (sum p log p + log S_tau) + (1 - alpha) log S_1
+    // + sum c (m - z), c = alpha tau p of an entry and 1 - alpha of the label: the last sum from
+    // here, against the largest z of the warp's entries first (masks of the type's lowest value
+    // cancel exactly).
+    float share_z = 0.f, share_c = 0.f, share_r = kLowest;
+    const bool has_l = (info.flags & kHasLabel) != 0;
     for (int j = tid; j < slots; j += nt) {
       if (j != tid) e = entries[j];
       if (e.index >= 0 && e.index >= lo && e.index < hi) {
-        mine[set][j] = e;
-        next[set][j] = atomicExch(&head[set][((e.index - lo) / VEC) & (nt - 1)], j);
+        const int at_part = e.index - lo, e0 = at_part / VEC * VEC + lo;  // its chunk's first
+        const bool held_here = whole || (e0 >= 0 && e0 + VEC <= classes);
+        const float zq =
+            held_here ? load_f(reinterpret_cast<const T *>(row_smem + set * nt * NV), at_part)
+                      : load_f(zb + row * a.classes, e.index);
+        const float c =
+            a.alpha * a.tau * e.p + (j == slots - 1 && has_l ? 1.f - a.alpha : 0.f);
+        if (c != 0.f) {
+          const float r = fmaxf(share_r, zq);
+          if (share_c != 0.f) share_z = fmaf(share_c, r - share_r, share_z);
+          share_z = fmaf(c, r - zq, share_z);
+          share_c += c, share_r = r;
+        }
+        mine[set][j] = Listed{e.index, e.p, zq};
+        next[set][j] = atomicExch(&head[set][(at_part / VEC) & (nt - 1)], j);
       }
     }
 
@@ -665,8 +678,21 @@ distill_resident_kernel(const ResidentArgs ra) {
         st.st += __shfl_xor_sync(0xFFFFFFFFu, st.st, o);
         if (TWO) st.s1 += __shfl_xor_sync(0xFFFFFFFFu, st.s1, o);
       }
+      if (warp * 32 < slots) {
+        const float r = warp_max(share_r);
+        if (share_c != 0.f) share_z = fmaf(share_c, r - share_r, share_z);
+        share_r = r;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          share_z += __shfl_xor_sync(0xFFFFFFFFu, share_z, o);
+          share_c += __shfl_xor_sync(0xFFFFFFFFu, share_c, o);
+        }
+      }
       if (parts == 1) {
-        if (lane == 0) stats[set][warp] = make_float4(st.m, st.st, st.s1, 0.f);
+        if (lane == 0) {
+          stats[set][warp] = make_float4(st.m, st.st, st.s1, 0.f);
+          shares[set][warp] = make_float4(share_z, share_c, share_r, 0.f);
+        }
         __syncthreads();
       } else {
         __syncwarp();  // the warp's entries are listed before its arrival
@@ -674,8 +700,12 @@ distill_resident_kernel(const ResidentArgs ra) {
           sm100::store_async_rank(&stats[set][part * warps + warp], joined + set, lane, st.m,
                                   st.st, st.s1, 0.f);
         if (lane == 0) {
+          sm100::store_async_rank(&shares[set][part * warps + warp], joined + set, 0, share_z,
+                                  share_c, share_r, 0.f);
           if (warp == 0)
-            sm100::mbar_arrive_expect_tx(joined + set, (uint32_t)(parts * warps * sizeof(float4)));
+            sm100::mbar_arrive_expect_tx(
+                joined + set, (uint32_t)(parts * warps *
+                                         (part == 0 ? 2 : 1) * sizeof(float4)));
           else
             sm100::mbar_arrive(joined + set);
         }
@@ -703,13 +733,22 @@ distill_resident_kernel(const ResidentArgs ra) {
         if (TWO) st.s1 += __shfl_xor_sync(0xFFFFFFFFu, st.s1, o);
       }
     }
+    float in_z = 0.f;
+    if (a.loss && part == 0 && warp == 0) {
+      for (int i = lane; i < parts * warps; i += 32) {
+        const float4 b = shares[set][i];
+        if (b.y != 0.f) in_z += fmaf(b.y, st.m - b.z, b.x);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) in_z += __shfl_xor_sync(0xFFFFFFFFu, in_z, o);
+    }
     // a row that is -inf throughout: q = 0, log q = -inf
     const float s_one = TWO ? st.s1 : st.st;
     const float inv_t = st.st == 0.f ? 0.f : __fdividef(1.f, st.st);  // sums lie in [1, classes]
     const float inv_1 = s_one == 0.f ? 0.f : __fdividef(1.f, s_one);
-    const bool has_t = (info.flags & kHasTeacher) != 0, has_l = (info.flags & kHasLabel) != 0;
+    const bool has_t = (info.flags & kHasTeacher) != 0;
     const bool bad = (info.flags & kBad) != 0 || failed;
-    if (tid == 0) held_set[held_rows] = HeldRow{st, info, row, bad};
+    if (tid == 0) held_set[held_rows] = HeldRow{st, info, in_z, bad, row};
     if (++held_rows == 32) flush();
 
     // ---- the gradient
@@ -754,7 +793,7 @@ distill_resident_kernel(const ResidentArgs ra) {
       head[set][tid] = -1;
       if (!bad)
         for (; j >= 0; j = next[set][j]) {
-          const Entry own = mine[set][j];
+          const Listed own = mine[set][j];
           const float d = own.z - st.m;
           float g = at * exp2_fast(d * kt);
           if (TWO) g = fmaf(a1, exp2_fast(d * kLog2e), g);
@@ -956,16 +995,15 @@ bool two_temperatures(const DistillArgs &a) {
   return a.alpha != 0.f && a.labels && a.alpha != 1.f && a.tau != 1.f;
 }
 
-template <typename T>
 int launch_prepare(const DistillArgs &a, const DistillWork &w, int blocks, cudaStream_t s) {
   if (a.top <= 32)
-    distill_prepare_kernel<T, 1><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
+    distill_prepare_kernel<1><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
                                                                     w.done);
   else if (a.top <= 64)
-    distill_prepare_kernel<T, 2><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
+    distill_prepare_kernel<2><<<blocks, kPrepareThreads, 0, s>>>(a, w.entries, w.info, w.counts,
                                                                     w.done);
   else
-    distill_prepare_kernel<T, kEntries / 32><<<blocks, kPrepareThreads, 0, s>>>(
+    distill_prepare_kernel<kEntries / 32><<<blocks, kPrepareThreads, 0, s>>>(
         a, w.entries, w.info, w.counts, w.done);
   return after_launch("distill_prepare_kernel");
 }
@@ -1043,8 +1081,7 @@ int run_distill(const char *what, const lnet_b200_distill_request *q, void *work
   const bool bf16 = q->dtype == LNET_BF16;
   ResidentPlan plan{};
   if (bf16 ? resident_plan<__nv_bfloat16>(q, dz, plan) : resident_plan<float>(q, dz, plan)) {
-    LNET_TRY(bf16 ? launch_prepare<__nv_bfloat16>(a, w, n_counts, stream)
-                  : launch_prepare<float>(a, w, n_counts, stream));
+    LNET_TRY(launch_prepare(a, w, n_counts, stream));
     a.counts = w.counts, a.n_counts = n_counts;
     const ResidentArgs ra{a, w.entries, w.info, w.done, loss && reduce ? loss : nullptr, mean};
     return bf16 ? launch_resident<__nv_bfloat16>(plan, ra, stream)

@@ -99,7 +99,8 @@ def check(z, index, teacher, labels, tau, alpha, reduction, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("rows,classes,top", [(1, 1, 1), (5, 3, 2), (4, 10, 4), (37, 1000, 10),
                                               (6, 1001, 7), (9, 4099, 33), (300, 517, 5),
-                                              (3, 70001, 16), (5, 32768, 64), (1, 100003, 40)])
+                                              (3, 70001, 16), (5, 32768, 64), (1, 100003, 40),
+                                              (700, 4099, 80), (250, 8200, 200), (3, 9000, 300)])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_loss_and_gradient(rows, classes, top, dtype, reduction, cuda_device):
     z, index, teacher, labels = make(rows, classes, top, dtype, rows + classes, cuda_device)
@@ -178,6 +179,17 @@ def test_rows_that_leave_nothing(cuda_device):
     assert float(dz[3, 4]) == pytest.approx(-0.5) and float(dz[3, 0]) == pytest.approx(1 / 19)
     assert float(loss[4]) == pytest.approx(kl, rel=1e-5)
     assert float(loss[5]) == 0 and bool((dz[5] == 0).all())
+    # the same rows through the kernels that take loss and gradient together
+    ok = torch.tensor([0, 1, 4, 5], device=cuda_device)
+    z3 = z.detach()[ok].clone().requires_grad_()
+    total = distillation_loss(z3, index[ok], teacher[ok], reduction="sum")
+    assert float(total.detach()) == pytest.approx(2 * kl, rel=1e-5)
+    assert torch.allclose(torch.autograd.grad(total, z3)[0], dz[ok])
+    for i in (2, 3):
+        zi = z.detach()[i:i + 1].clone().requires_grad_()
+        total = distillation_loss(zi, index[i:i + 1], teacher[i:i + 1], reduction="sum")
+        assert float(total.detach()) == inf
+        assert torch.allclose(torch.autograd.grad(total, zi)[0], dz[i:i + 1])
     none = torch.full((6, 2), -1, device=cuda_device)
     z2 = z.detach().clone().requires_grad_()
     total = distillation_loss(z2, none, teacher)
@@ -191,6 +203,10 @@ def test_infinite_and_nan_logits(cuda_device):
     index = torch.zeros(3, 1, dtype=torch.int64, device=cuda_device)
     loss = distillation_loss(z, index, torch.zeros(3, 1, device=cuda_device), reduction="none")
     assert bool(loss[:2].isnan().all()) and float(loss[2]) == pytest.approx(math.log(8), rel=1e-5)
+    z.requires_grad_()
+    total = distillation_loss(z, index, torch.zeros(3, 1, device=cuda_device))
+    dz, = torch.autograd.grad(total, z)
+    assert bool(total.isnan()) and bool(dz[:2].isnan().all()) and bool(torch.isfinite(dz[2]).all())
 
 
 def test_an_index_past_the_classes_is_nan_and_stays_in_its_row(cuda_device):
