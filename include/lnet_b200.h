@@ -482,8 +482,9 @@ int lnet_b200_residual_rms_norm_backward(const void *stream_in, const float *rst
  *   y = f(a) + residual,  f: 0 identity, 1 ReLU, 2 SiLU, 3 GELU (erf).
  * `dtype` is the operands' type: LNET_BF16, or LNET_E4M3 with a scale for every row
  * of x and of weight.  bias, residual, y are bf16; bias and residual may be NULL.
- * Sums are fp32, y is rounded once.  Operands whose rows do not start on 16-byte
- * boundaries are copied to the workspace first. */
+ * Sums are fp32, y is rounded once.  Rows of x and weight may lie further apart than
+ * `inner` (x_pitch, weight_pitch); where they do not start on 16-byte boundaries, the
+ * operand is copied to the workspace first (more than 8 rows). */
 typedef struct lnet_b200_linear_request {
   int64_t rows;
   int64_t inner;
@@ -496,7 +497,15 @@ typedef struct lnet_b200_linear_request {
   const void *residual;      /* [rows, outer] or NULL */
   const float *x_scale;      /* [rows] (8-bit operands) */
   const float *weight_scale; /* [outer] (8-bit operands) */
+  int64_t x_pitch;           /* elements between rows of x; 0: inner */
+  int64_t weight_pitch;      /* elements between rows of weight; 0: inner */
 } lnet_b200_linear_request;
+
+/* Rows of a bf16 or e4m3 matrix copied to another pitch (elements; zeros after `cols`), for
+ * operands that are used more than once and whose rows are not 16-byte aligned. */
+int lnet_b200_linear_pack(const void *src, int32_t dtype, int64_t rows, int64_t cols,
+                          int64_t src_pitch, void *dst, int64_t dst_pitch,
+                          lnet_stream_t stream);
 
 int lnet_b200_linear_workspace_size(const lnet_b200_linear_request *req, size_t *bytes);
 /* preact [rows, outer] bf16 receives a where it is not NULL: the gradient through an

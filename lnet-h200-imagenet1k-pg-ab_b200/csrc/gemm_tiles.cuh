@@ -227,8 +227,8 @@ __device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, int64_t M, 
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 s = *reinterpret_cast<const float4 *>(scale + j);
-      v[j] *= row_scale * s.x, v[j + 1] *= row_scale * s.y;
-      v[j + 2] *= row_scale * s.z, v[j + 3] *= row_scale * s.w;
+      v[j] = v[j] * row_scale * s.x, v[j + 1] = v[j + 1] * row_scale * s.y;
+      v[j + 2] = v[j + 2] * row_scale * s.z, v[j + 3] = v[j + 3] * row_scale * s.w;
     }
   }
   if (e.bias) {
@@ -441,6 +441,11 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
       if (in && w.split < 0) {  // while the accumulators are not there yet
         stage_columns(p.e, p.N, col0, COLS, bias, scale);
         if (p.e.row_scale && row0 + lane < p.M) rs = __ldg(p.e.row_scale + row0 + lane);
+        if (p.e.residual && row0 + lane < p.M) {  // the residual's lines on their way to L2
+          const __nv_bfloat16 *line = p.e.residual + (row0 + lane) * p.N + col0;
+          for (int c = 0; c < COLS && col0 + c < p.N; c += 64)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(line + c));
+        }
       }
       __syncwarp();
       if (ok) ok = wait(acc_full + acc, acc_phase);

@@ -31,7 +31,7 @@ constexpr int kSlopeLanes = 8, kSlopeBlocks = 4;  // row lanes and resident bloc
 struct VectorArgs {
   const void *x, *w;
   TileEpilogue e;
-  int64_t N, K;
+  int64_t N, K, x_pitch, w_pitch;
   int rows;
 };
 
@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs
   for (int r = 0; r < R; ++r) acc[r] = 0.f;
   if (VEC) {
     const uint4 *w = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.w) +
-                                                     col * p.K * ES);
+                                                     col * p.w_pitch * ES);
     const uint4 *x = reinterpret_cast<const uint4 *>(p.x);
     const int nc = (int)(p.K / E);
     for (int c0 = lane; c0 < nc; c0 += 32 * U) {
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs
         for (int r = 0; r < R; ++r) {
           if (r >= p.rows) break;
           float xv[E];
-          operand_values<FP8>(__ldg(x + (int64_t)r * nc + c0 + 32 * u), xv);
+          operand_values<FP8>(__ldg(x + r * (p.x_pitch / E) + c0 + 32 * u), xv);
 #pragma unroll
           for (int i = 0; i < E; ++i) acc[r] = fmaf(xv[i], wv[i], acc[r]);
         }
@@ -114,10 +114,10 @@ __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs
     }
   } else {
     for (int64_t k = lane; k < p.K; k += 32) {
-      const float wv = operand_value<FP8>(p.w, col * p.K + k);
+      const float wv = operand_value<FP8>(p.w, col * p.w_pitch + k);
 #pragma unroll
       for (int r = 0; r < R; ++r)
-        if (r < p.rows) acc[r] = fmaf(operand_value<FP8>(p.x, r * p.K + k), wv, acc[r]);
+        if (r < p.rows) acc[r] = fmaf(operand_value<FP8>(p.x, r * p.x_pitch + k), wv, acc[r]);
     }
   }
   float mine = 0.f;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs
 // Rows copied to a padded pitch (elements of ES bytes; the padding is zero).
 template <int ES>
 __global__ void __launch_bounds__(kPackThreads)
-pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols,
+pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols, int64_t src_pitch,
             uint8_t *__restrict__ dst, int64_t pitch) {
   const int64_t total = rows * pitch;
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
@@ -140,10 +140,10 @@ pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols,
     const int64_t r = i / pitch, c = i - r * pitch;
     if (ES == 2) {
       uint16_t v = 0;
-      if (c < cols) v = reinterpret_cast<const uint16_t *>(src)[r * cols + c];
+      if (c < cols) v = reinterpret_cast<const uint16_t *>(src)[r * src_pitch + c];
       reinterpret_cast<uint16_t *>(dst)[i] = v;
     } else {
-      dst[i] = c < cols ? src[r * cols + c] : 0;
+      dst[i] = c < cols ? src[r * src_pitch + c] : 0;
     }
   }
 }
@@ -284,9 +284,10 @@ ProductPlan product_plan(int64_t M, int64_t N, int kblocks) {
       if (splits > 1 && (tail == 0 || tail * splits > slots || kblocks / splits < 4)) break;
       double cost = kFill + waves * whole;
       if (tail) cost += s.block * cdiv(kblocks, splits) + 6;
-      // the sums are written and read once (about 6 TB/s), and one more kernel runs
+      // the sums are written and read once (about 6 TB/s), and one more kernel runs (5 us on the
+      // GPU and 3 on the host)
       const int64_t floats = splits > 1 ? tail * splits * s.ctas * kTileM * s.bn : 0;
-      if (splits > 1) cost += 45 + floats * 8 / 4.2e5;
+      if (splits > 1) cost += 90 + floats * 8 / 4.2e5;
       if (best_cost == 0 || cost < best_cost) {
         best_cost = cost;
         const int64_t full = splits > 1 ? waves * slots : tiles;
@@ -357,21 +358,32 @@ int product(const TileOperand &a, const TileOperand &b, const TileEpilogue &e, f
 
 bool tma_rows(const void *p, int64_t pitch_bytes) { return aligned16(p) && pitch_bytes % 16 == 0; }
 
-// `o` itself, or its copy with padded rows (element (i, j) of a rows x cols matrix).
+int launch_pack(const void *src, int64_t rows, int64_t cols, int64_t src_pitch, int elem, void *dst,
+                int64_t pitch, cudaStream_t s) {
+  const int64_t total = rows * pitch;
+  const int blocks = (int)std::min<int64_t>(cdiv(total, kPackThreads * 4), (int64_t)sm_count() * 16);
+  const auto *from = reinterpret_cast<const uint8_t *>(src);
+  auto *to = reinterpret_cast<uint8_t *>(dst);
+  if (elem == 2)
+    pack_kernel<2><<<blocks, kPackThreads, 0, s>>>(from, rows, cols, src_pitch, to, pitch);
+  else
+    pack_kernel<1><<<blocks, kPackThreads, 0, s>>>(from, rows, cols, src_pitch, to, pitch);
+  return after_launch("linear_pack_kernel");
+}
+
+// `o` itself, or its copy with padded rows (a rows x cols matrix in memory).
 int packed(TileOperand &o, int64_t rows, int64_t cols, int elem, void *copy, cudaStream_t s) {
   if (!copy) return LNET_OK;
   const int64_t pitch = (int64_t)align_up((size_t)cols * elem, 16) / elem;
-  const int64_t total = rows * pitch;
-  const int blocks = (int)std::min<int64_t>(cdiv(total, kPackThreads * 4), (int64_t)sm_count() * 16);
-  if (elem == 2)
-    pack_kernel<2><<<blocks, kPackThreads, 0, s>>>(reinterpret_cast<const uint8_t *>(o.ptr), rows,
-                                                   cols, reinterpret_cast<uint8_t *>(copy), pitch);
-  else
-    pack_kernel<1><<<blocks, kPackThreads, 0, s>>>(reinterpret_cast<const uint8_t *>(o.ptr), rows,
-                                                   cols, reinterpret_cast<uint8_t *>(copy), pitch);
+  LNET_TRY(launch_pack(o.ptr, rows, cols, o.pitch, elem, copy, pitch, s));
   o.ptr = copy;
   o.pitch = pitch;
-  return after_launch("linear_pack_kernel");
+  return LNET_OK;
+}
+
+int64_t x_pitch(const lnet_b200_linear_request *q) { return q->x_pitch ? q->x_pitch : q->inner; }
+int64_t w_pitch(const lnet_b200_linear_request *q) {
+  return q->weight_pitch ? q->weight_pitch : q->inner;
 }
 
 int check_linear(const char *what, const lnet_b200_linear_request *q) {
@@ -385,6 +397,10 @@ int check_linear(const char *what, const lnet_b200_linear_request *q) {
   if (cdiv(q->rows, 128) * cdiv(q->outer, 64) > most || cdiv(q->rows, 128) * cdiv(q->inner, 64) > most ||
       cdiv(q->outer, 128) * cdiv(q->inner, 64) > most)
     return fail(LNET_ERR_INVALID_ARGUMENT, "%s: a product has more than 2^30 tiles", what);
+  for (int64_t pitch : {x_pitch(q), w_pitch(q)})
+    if (pitch < q->inner || pitch > (int64_t)1 << 36)
+      return fail(LNET_ERR_INVALID_ARGUMENT, "%s: a pitch of %lld, inner %lld", what,
+                  (long long)pitch, (long long)q->inner);
   if (q->dtype != LNET_BF16 && q->dtype != LNET_E4M3)
     return fail(LNET_ERR_UNSUPPORTED, "%s: operands must be bf16 or e4m3", what);
   if (q->activation < kActNone || q->activation > kActGelu)
@@ -407,8 +423,8 @@ ForwardWork forward_work(Arena &ar, const lnet_b200_linear_request *q) {
   if (q->rows <= kVectorRows) return f;
   const int elem = q->dtype == LNET_BF16 ? 2 : 1;
   const size_t pitch = align_up((size_t)q->inner * elem, 16);
-  if (!tma_rows(q->x, q->inner * elem)) f.x = ar.take<uint8_t>(q->rows * pitch);
-  if (!tma_rows(q->weight, q->inner * elem)) f.w = ar.take<uint8_t>(q->outer * pitch);
+  if (!tma_rows(q->x, x_pitch(q) * elem)) f.x = ar.take<uint8_t>(q->rows * pitch);
+  if (!tma_rows(q->weight, w_pitch(q) * elem)) f.w = ar.take<uint8_t>(q->outer * pitch);
   const ProductPlan p = product_plan(q->rows, q->outer, (int)cdiv(q->inner * elem, 128));
   if (p.partial_floats) f.partial = ar.take<float>(p.partial_floats);
   return f;
@@ -436,8 +452,8 @@ BackwardWork backward_work(Arena &ar, const lnet_b200_linear_request *q, const v
   const size_t pitch_out = align_up((size_t)q->outer * 2, 16);
   if ((want_dx || want_dw) && (pre || !tma_rows(dy, q->outer * 2)))
     b.da = ar.take<__nv_bfloat16>(q->rows * pitch_out / 2);
-  if (want_dw && !tma_rows(q->x, q->inner * 2)) b.x = ar.take<uint8_t>(q->rows * pitch_in);
-  if (want_dx && !tma_rows(q->weight, q->inner * 2)) b.w = ar.take<uint8_t>(q->outer * pitch_in);
+  if (want_dw && !tma_rows(q->x, x_pitch(q) * 2)) b.x = ar.take<uint8_t>(q->rows * pitch_in);
+  if (want_dx && !tma_rows(q->weight, w_pitch(q) * 2)) b.w = ar.take<uint8_t>(q->outer * pitch_in);
   int64_t partial = 0;
   if (want_dx)
     partial = product_plan(q->rows, q->inner, (int)cdiv(q->outer, 64)).partial_floats;
@@ -505,20 +521,42 @@ extern "C" int lnet_b200_linear_forward(const lnet_b200_linear_request *req, voi
   e.col_scale = fp8 ? req->weight_scale : nullptr;
   e.act = req->activation;
   if (req->rows <= kVectorRows) {
-    const VectorArgs v{req->x, req->weight, e, req->outer, req->inner, (int)req->rows};
-    const bool vec = tma_rows(req->x, req->inner * elem) && tma_rows(req->weight, req->inner * elem);
+    const VectorArgs v{req->x,       req->weight,  e,           req->outer, req->inner,
+                       x_pitch(req), w_pitch(req), (int)req->rows};
+    const bool vec = req->inner * elem % 16 == 0 && tma_rows(req->x, x_pitch(req) * elem) &&
+                     tma_rows(req->weight, w_pitch(req) * elem);
     if (fp8)
       vec ? launch_vector<true, true>(v, stream) : launch_vector<true, false>(v, stream);
     else
       vec ? launch_vector<false, true>(v, stream) : launch_vector<false, false>(v, stream);
     return after_launch("linear_vector_kernel");
   }
-  TileOperand a{req->x, req->rows, req->inner, req->inner, false};
-  TileOperand b{req->weight, req->outer, req->inner, req->inner, false};
+  TileOperand a{req->x, req->rows, req->inner, x_pitch(req), false};
+  TileOperand b{req->weight, req->outer, req->inner, w_pitch(req), false};
   LNET_TRY(packed(a, req->rows, req->inner, elem, f.x, stream));
   LNET_TRY(packed(b, req->outer, req->inner, elem, f.w, stream));
   return fp8 ? product<false, false, true>(a, b, e, f.partial, stream)
              : product<false, false, false>(a, b, e, f.partial, stream);
+}
+
+extern "C" int lnet_b200_linear_pack(const void *src, int32_t dtype, int64_t rows, int64_t cols,
+                                     int64_t src_pitch, void *dst, int64_t dst_pitch,
+                                     lnet_stream_t stream) {
+  const char *what = "linear_pack";
+  const int64_t most = (int64_t)1 << 36;
+  if (rows < 0 || cols < 1 || src_pitch < cols || dst_pitch < cols || src_pitch > most ||
+      dst_pitch > most || rows > (int64_t)1 << 30 ||
+      (rows > 0 && std::max(src_pitch, dst_pitch) > ((int64_t)1 << 46) / rows))
+    return fail(LNET_ERR_INVALID_ARGUMENT, "%s: rows %lld, cols %lld, pitches %lld and %lld", what,
+                (long long)rows, (long long)cols, (long long)src_pitch, (long long)dst_pitch);
+  if (dtype != LNET_BF16 && dtype != LNET_E4M3)
+    return fail(LNET_ERR_UNSUPPORTED, "%s: operands must be bf16 or e4m3", what);
+  reset_launches();
+  if (rows == 0) return LNET_OK;
+  if (!src || !dst) return fail(LNET_ERR_INVALID_ARGUMENT, "%s: a NULL pointer", what);
+  begin_entry(stream);
+  return launch_pack(src, rows, cols, src_pitch, dtype == LNET_BF16 ? 2 : 1, dst, dst_pitch,
+                     stream);
 }
 
 static int check_backward(const char *what, const lnet_b200_linear_request *req,
@@ -590,7 +628,7 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
   const void *da = w.da ? (const void *)w.da : dy;
   if (dx) {
     TileOperand a{da, M, N, pitch, false};
-    TileOperand b{req->weight, K, N, K, true};
+    TileOperand b{req->weight, K, N, w_pitch(req), true};
     LNET_TRY(packed(b, N, K, 2, w.w, stream));
     TileEpilogue e{};
     e.out = reinterpret_cast<__nv_bfloat16 *>(dx);
@@ -598,7 +636,7 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
   }
   if (dweight) {
     TileOperand a{da, N, M, pitch, true};
-    TileOperand b{req->x, K, M, K, true};
+    TileOperand b{req->x, K, M, x_pitch(req), true};
     LNET_TRY(packed(b, M, K, 2, w.x, stream));
     TileEpilogue e{};
     e.out = reinterpret_cast<__nv_bfloat16 *>(dweight);

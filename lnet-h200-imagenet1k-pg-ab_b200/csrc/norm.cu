@@ -280,25 +280,50 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
   }
 }
 
-// A matrix's rows in e4m3 with the scale max|row| / 448: what a serving program does once to
-// its weights.  A block a row, the second sweep from L2.
-template <typename T>
+// A matrix's rows in e4m3 with the scale max|row| / 448: a serving program's weights, once, and the
+// activations between two 8-bit products.  A block a row, the second sweep from L1 or L2.
+template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t *q,
                      float *scales) {
   __shared__ float scratch[33];
+  const int64_t nvec = dim / VEC;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const T *p = x + row * dim;
     float m = 0.f, k;
-    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x)
-      m = MaxMagnitudeOp::of(m, fabsf(load_f(x, row * dim + c)));
+    for (int64_t c = threadIdx.x; c < nvec; c += blockDim.x) {
+      RowChunk<T, VEC> u;
+      Lanes<VEC> l[lanes_of<VEC>()];
+      u.load(p + c * VEC);
+      get_lanes(u, l);
+      m = chunk_magnitude<VEC>(m, l);
+    }
     m = group_reduce<0, MaxMagnitudeOp>(m, scratch);
     const float scale = e4m3_scale(m, 1.f, k);
     if (threadIdx.x == 0) scales[row] = scale;
-    for (int64_t c = threadIdx.x; c < dim; c += blockDim.x) {
-      const Single v{load_f(x, row * dim + c)};
-      store_e4m3<1>(q + row * dim + c, &v, k);
+    for (int64_t c = threadIdx.x; c < nvec; c += blockDim.x) {
+      RowChunk<T, VEC> u;
+      Lanes<VEC> l[lanes_of<VEC>()];
+      u.load(p + c * VEC);
+      get_lanes(u, l);
+      store_e4m3<VEC>(q + row * dim + c * VEC, l, k);
     }
   }
+}
+
+template <typename T>
+int quantize_typed(const T *x, int64_t rows, int64_t dim, uint8_t *q, float *scales,
+                   cudaStream_t s) {
+  constexpr int VEC = vec_of<T>();
+  const bool vec = dim % VEC == 0 && aligned16(x) && aligned16(q);
+  const int64_t nvec = vec ? dim / VEC : dim;
+  const int threads = (int)std::min<int64_t>(256, (nvec + 31) / 32 * 32);
+  const int blocks = (int)std::min<int64_t>(rows, (int64_t)sm_count() * (2048 / threads));
+  if (vec)
+    quantize_rows_kernel<T, VEC><<<blocks, threads, 0, s>>>(x, rows, dim, q, scales);
+  else
+    quantize_rows_kernel<T, 1><<<blocks, threads, 0, s>>>(x, rows, dim, q, scales);
+  return after_launch("quantize_rows_kernel");
 }
 
 struct NormGradArgs {
@@ -649,14 +674,10 @@ extern "C" int lnet_b200_quantize_rows_fp8(const void *x, int32_t dtype, int64_t
   if (!x || !values || !scales)
     return fail(LNET_ERR_INVALID_ARGUMENT, "%s: x, values, scales must not be NULL", what);
   begin_entry(stream);
-  const int blocks = (int)std::min<int64_t>(rows, (int64_t)sm_count() * 8);
-  if (dtype == LNET_BF16)
-    quantize_rows_kernel<<<blocks, 256, 0, stream>>>(reinterpret_cast<const __nv_bfloat16 *>(x),
-                                                     rows, dim, values, scales);
-  else
-    quantize_rows_kernel<<<blocks, 256, 0, stream>>>(reinterpret_cast<const float *>(x), rows, dim,
-                                                     values, scales);
-  return after_launch("quantize_rows_kernel");
+  return dtype == LNET_BF16
+             ? quantize_typed(reinterpret_cast<const __nv_bfloat16 *>(x), rows, dim, values, scales,
+                              stream)
+             : quantize_typed(reinterpret_cast<const float *>(x), rows, dim, values, scales, stream);
 }
 
 extern "C" int lnet_b200_residual_rms_norm_workspace_size(int32_t dtype, int64_t rows, int64_t dim,

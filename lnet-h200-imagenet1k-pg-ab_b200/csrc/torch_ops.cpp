@@ -36,6 +36,7 @@ using OptTensor = std::optional<Tensor>;
   X(residual_rms_norm_workspace_size)                                                            \
   X(residual_rms_norm_backward)                                                                  \
   X(quantize_rows_fp8)                                                                           \
+  X(linear_pack)                                                                                 \
   X(linear_workspace_size)                                                                       \
   X(linear_forward)                                                                              \
   X(linear_backward_workspace_size)                                                              \
@@ -162,38 +163,72 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
 };
 
 // ---------------------------------------------------------------- linear
+// A product's operand as [rows, K] with unit column stride.  Where the product runs on tiles (more
+// rows than kFewRows) its rows start on 16-byte boundaries: as they lie, or in a padded copy, made
+// once for the forward and the backward pass.
+constexpr int64_t kFewRows = 8;
+Tensor operand(const Tensor &t, bool tiles) {
+  const int64_t k = t.size(-1), elem = (int64_t)t.element_size();
+  Tensor m = t;
+  if (t.dim() != 2 || t.stride(1) != 1 || (t.size(0) > 1 && t.stride(0) < k))
+    m = t.contiguous().view({rows_of(t), k});
+  const int64_t pitch = m.size(0) > 1 ? m.stride(0) : k;
+  const bool aligned = (uintptr_t)ptr(m) % 16 == 0 && (m.size(0) <= 1 || pitch * elem % 16 == 0);
+  if (!tiles || aligned || m.size(0) == 0) return m;
+  const int64_t wide = (k * elem + 15) / 16 * 16 / elem;
+  Tensor copy = at::empty({m.size(0), wide}, m.options());
+  check(lib.linear_pack(ptr(m), dtype_of(m), m.size(0), k, pitch, ptr(copy), wide, stream_of(m)),
+        "linear_pack");
+  return copy.narrow(1, 0, k);
+}
 lnet_b200_linear_request linear_request(const Tensor &x, const Tensor &w, const Tensor &b,
                                         const Tensor &r, int64_t act, const Tensor &xs,
                                         const Tensor &ws) {
   lnet_b200_linear_request q{};
-  q.rows = rows_of(x), q.inner = x.size(-1), q.outer = w.size(0);
+  q.rows = x.size(0), q.inner = x.size(1), q.outer = w.size(0);
   q.dtype = dtype_of(x), q.activation = (int32_t)act;
   q.x = ptr(x), q.weight = ptr(w), q.bias = ptr(b), q.residual = ptr(r);
   q.x_scale = (const float *)ptr(xs), q.weight_scale = (const float *)ptr(ws);
+  // one row has no pitch; its bytes, up to the next 16, may not be there: no tile reads them
+  q.x_pitch = q.rows > 1 ? x.stride(0) : 0, q.weight_pitch = q.outer > 1 ? w.stride(0) : 0;
   return q;
 }
-std::pair<Tensor, Tensor> linear_forward(const Tensor &x, const lnet_b200_linear_request &q,
-                                         bool keep) {
+struct LinearOut {
+  Tensor y, pre, x, w;  // x, w: the operands as they were used
+};
+LinearOut linear_forward(const Tensor &x, const Tensor &w, const Tensor &b, const Tensor &r,
+                         int64_t act, const Tensor &xs, const Tensor &ws, bool keep) {
+  const bool tiles = rows_of(x) > kFewRows;
+  LinearOut o;
+  o.x = operand(x, tiles), o.w = operand(w, tiles);
+  const Tensor bc = dense(b), rc = dense(r), xsc = dense(xs), wsc = dense(ws);
+  const auto q = linear_request(o.x, o.w, bc, rc, act, xsc, wsc);
   size_t bytes = 0;
   check(lib.linear_workspace_size(&q, &bytes), "linear_workspace_size");
-  auto shape = x.sizes().vec();
-  shape.back() = q.outer;
-  Tensor y = at::empty(shape, x.options().dtype(at::kBFloat16)), pre;
-  if (keep) pre = at::empty_like(y);
-  Tensor ws = workspace(bytes, x);
-  check(lib.linear_forward(&q, ptr(ws), bytes, ptr(y), ptr(pre), stream_of(x)), "linear_forward");
-  return {y, pre};
+  if (x.dim() == 2) {
+    o.y = at::empty({q.rows, q.outer}, x.options().dtype(at::kBFloat16));
+  } else {
+    auto shape = x.sizes().vec();
+    shape.back() = q.outer;
+    o.y = at::empty(shape, x.options().dtype(at::kBFloat16));
+  }
+  if (keep) o.pre = at::empty_like(o.y);
+  Tensor space = workspace(bytes, x);
+  check(lib.linear_forward(&q, ptr(space), bytes, ptr(o.y), ptr(o.pre), stream_of(x)),
+        "linear_forward");
+  return o;
 }
+// x and w as linear_forward left them; dx in `x_sizes`.
 variable_list linear_backward(const Tensor &x, const Tensor &w, int64_t act, const Tensor &pre,
-                              const Tensor &dy, int64_t need) {
+                              const Tensor &dy, int64_t need, at::IntArrayRef x_sizes) {
   const auto q = linear_request(x, w, Tensor(), Tensor(), act, Tensor(), Tensor());
   size_t bytes = 0;
   check(lib.linear_backward_workspace_size(&q, ptr(pre), ptr(dy), need & 1, need & 2, need & 4,
                                            &bytes),
         "linear_backward_workspace_size");
   Tensor dx, dw, db, ws = workspace(bytes, x);
-  if (need & 1) dx = at::empty_like(x);
-  if (need & 2) dw = at::empty_like(w);
+  if (need & 1) dx = at::empty(x_sizes, x.options());
+  if (need & 2) dw = at::empty({q.outer, q.inner}, x.options());
   if (need & 4) db = at::empty({q.outer}, x.options());
   check(lib.linear_backward(&q, ptr(pre), ptr(dy), ptr(ws), bytes, ptr(dx), ptr(dw), ptr(db),
                             stream_of(x)),
@@ -207,13 +242,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const int64_t need = (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) |
                          (b.has_value() && b->requires_grad() ? 4 : 0) |
                          (r.has_value() && r->requires_grad() ? 8 : 0);
-    const Tensor xc = dense(x), wc = dense(w), bc = dense(b), rc = dense(r);
-    auto [y, pre] = linear_forward(xc, linear_request(xc, wc, bc, rc, act, Tensor(), Tensor()),
-                                   act != 0 && (need & 7));
+    LinearOut o = linear_forward(x, w, b.value_or(Tensor()), r.value_or(Tensor()), act, Tensor(),
+                                 Tensor(), act != 0 && (need & 7));
     ctx->saved_data["need"] = need;
     ctx->saved_data["act"] = act;
-    ctx->save_for_backward({xc, wc, pre});
-    return y;
+    if (x.dim() != 2) ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->save_for_backward({o.x, o.w, o.pre});
+    return o.y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const int64_t need = ctx->saved_data["need"].toInt(), act = ctx->saved_data["act"].toInt();
@@ -221,7 +256,10 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     if (need & 7) {
       const auto saved = ctx->get_saved_variables();
       c10::cuda::CUDAGuard guard(saved[0].device());
-      g = linear_backward(saved[0], saved[1], act, saved[2], dense(grads[0]), need);
+      const auto sizes = ctx->saved_data.find("sizes");
+      const auto shape = sizes == ctx->saved_data.end() ? saved[0].sizes().vec()
+                                                        : sizes->second.toIntVector();
+      g = linear_backward(saved[0], saved[1], act, saved[2], dense(grads[0]), need, shape);
     }
     return once({g[0], g[1], g[2], need & 8 ? grads[0] : Tensor(), Tensor()}, "linear_act");
   }
@@ -484,8 +522,7 @@ PyObject *py_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
     if (tracked({&x, &w, &b, &r})) {
       y = LinearFunction::apply(x, w, opt(b), opt(r), act);
     } else {
-      const Tensor xc = dense(x), wc = dense(w), bc = dense(b), rc = dense(r);
-      y = linear_forward(xc, linear_request(xc, wc, bc, rc, act, Tensor(), Tensor()), false).first;
+      y = linear_forward(x, w, b, r, act, Tensor(), Tensor(), false).y;
     }
   }
   return wrap(y);
@@ -503,7 +540,8 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   {
     NoGil gil;
     c10::cuda::CUDAGuard guard(x.device());
-    g = linear_backward(dense(x), dense(w), act, dense(pre), dense(dy), 7);
+    g = linear_backward(operand(x, true), operand(w, true), act, dense(pre), dense(dy), 7,
+                        x.sizes());
   }
   return wrap_tuple({g[0], g[1], g[2]});
   END_HANDLE_TH_ERRORS
@@ -516,14 +554,13 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]);
   const Tensor b = optional_arg(args[2]), r = optional_arg(args[3]);
   const int64_t act = int_arg(args[4]);
-  std::pair<Tensor, Tensor> out;
+  LinearOut out;
   {
     NoGil gil;
     c10::cuda::CUDAGuard guard(x.device());
-    const Tensor xc = dense(x), wc = dense(w), bc = dense(b), rc = dense(r);
-    out = linear_forward(xc, linear_request(xc, wc, bc, rc, act, Tensor(), Tensor()), act != 0);
+    out = linear_forward(x, w, b, r, act, Tensor(), Tensor(), act != 0);
   }
-  return wrap_tuple({out.first, out.second});
+  return wrap_tuple({out.y, out.pre});
   END_HANDLE_TH_ERRORS
 }
 
@@ -539,9 +576,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *args, Py_ssize_t n) {
     NoGil gil;
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(x.device());
-    const Tensor xc = dense(x), wc = dense(w), bc = dense(b), rc = dense(r);
-    const Tensor xsc = dense(xs), wsc = dense(ws);
-    y = linear_forward(xc, linear_request(xc, wc, bc, rc, act, xsc, wsc), false).first;
+    y = linear_forward(x, w, b, r, act, xs, ws, false).y;
   }
   return wrap(y);
   END_HANDLE_TH_ERRORS

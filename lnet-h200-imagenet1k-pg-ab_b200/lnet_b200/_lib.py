@@ -93,6 +93,8 @@ class LinearRequest(ctypes.Structure):
         ("residual", _c_p),
         ("x_scale", _c_p),
         ("weight_scale", _c_p),
+        ("x_pitch", _i64),
+        ("weight_pitch", _i64),
     ]
 
 
@@ -250,6 +252,9 @@ SIGNATURES = {
     ),
     "lnet_b200_quantize_rows_fp8": (
         ctypes.c_int, [_c_p, _i32, _i64, _i64, _c_p, _c_p, _c_p]
+    ),
+    "lnet_b200_linear_pack": (
+        ctypes.c_int, [_c_p, _i32, _i64, _i64, _i64, _c_p, _i64, _c_p]
     ),
     "lnet_b200_linear_workspace_size": (
         ctypes.c_int, [ctypes.POINTER(LinearRequest), ctypes.POINTER(ctypes.c_size_t)]

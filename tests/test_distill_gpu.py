@@ -265,3 +265,49 @@ def test_no_rows_no_entries_and_determinism(cuda_device):
         loss = distillation_loss(z, index, teacher, labels=labels, temperature=2.0, alpha=0.5)
         runs.append((loss.detach(), torch.autograd.grad(loss, z)[0]))
     assert all(torch.equal(r[0], runs[0][0]) and torch.equal(r[1], runs[0][1]) for r in runs)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 logits: the last rows' losses and gradients against the same rows alone."""
+    rows, classes = 32800, 65504
+    z = torch.zeros(rows, classes, dtype=torch.bfloat16, device=cuda_device)
+    g = torch.Generator().manual_seed(1)
+    z[-8:] = (torch.randn(8, classes, generator=g) * 2).bfloat16().to(cuda_device)
+    index = torch.randint(0, classes, (rows, 4), generator=g).to(cuda_device)
+    teacher = torch.randn(rows, 4, generator=g).to(cuda_device)
+    z.requires_grad_()
+    loss = distillation_loss(z, index, teacher, reduction="sum")
+    dz, = torch.autograd.grad(loss, z)
+    tail = z.detach()[-8:].clone().requires_grad_()
+    loss2 = distillation_loss(tail, index[-8:], teacher[-8:], reduction="sum")
+    dz2, = torch.autograd.grad(loss2, tail)
+    assert z.numel() > 1 << 31 and torch.equal(dz[-8:], dz2)
+    each = distillation_loss(z.detach(), index, teacher, reduction="none")
+    assert torch.equal(each[-8:], distillation_loss(tail.detach(), index[-8:], teacher[-8:],
+                                                    reduction="none")) or \
+        float((each[-8:].sum() - loss2.detach()).abs()) <= 1e-4 * float(loss2.detach())
+    assert float((each.double().sum() - loss.detach().double()).abs()) <= 1e-5 * float(loss.detach())
+
+
+def test_capture(cuda_device):
+    """Loss and gradient in a CUDA graph, replayed on new logits."""
+    z, index, teacher, labels = make(40, 1000, 10, torch.float32, 3, cuda_device)
+    z.requires_grad_()
+
+    def step():
+        loss = distillation_loss(z, index, teacher, labels=labels, temperature=2.0, alpha=0.5)
+        return loss.detach(), torch.autograd.grad(loss, z)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        z.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, step()))

@@ -177,6 +177,28 @@ def test_strides_alignment_and_shapes(cuda_device):
     assert torch.equal(linear_act(x, w, odd_bias, r, activation="silu"), want)
 
 
+def test_rows_further_apart_than_their_length(cuda_device):
+    """Operands with a row pitch are read as they lie, forward and backward, few rows and many."""
+    for m in (5, 60, 300):
+        x, w, b, r = inputs(m, 96, 80, cuda_device)
+        wide_x = torch.full((m, 200), math.nan, dtype=x.dtype, device=cuda_device)
+        wide_w = torch.full((80, 136), math.nan, dtype=x.dtype, device=cuda_device)
+        wide_x[:, 8:104], wide_w[:, 16:112] = x, w
+        dy = make((m, 80), 5, cuda_device)
+        grads = []
+        for xi, wi in ((x, w), (wide_x[:, 8:104], wide_w[:, 16:112])):
+            xi, wi = xi.detach().requires_grad_(), wi.detach().requires_grad_()
+            y = linear_act(xi, wi, b, r, activation="gelu")
+            grads.append((y.detach(), *torch.autograd.grad(y, [xi, wi], dy)))
+        assert all(torch.equal(p, q) for p, q in zip(*grads))
+        xq, xs = quantize_rows_fp8(x)
+        wq, ws = quantize_rows_fp8(w)
+        want = linear_act_fp8(xq, xs, wq, ws, b, r)
+        pad = torch.zeros(m, 160, dtype=torch.uint8, device=cuda_device)
+        pad[:, 16:112] = xq.view(torch.uint8)
+        assert torch.equal(linear_act_fp8(pad.view(xq.dtype)[:, 16:112], xs, wq, ws, b, r), want)
+
+
 def test_infinities_stay_in_their_rows(cuda_device):
     x, w, b, _ = inputs(200, 96, 160, cuda_device)
     x[17, 5] = math.inf
@@ -221,6 +243,42 @@ def test_determinism_and_streams(cuda_device):
         again = step()
     side.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(first, again))
+
+
+def test_capture(cuda_device):
+    """Forward and gradient in a CUDA graph, replayed on new values."""
+    x, w, b, r = (t.requires_grad_() for t in inputs(300, 96, 384, cuda_device))
+    dy = make((300, 384), 5, cuda_device)
+
+    def step():
+        y = linear_act(x, w, b, r, activation="gelu")
+        return (y.detach(), *torch.autograd.grad(y, [x, w, b], dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.copy_(make((300, 96), 11, cuda_device))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, step()))
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """An output of more than 2^31 elements: its last rows against the same rows alone."""
+    m, k, n = (1 << 21) + 300, 64, 1032
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device=cuda_device)
+    x[-200:] = make((200, k), 1, cuda_device)
+    w, b = make((n, k), 2, cuda_device), make((n,), 3, cuda_device)
+    y = linear_act(x, w, b, activation="relu")
+    assert y.numel() > 1 << 31
+    assert torch.equal(y[-200:], linear_act(x[-200:].clone(), w, b, activation="relu"))
+    assert torch.equal(y[:100], linear_act(x[:100].clone(), w, b, activation="relu"))
 
 
 def test_fp8_refuses_a_gradient(cuda_device):

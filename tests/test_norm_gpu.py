@@ -221,6 +221,46 @@ def test_another_stream(cuda_device):
     assert torch.equal(y, want)
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 elements: the last rows, forward and backward, against the same rows alone."""
+    m, d = (1 << 21) + 100, 1032
+    x = torch.ones(m, d, dtype=torch.bfloat16, device=cuda_device)
+    x[-64:] = make((64, d), torch.bfloat16, 1, cuda_device)
+    w = 1 + make((d,), torch.float32, 2, cuda_device, 0.2)
+    x.requires_grad_()
+    y, _ = residual_rms_norm(x, w)
+    dx, = torch.autograd.grad(y, [x], x.detach())
+    tail = x.detach()[-64:].clone().requires_grad_()
+    y2, _ = residual_rms_norm(tail, w)
+    dx2, = torch.autograd.grad(y2, [tail], tail.detach())
+    assert torch.equal(y.detach()[-64:], y2.detach()) and torch.equal(dx[-64:], dx2)
+
+
+def test_capture(cuda_device):
+    """Forward and gradient in a CUDA graph, replayed on new values."""
+    x = make((300, 96), torch.bfloat16, 1, cuda_device).requires_grad_()
+    w = torch.ones(96, device=cuda_device, requires_grad=True)
+    dy = make((300, 96), torch.bfloat16, 2, cuda_device)
+
+    def step():
+        y, h = residual_rms_norm(x, w, dy)
+        return (y.detach(), *torch.autograd.grad([y, h], [x, w], [dy, dy]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.copy_(make((300, 96), torch.bfloat16, 11, cuda_device))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, step()))
+
+
 def test_fp8_refuses_a_gradient(cuda_device):
     x = make((4, 96), torch.bfloat16, 1, cuda_device).requires_grad_()
     with pytest.raises(RuntimeError, match="no gradient"):
