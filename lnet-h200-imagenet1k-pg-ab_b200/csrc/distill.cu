@@ -24,6 +24,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "rows.cuh"
@@ -441,23 +442,22 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 }
 
 // Then the row.  A persistent cluster of 1 to 8 blocks takes one at a time.  A thread holds up to
-// kResident chunks of 16 bytes of it and their exponentials in registers, both relative to the
+// NV chunks of 16 bytes of it and their exponentials in registers, both relative to the
 // largest of its own elements, so that z is read once and each exponential is computed once:
 //   dz = [at e^((m_t - m) / tau)] e^((z - m_t) / tau) + [a1 e^(m_t - m)] e^(z - m_t).
-// The next row is brought to L2 meanwhile.  The warps' maxima and sums are joined over the
+// The next row's part arrives in shared memory meanwhile (bulk copies).  The warps' maxima and sums are joined over the
 // cluster: each warp stores its own into every block's shared memory (st.async, two sets in turn)
 // and every block waits for all of them on an mbarrier of its own.  A cluster barrier in its place
 // also waited for the block's gradient stores.
 // An entry is handed to the thread that holds its element (a list a thread in shared memory),
 // which writes the corrected value over its own store: no second barrier.
-// The exponentials take 64 registers a thread, 128 with the rest, so 512 threads fill an SM.  The
-// joins leave a block idle for about half of a row's time: four blocks of 128 threads on an SM and
-// clusters of 8 took 339 us for 8192 rows of 32768 bf16 classes (two temperatures), two of 256 and
-// clusters of 4 398 us, five of 128 (96 registers, some spilled) 359 us.  Blocks of 512 serve the
-// rows that 8 of 128 do not hold.  Bound by instructions and the join's latency (0.53 instructions
-// a clock and scheduler), at 0.49 of the measured HBM rate.
-constexpr int kResident = 4;
-constexpr int kSmallThreads = 128, kSmallBlocks = 4;
+// 8192 rows of 32768 bf16 classes, two temperatures: 294 us with three blocks an SM of 128 threads, 64
+// elements a thread (168 registers) and clusters of 4; 317 with four of 32 elements and clusters of
+// 8; 315 with six of 64 threads; 341 with one of 256.  What bounds it is the time that a cluster's
+// blocks wait for the slowest of them (0.4 instructions a clock and scheduler), at 0.57 of the measured
+// HBM rate; the sweep-twice kernel took 637 us.  Rows of up to 128 x 4 chunks take 4 chunks a thread
+// and one block; rows that 8 blocks of 128 x 8 do not hold take up to 512 threads of 4.
+constexpr int kSmallThreads = 128;
 constexpr int kLargeThreads = 512;
 constexpr int kResidentParts = 8;
 
@@ -709,7 +709,7 @@ distill_resident_kernel(const ResidentArgs ra) {
           else
             sm100::mbar_arrive(joined + set);
         }
-        if (!failed) failed = !sm100::mbar_wait_cluster_bounded(joined + set, phase, 1000000u);
+        if (!failed) failed = !sm100::mbar_wait_bounded(joined + set, phase, 1000000u);
       }
     }
     {
@@ -951,7 +951,8 @@ bool resident_plan(const lnet_b200_distill_request *q, const void *dz, ResidentP
   p.aligned = zp % 16 == 0 && q->classes % VEC == 0;
   // one chunk more where a row may start inside a chunk
   const int64_t chunks = cdiv(q->classes, VEC) + (p.aligned ? 0 : 1);
-  // The smallest blocks that 8 of hold the row: 64 or 128 threads, then 256 or 512.
+  // The smallest block that holds the row, 64 or 128 threads of 4 chunks; then 128 of 8, up to 8
+  // blocks of them; then 256 or 512 threads of 4.  (A warp a row was slower for 56 and 366 classes.)
   p.threads = 64, p.parts = 1, p.nv = 4;
   auto holds = [&] { return chunks <= (int64_t)p.parts * p.threads * p.nv; };
   while (p.threads < kSmallThreads && !holds()) p.threads *= 2;
@@ -979,12 +980,22 @@ int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStre
   cfg.dynamicSmemBytes = 2 * p.threads * NV * 16;
   // Clusters that run at once: fewer than SMs / parts, since a cluster stays inside one group of
   // SMs.  A waiting cluster would double the time of a persistent grid.
-  int clusters = 0;
-  if (p.parts == 1)
-    clusters = sm_count() * (MAXT == kSmallThreads ? kSmallBlocks * kSmallThreads : MAXT) / p.threads;
-  else
-    LNET_TRY(cuda_check(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg),
-                        "distill_resident_kernel occupancy"));
+  static std::atomic<int> known[kResidentParts + 1][kLargeThreads / 32 + 1];
+  std::atomic<int> &cached = known[p.parts][p.threads / 32];
+  int clusters = cached.load();
+  if (clusters == 0) {
+    if (p.parts == 1) {
+      LNET_TRY(cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(
+                              &clusters, kernel, p.threads, cfg.dynamicSmemBytes),
+                          "distill_resident_kernel occupancy"));
+      clusters *= sm_count();
+    } else {
+      LNET_TRY(cuda_check(cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg),
+                          "distill_resident_kernel occupancy"));
+    }
+    clusters = std::max(1, clusters);
+    cached.store(clusters);
+  }
   clusters = (int)std::max<int64_t>(1, std::min<int64_t>(a.d.rows, clusters));
   cfg.gridDim = dim3((unsigned)(clusters * p.parts));
   LNET_TRY(cuda_check(cudaLaunchKernelEx(&cfg, kernel, a), "distill_resident_kernel"));

@@ -31,9 +31,14 @@
 namespace lnet {
 
 constexpr int kTileM = 128;             // rows of A a CTA holds
-constexpr int kTileThreads = 320;       // loader, MMA issuer, 8 epilogue warps
+// 8 warps leave shared memory for 6 stages: 16, with 5, cost 4 % at K = 2048 and took 8 % off GELU at
+// K = 96.  Asking for the next block from TMEM before working on one changed nothing.
 constexpr int kEpiWarps = 8;
-constexpr uint32_t kTileWaitLimit = 1000000u;  // about 1 s of 1 us tries
+constexpr int kTileThreads = 64 + 32 * kEpiWarps;  // loader, MMA issuer, epilogue warps
+// A try of 1 us suspends the waiting threads; shorter ones changed no time, and their polling takes
+// power from the tensor cores.
+constexpr uint32_t kTileWaitHint = 1000u;
+constexpr uint32_t kTileWaitLimit = 1000000u;  // tries: about a second
 constexpr int kTileSmemLimit = 227 * 1024;
 
 enum LinearActivation { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
@@ -134,10 +139,27 @@ struct TileEpilogue {
   int act;
 };
 
+// Division of n < 2^31 by a number known before the launch (Granlund and Montgomery, Division by
+// Invariant Integers using Multiplication): the roles find their next tile with it, and the loader,
+// one thread, was held up by the dozens of dependent instructions of plain divisions.
+struct FastDiv {
+  uint32_t d, m;
+  int s;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t div) : d(div), s(0) {
+    while ((1ull << s) < div) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - div)) / div + 1);
+  }
+  __device__ __forceinline__ int quotient(int n) const {
+    return (int)((__umulhi(m, (uint32_t)n) + (uint32_t)n) >> s);
+  }
+};
+
 struct TileArgs {
   CUtensorMap a, b;
   TileEpilogue e;
   int64_t M, N;
+  FastDiv by_band, by_last, by_splits;  // 8 n_tiles, rows of the last band, splits
   // Tiles 0 to full - 1 take all of k; the others are split into `splits` ranges of k each, whose
   // fp32 sums go to `partial` [tile - full][split][CTA][BN / 4][128 rows][4].
   int m_tiles, n_tiles, full, splits, kblocks;
@@ -151,7 +173,7 @@ struct TileShape {
   static constexpr int A_BYTES = kTileM * 128, B_BYTES = NB * 128;
   static constexpr int STAGE = A_BYTES + B_BYTES;
   // a warp's 32 x 32 bf16 block on its way to memory, and its columns' bias and scale (fp32)
-  static constexpr int WARP_COLS = BN / 2 >= 32 ? BN / 2 : 32;
+  static constexpr int WARP_COLS = BN / (kEpiWarps / 4) >= 32 ? BN / (kEpiWarps / 4) : 32;
   static constexpr int WARP_BYTES = 2048 + 2 * WARP_COLS * 4;
   static constexpr int OTHER = 1024 /* alignment */ + 512 /* barriers */ + kEpiWarps * WARP_BYTES;
   static constexpr int STAGES =
@@ -164,12 +186,28 @@ struct TileShape {
 // A warp holds a 32 x 32 block of a, a lane a row.  Rows of a block lie N elements apart, so a lane
 // that moved its own row would touch 32 lines an instruction; the block goes through shared memory
 // (64-byte rows, 16-byte units exchanged so that neither side has bank conflicts) and moves as 4
-// lanes a row.
+// lanes a row, or, where rows are not 16-byte aligned, as a row an instruction.
 __device__ __forceinline__ uint4 *block_unit(uint8_t *block, int row, int unit) {
   return reinterpret_cast<uint4 *>(block + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
 }
+__device__ __forceinline__ __nv_bfloat16 *block_element(uint8_t *block, int row, int col) {
+  return reinterpret_cast<__nv_bfloat16 *>(block_unit(block, row, col >> 3)) + (col & 7);
+}
+// Where a lane's units of a warp's rows lie: row (lane / 4) + 8 i, unit lane % 4 of 32 columns.
+struct BlockRows {
+  int64_t at;   // element offset of the lane's first unit in column 0
+  int64_t row0, M, N;
+  uint32_t ok;  // bit i: row i of the lane is inside
+};
+__device__ __forceinline__ BlockRows block_rows(int64_t row0, int64_t M, int64_t N) {
+  const int lane = threadIdx.x & 31;
+  BlockRows b{(row0 + (lane >> 2)) * N + (lane & 3) * 8, row0, M, N, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) b.ok |= (row0 + (lane >> 2) + 8 * i < M ? 1u : 0u) << i;
+  return b;
+}
 __device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv_bfloat16 *dst,
-                                            int64_t row0, int64_t col, int64_t M, int64_t N) {
+                                            const BlockRows &b, int64_t col, bool vec) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -178,31 +216,58 @@ __device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv
     *block_unit(block, lane, u) = c.raw;
   }
   __syncwarp();
-  const int64_t at = col + (lane & 3) * 8;
+  if (vec) {
+    __nv_bfloat16 *p = dst + b.at + col;
+    const bool in = col + (lane & 3) * 8 < b.N;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 8 + (lane >> 2);
-    if (row0 + r < M && at < N)
-      *reinterpret_cast<uint4 *>(dst + (row0 + r) * N + at) = *block_unit(block, r, lane & 3);
+    for (int i = 0; i < 4; ++i) {
+      if (in && (b.ok >> i & 1))
+        *reinterpret_cast<uint4 *>(p) = *block_unit(block, i * 8 + (lane >> 2), lane & 3);
+      p += 8 * b.N;
+    }
+  } else if (col + lane < b.N) {
+    __nv_bfloat16 *p = dst + b.row0 * b.N + col + lane;
+    const int rows = (int)min((int64_t)32, b.M - b.row0);
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r, p += b.N) *p = *block_element(block, r, lane);
   }
   __syncwarp();
 }
 // 16-byte units of a block of `src`: issued early, used by block_add.
-__device__ __forceinline__ void block_fetch(const __nv_bfloat16 *src, uint4 *u, int64_t row0,
-                                            int64_t col, int64_t M, int64_t N) {
-  const int lane = threadIdx.x & 31;
-  const int64_t at = col + (lane & 3) * 8;
+__device__ __forceinline__ void block_fetch(const __nv_bfloat16 *src, uint4 *u, const BlockRows &b,
+                                            int64_t col) {
+  const __nv_bfloat16 *p = src + b.at + col;
+  const bool in = col + (threadIdx.x & 3) * 8 < b.N;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int64_t r = row0 + i * 8 + (lane >> 2);
     u[i] = make_uint4(0, 0, 0, 0);
-    if (r < M && at < N) u[i] = __ldg(reinterpret_cast<const uint4 *>(src + r * N + at));
+    if (in && (b.ok >> i & 1)) u[i] = __ldg(reinterpret_cast<const uint4 *>(p));
+    p += 8 * b.N;
   }
 }
-__device__ __forceinline__ void block_add(uint8_t *block, const uint4 *u, float *v) {
+// v += the block of `src`, whose units are in `u` where `vec`.
+__device__ __forceinline__ void block_add(uint8_t *block, const __nv_bfloat16 *src, const uint4 *u,
+                                          float *v, const BlockRows &b, int64_t col, bool vec) {
   const int lane = threadIdx.x & 31;
+  if (vec) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) *block_unit(block, i * 8 + (lane >> 2), lane & 3) = u[i];
+    for (int i = 0; i < 4; ++i) *block_unit(block, i * 8 + (lane >> 2), lane & 3) = u[i];
+  } else if (col + lane < b.N) {
+    const __nv_bfloat16 *p = src + b.row0 * b.N + col + lane;
+    const int rows = (int)min((int64_t)32, b.M - b.row0);
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 rows on their way at once
+      uint16_t q[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        q[r] = r0 + r < rows
+                   ? __ldg(reinterpret_cast<const uint16_t *>(p + (int64_t)(r0 + r) * b.N))
+                   : (uint16_t)0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        *reinterpret_cast<uint16_t *>(block_element(block, r0 + r, lane)) = q[r];
+    }
+  }
   __syncwarp();
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -211,51 +276,40 @@ __device__ __forceinline__ void block_add(uint8_t *block, const uint4 *u, float 
     float w[8];
     c.get(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[8 * k + i] += w[i];
+    for (int i = 0; i < 8; i += 2)
+      unpair(pair(v[8 * k + i], v[8 * k + i + 1]) + pair(w[i], w[i + 1]), v[8 * k + i],
+             v[8 * k + i + 1]);
   }
   __syncwarp();
 }
 
 // The block's 32 columns of bias and scale come from shared memory (`bias`, `scale`; scale only
 // with row scales); `res` holds the residual's units.  Every lane of the warp takes part.
-__device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, int64_t M, int64_t N, bool vec,
-                                              float *v, int64_t row0, int64_t col, float row_scale,
+__device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, const BlockRows &b, bool vec,
+                                              float *v, int64_t col, float row_scale,
                                               const float *bias, const float *scale,
                                               uint8_t *block, const uint4 *res) {
-  const int lane = threadIdx.x & 31;
   if (e.col_scale) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
       const float4 s = *reinterpret_cast<const float4 *>(scale + j);
-      v[j] = v[j] * row_scale * s.x, v[j + 1] = v[j + 1] * row_scale * s.y;
-      v[j + 2] = v[j + 2] * row_scale * s.z, v[j + 3] = v[j + 3] * row_scale * s.w;
+      const Pair rs = pair(row_scale, row_scale);
+      unpair(pair(v[j], v[j + 1]) * rs * pair(s.x, s.y), v[j], v[j + 1]);
+      unpair(pair(v[j + 2], v[j + 3]) * rs * pair(s.z, s.w), v[j + 2], v[j + 3]);
     }
   }
   if (e.bias) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4) {
-      const float4 b = *reinterpret_cast<const float4 *>(bias + j);
-      v[j] += b.x, v[j + 1] += b.y, v[j + 2] += b.z, v[j + 3] += b.w;
+      const float4 q = *reinterpret_cast<const float4 *>(bias + j);
+      unpair(pair(v[j], v[j + 1]) + pair(q.x, q.y), v[j], v[j + 1]);
+      unpair(pair(v[j + 2], v[j + 3]) + pair(q.z, q.w), v[j + 2], v[j + 3]);
     }
   }
-  if (vec) {
-    if (e.pre) block_store(block, v, e.pre, row0, col, M, N);
-    act_values<32>(v, e.act);
-    if (e.residual) block_add(block, res, v);
-    block_store(block, v, e.out, row0, col, M, N);
-    return;
-  }
-  const int64_t row = row0 + lane, off = row * N + col;
-  if (row >= M) return;
-  if (e.pre) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < N) store_f(e.pre, off + j, v[j]);
-  }
+  if (e.pre) block_store(block, v, e.pre, b, col, vec);
   act_values<32>(v, e.act);
-#pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (col + j < N) store_f(e.out, off + j, v[j] + (e.residual ? load_f(e.residual, off + j) : 0.f));
+  if (e.residual) block_add(block, e.residual, res, v, b, col, vec);
+  block_store(block, v, e.out, b, col, vec);
 }
 
 // Bias and scale of `n` columns from `col` on into a warp's shared memory (0 past N).
@@ -273,20 +327,20 @@ struct TileUnit {
 };
 __device__ __forceinline__ TileUnit unit_at(const TileArgs &p, int t) {
   if (t < p.full) return TileUnit{t, -1, 0, p.kblocks};
-  const int u = t - p.full, tile = u / p.splits, split = u - tile * p.splits;
+  const int u = t - p.full, tile = p.by_splits.quotient(u), split = u - tile * p.splits;
   return TileUnit{p.full + tile, split, (int)((int64_t)p.kblocks * split / p.splits),
                   (int)((int64_t)p.kblocks * (split + 1) / p.splits)};
 }
 
 // Tile order: bands of 8 row tiles, down the rows inside a column, so that a
 // wave of CTAs shares few operand tiles in L2.
+constexpr int kBand = 8;
 __device__ __forceinline__ void tile_at(const TileArgs &p, int t, int &m, int &n) {
-  constexpr int kBand = 8;
-  const int band = t / (kBand * p.n_tiles);
-  const int height = min(kBand, p.m_tiles - band * kBand);
+  const int band = p.by_band.quotient(t);
   t -= band * kBand * p.n_tiles;
-  n = t / height;
-  m = band * kBand + t % height;
+  const bool last = p.m_tiles - band * kBand < kBand;
+  n = last ? p.by_last.quotient(t) : t / kBand;
+  m = band * kBand + t - n * (last ? (int)p.by_last.d : kBand);
 }
 
 template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
@@ -339,9 +393,9 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
   const int units = p.full + (p.m_tiles * p.n_tiles - p.full) * p.splits;
   const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    bool ok = sm100::mbar_try_wait_cluster(bar, parity, 1000u);
+    bool ok = sm100::mbar_try_wait(bar, parity, kTileWaitHint);
     for (uint32_t i = 0; i < kTileWaitLimit && !ok && !*failed; ++i)
-      ok = sm100::mbar_try_wait_cluster(bar, parity, 1000u);
+      ok = sm100::mbar_try_wait(bar, parity, kTileWaitHint);
     if (!ok) *failed = 1;
     return ok;
   };
@@ -350,6 +404,8 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
+    // the barriers of the pair's first CTA
+    const uint32_t full0 = CTAS == 2 ? sm100::map_to_rank(full, 0) : sm100::smem_u32(full);
     for (int t = first; t < units && ok; t += step) {
       const TileUnit w = unit_at(p, t);
       int m, n;
@@ -358,8 +414,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
       for (int k = w.k0; k < w.k1; ++k) {
         if (issued >= STAGES && !(ok = wait(empty + stage, phase ^ 1))) break;
         if (leader) sm100::mbar_arrive_expect_tx(full + stage, CTAS * S::STAGE);
-        const uint32_t bar = CTAS == 2 ? sm100::map_to_rank(full + stage, 0)
-                                       : sm100::smem_u32(full + stage);
+        const uint32_t bar = full0 + stage * 8;
         const uint32_t da = sm100::smem_u32(smem + stage * S::STAGE), db = da + S::A_BYTES;
         if (A_MN) {
 #pragma unroll
@@ -386,7 +441,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
       uint64_t *e = empty + back % STAGES, *f = full + back % STAGES;
       const uint32_t par = (uint32_t)(back / STAGES) & 1;
       if (!(ok && wait(e, par)) && leader)
-        sm100::mbar_wait_bounded(f, par, kTileWaitLimit / 10);
+        sm100::mbar_wait_bounded(f, par, 100000u);
     }
   } else if (warp == 1 && lane == 0 && leader) {  // ------------------------ MMA issuer
     constexpr uint32_t idesc =
@@ -419,12 +474,12 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
     }
     if (!ok) {  // the MMAs in flight end before TMEM is freed
       sm100::mma_commit_group<CTAS>(drain);
-      sm100::mbar_wait_bounded(drain, 0, kTileWaitLimit / 10);
+      sm100::mbar_wait_bounded(drain, 0, 100000u);
     }
   } else if (warp >= 2) {  // ----------------------------------------------- epilogue
-    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    const int ew = warp - 2, quad = warp & 3, group = ew >> 2;
     constexpr int COLS = S::WARP_COLS;
-    const bool mine = half * COLS < BN;
+    const bool mine = group * COLS < BN;
     uint8_t *block = warp_smem + ew * S::WARP_BYTES;
     float *bias = reinterpret_cast<float *>(block + 2048), *scale = bias + COLS;
     int acc = 0;
@@ -435,8 +490,9 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
       int m, n;
       tile_at(p, w.tile, m, n);
       const int64_t row0 = (int64_t)(m * CTAS + (int)rank) * kTileM + quad * 32;
-      const int64_t col0 = (int64_t)n * BN + half * COLS;
+      const int64_t col0 = (int64_t)n * BN + group * COLS;
       const bool in = mine && row0 < p.M && col0 < p.N;
+      const BlockRows rows = block_rows(row0, p.M, p.N);
       float rs = 1.f;
       if (in && w.split < 0) {  // while the accumulators are not there yet
         stage_columns(p.e, p.N, col0, COLS, bias, scale);
@@ -451,39 +507,43 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
       if (ok) ok = wait(acc_full + acc, acc_phase);
       ok = __all_sync(0xFFFFFFFFu, ok);
       sm100::tc_fence_after();
+      // The accumulators are free once they are in registers, before the stores.
+      auto release = [&] {
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CTAS == 2)
+            sm100::mbar_arrive_rank(acc_empty + acc, 0);
+          else
+            sm100::mbar_arrive(acc_empty + acc);
+        }
+      };
+      if (!in) release();
 #pragma unroll 1
       for (int c = 0; in && c < COLS && col0 + c < p.N; c += 32) {
-        const bool res = w.split < 0 && p.e.residual && p.vec;
         uint4 ru[4];
-        if (res) block_fetch(p.e.residual, ru, row0, col0 + c, p.M, p.N);
+        if (w.split < 0 && p.e.residual && p.vec) block_fetch(p.e.residual, ru, rows, col0 + c);
         float v[32];
-        __syncwarp();
         if (ok) {
-          sm100::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + half * COLS + c, v);
+          sm100::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + group * COLS + c, v);
           sm100::tmem_ld_wait();
         } else {
 #pragma unroll
           for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(0x7FC00000u);
         }
+        if (c + 32 >= COLS || col0 + c + 32 >= p.N) release();
         if (w.split < 0) {
-          tile_epilogue(p.e, p.M, p.N, p.vec, v, row0, col0 + c, rs, bias + c, scale + c, block, ru);
+          tile_epilogue(p.e, rows, p.vec, v, col0 + c, rs, bias + c, scale + c, block, ru);
         } else {
           float4 *out = reinterpret_cast<float4 *>(p.partial) +
                         (((int64_t)(w.tile - p.full) * p.splits + w.split) * CTAS + rank) *
                             (BN / 4 * kTileM) +
-                        (half * COLS + c) / 4 * kTileM + quad * 32 + lane;
+                        (group * COLS + c) / 4 * kTileM + quad * 32 + lane;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             out[j * kTileM] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
         }
-      }
-      sm100::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CTAS == 2)
-          sm100::mbar_arrive_rank(acc_empty + acc, 0);
-        else
-          sm100::mbar_arrive(acc_empty + acc);
+        __syncwarp();
       }
       if (++acc == 2) acc = 0, acc_phase ^= 1;
     }
@@ -523,7 +583,8 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_co
   stage_columns(p.e, p.N, col, 32, bias, scale);
   __syncwarp();
   uint4 ru[4];
-  if (p.e.residual && p.vec) block_fetch(p.e.residual, ru, row0, col, p.M, p.N);
+  const BlockRows rows = block_rows(row0, p.M, p.N);
+  if (p.e.residual && p.vec) block_fetch(p.e.residual, ru, rows, col);
   const float rs = p.e.row_scale && row0 + lane < p.M ? __ldg(p.e.row_scale + row0 + lane) : 1.f;
   float v[32];
 #pragma unroll
@@ -539,7 +600,7 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_co
       v[4 * j] += u.x, v[4 * j + 1] += u.y, v[4 * j + 2] += u.z, v[4 * j + 3] += u.w;
     }
   }
-  tile_epilogue(p.e, p.M, p.N, p.vec, v, row0, col, rs, bias, scale, block, ru);
+  tile_epilogue(p.e, rows, p.vec, v, col, rs, bias, scale, block, ru);
 }
 
 // ---------------------------------------------------------------- host side

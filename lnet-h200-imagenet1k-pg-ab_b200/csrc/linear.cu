@@ -15,7 +15,10 @@
 //     products (fp32 on the way, and in the bias' column sums).
 // TMA wants 16-byte aligned rows: an operand with other rows is first copied to
 // the workspace with its rows padded.
+#include <string.h>
+
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_tiles.cuh"
 #include "rows.cuh"
@@ -32,7 +35,7 @@ struct VectorArgs {
   const void *x, *w;
   TileEpilogue e;
   int64_t N, K, x_pitch, w_pitch;
-  int rows;
+  int rows, split;  // warps that share a column's k: 1, 2, 4 or 8
 };
 
 __device__ __forceinline__ float2 e4m3_pair_value(uint16_t q) {
@@ -76,48 +79,68 @@ __device__ __forceinline__ void scalar_epilogue(const TileEpilogue &e, float a, 
   store_f(e.out, off, a);
 }
 
-// R rows of x against every weight row; a warp a column.
+// R rows of x against every weight row.  A warp a column, or, where columns are few, a block's warps
+// share its k in turns and the sums are added in order.
 template <bool FP8, int R, bool VEC>
 __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs p) {
   constexpr int E = FP8 ? 16 : 8, ES = FP8 ? 1 : 2;
   constexpr int U = R <= 2 ? 4 : 2;
-  const int lane = threadIdx.x & 31;
-  const int64_t col = (int64_t)blockIdx.x * (kVectorThreads / 32) + (threadIdx.x >> 5);
-  if (col >= p.N) return;
+  constexpr int WARPS = kVectorThreads / 32;
+  __shared__ float parts[WARPS][R];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int turn = warp & (p.split - 1), stride = 32 * p.split, first = turn * 32 + lane;
+  const int64_t col = (int64_t)blockIdx.x * (WARPS / p.split) + warp / p.split;
+  const bool live = col < p.N;
   float acc[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) acc[r] = 0.f;
-  if (VEC) {
+  if (!live) {
+  } else if (VEC) {
     const uint4 *w = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(p.w) +
                                                      col * p.w_pitch * ES);
     const uint4 *x = reinterpret_cast<const uint4 *>(p.x);
     const int nc = (int)(p.K / E);
-    for (int c0 = lane; c0 < nc; c0 += 32 * U) {
+    for (int c0 = first; c0 < nc; c0 += stride * U) {
       uint4 wu[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        wu[u] = c0 + 32 * u < nc ? __ldg(w + c0 + 32 * u) : make_uint4(0, 0, 0, 0);
+        wu[u] = c0 + stride * u < nc ? __ldg(w + c0 + stride * u) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        if (c0 + 32 * u >= nc) break;
+        if (c0 + stride * u >= nc) break;
         float wv[E];
         operand_values<FP8>(wu[u], wv);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
           if (r >= p.rows) break;
           float xv[E];
-          operand_values<FP8>(__ldg(x + r * (p.x_pitch / E) + c0 + 32 * u), xv);
+          operand_values<FP8>(__ldg(x + r * (p.x_pitch / E) + c0 + stride * u), xv);
 #pragma unroll
           for (int i = 0; i < E; ++i) acc[r] = fmaf(xv[i], wv[i], acc[r]);
         }
       }
     }
   } else {
-    for (int64_t k = lane; k < p.K; k += 32) {
-      const float wv = operand_value<FP8>(p.w, col * p.w_pitch + k);
+    constexpr int S = 8;  // loads in flight: an element each
+    for (int64_t k0 = first; k0 < p.K; k0 += (int64_t)stride * S) {
+      float wv[S];
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (r < p.rows) acc[r] = fmaf(operand_value<FP8>(p.x, r * p.x_pitch + k), wv, acc[r]);
+      for (int u = 0; u < S; ++u) {
+        const int64_t k = k0 + stride * u;
+        wv[u] = k < p.K ? operand_value<FP8>(p.w, col * p.w_pitch + k) : 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r >= p.rows) break;
+        float xv[S];
+#pragma unroll
+        for (int u = 0; u < S; ++u) {
+          const int64_t k = k0 + stride * u;
+          xv[u] = k < p.K ? operand_value<FP8>(p.x, r * p.x_pitch + k) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < S; ++u) acc[r] = fmaf(xv[u], wv[u], acc[r]);
+      }
     }
   }
   float mine = 0.f;
@@ -126,24 +149,48 @@ __global__ void __launch_bounds__(kVectorThreads) vector_kernel(const VectorArgs
     const float s = group_reduce<32, SumOp>(acc[r], nullptr);
     if (lane == r) mine = s;
   }
-  if (lane < p.rows) scalar_epilogue(p.e, mine, lane, col, p.N);
+  if (p.split > 1) {
+    if (lane < R) parts[warp][lane] = mine;
+    __syncthreads();
+    if (turn) return;
+    if (lane < R)
+      for (int s = 1; s < p.split; ++s) mine += parts[warp + s][lane];
+  }
+  if (live && lane < p.rows) scalar_epilogue(p.e, mine, lane, col, p.N);
 }
 
-// Rows copied to a padded pitch (elements of ES bytes; the padding is zero).
+// Rows copied to a padded pitch (elements of ES bytes; the padding is zero).  A lane writes 16 bytes,
+// a warp a stretch of a row.
 template <int ES>
 __global__ void __launch_bounds__(kPackThreads)
 pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols, int64_t src_pitch,
             uint8_t *__restrict__ dst, int64_t pitch) {
-  const int64_t total = rows * pitch;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / pitch, c = i - r * pitch;
-    if (ES == 2) {
-      uint16_t v = 0;
-      if (c < cols) v = reinterpret_cast<const uint16_t *>(src)[r * src_pitch + c];
-      reinterpret_cast<uint16_t *>(dst)[i] = v;
+  using E = std::conditional_t<ES == 2, uint16_t, uint8_t>;
+  constexpr int PER = 16 / ES;
+  const int lane = threadIdx.x & 31;
+  const int64_t stretches = (pitch + 32 * PER - 1) / (32 * PER), total = rows * stretches;
+  for (int64_t s = (int64_t)blockIdx.x * (kPackThreads / 32) + (threadIdx.x >> 5); s < total;
+       s += (int64_t)gridDim.x * (kPackThreads / 32)) {
+    const int64_t r = s / stretches, c0 = ((s - r * stretches) * 32 + lane) * PER;
+    if (c0 >= pitch) continue;
+    const E *from = reinterpret_cast<const E *>(src) + r * src_pitch + c0;
+    E v[PER];
+    if (c0 + PER <= cols) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = __ldg(from + i);
     } else {
-      dst[i] = c < cols ? src[r * src_pitch + c] : 0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] = c0 + i < cols ? __ldg(from + i) : (E)0;
+    }
+    E *to = reinterpret_cast<E *>(dst) + r * pitch + c0;
+    if (c0 + PER <= pitch && (reinterpret_cast<uintptr_t>(to) & 15) == 0) {
+      uint4 u;
+      memcpy(&u, v, 16);
+      *reinterpret_cast<uint4 *>(to) = u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (c0 + i < pitch) to[i] = v[i];
     }
   }
 }
@@ -280,10 +327,10 @@ ProductPlan product_plan(int64_t M, int64_t N, int kblocks) {
     constexpr double kFill = 24;  // pipeline fill and the last epilogue, once
     const double whole = s.block * kblocks + 6;
     for (int splits = 1; splits <= 64; ++splits) {
-      // every split keeps 4 k blocks, and all splits run at once
-      if (splits > 1 && (tail == 0 || tail * splits > slots || kblocks / splits < 4)) break;
+      // every split keeps 4 k blocks, and the splits take 3 rounds at most
+      if (splits > 1 && (tail == 0 || tail * splits > 3 * slots || kblocks / splits < 4)) break;
       double cost = kFill + waves * whole;
-      if (tail) cost += s.block * cdiv(kblocks, splits) + 6;
+      if (tail) cost += cdiv(tail * splits, slots) * (s.block * cdiv(kblocks, splits) + 6);
       // the sums are written and read once (about 6 TB/s), and one more kernel runs (5 us on the
       // GPU and 3 on the host)
       const int64_t floats = splits > 1 ? tail * splits * s.ctas * kTileM * s.bn : 0;
@@ -352,6 +399,9 @@ int product(const TileOperand &a, const TileOperand &b, const TileEpilogue &e, f
   args.m_tiles = q.m_tiles, args.n_tiles = q.n_tiles, args.full = q.full;
   args.splits = q.splits, args.kblocks = kblocks;
   args.partial = partial;
+  args.by_band = FastDiv(kBand * q.n_tiles);
+  args.by_last = FastDiv(q.m_tiles % kBand ? q.m_tiles % kBand : kBand);
+  args.by_splits = FastDiv(q.splits);
   args.vec = N % 8 == 0 && aligned16(e.out) && aligned16(e.pre) && aligned16(e.residual);
   return launch_kind<A_MN, B_MN, FP8>(q, a, b, args, s);
 }
@@ -360,8 +410,9 @@ bool tma_rows(const void *p, int64_t pitch_bytes) { return aligned16(p) && pitch
 
 int launch_pack(const void *src, int64_t rows, int64_t cols, int64_t src_pitch, int elem, void *dst,
                 int64_t pitch, cudaStream_t s) {
-  const int64_t total = rows * pitch;
-  const int blocks = (int)std::min<int64_t>(cdiv(total, kPackThreads * 4), (int64_t)sm_count() * 16);
+  const int64_t warps = rows * cdiv(pitch, 32 * 16 / elem);
+  const int blocks =
+      (int)std::min<int64_t>(cdiv(warps, kPackThreads / 32), (int64_t)sm_count() * 32);
   const auto *from = reinterpret_cast<const uint8_t *>(src);
   auto *to = reinterpret_cast<uint8_t *>(dst);
   if (elem == 2)
@@ -469,7 +520,7 @@ BackwardWork backward_work(Arena &ar, const lnet_b200_linear_request *q, const v
 
 template <bool FP8, bool VEC>
 void launch_vector(const VectorArgs &v, cudaStream_t s) {
-  const unsigned blocks = (unsigned)cdiv(v.N, kVectorThreads / 32);
+  const unsigned blocks = (unsigned)cdiv(v.N, kVectorThreads / 32 / v.split);
   if (v.rows == 1)
     vector_kernel<FP8, 1, VEC><<<blocks, kVectorThreads, 0, s>>>(v);
   else if (v.rows == 2)
@@ -521,10 +572,15 @@ extern "C" int lnet_b200_linear_forward(const lnet_b200_linear_request *req, voi
   e.col_scale = fp8 ? req->weight_scale : nullptr;
   e.act = req->activation;
   if (req->rows <= kVectorRows) {
-    const VectorArgs v{req->x,       req->weight,  e,           req->outer, req->inner,
-                       x_pitch(req), w_pitch(req), (int)req->rows};
+    VectorArgs v{req->x,       req->weight,  e,           req->outer, req->inner,
+                 x_pitch(req), w_pitch(req), (int)req->rows, 1};
     const bool vec = req->inner * elem % 16 == 0 && tma_rows(req->x, x_pitch(req) * elem) &&
                      tma_rows(req->weight, w_pitch(req) * elem);
+    // two blocks an SM, as long as every warp keeps a load a lane
+    const int64_t loads = req->inner * elem / (vec ? 16 : elem);
+    while (v.split < kVectorThreads / 32 && v.N * v.split < (int64_t)sm_count() * 16 &&
+           loads >= 64 * v.split)
+      v.split *= 2;
     if (fp8)
       vec ? launch_vector<true, true>(v, stream) : launch_vector<true, false>(v, stream);
     else

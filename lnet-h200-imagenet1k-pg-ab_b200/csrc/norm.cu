@@ -13,11 +13,13 @@
 // warp (the fewest that hold it in 4 chunks each, so that a 96-wide bf16 row
 // uses 4 lanes x 3 chunks and no lane idles); a longer one to a block of up to
 // 512 threads; one that 512 threads cannot hold is read again from L2 (wide
-// kernels).
+// kernels).  Rows of other lengths than a multiple of 16 bytes keep the 16-byte
+// loads, shifted to the boundaries (SHIFT).
 #include <cuda_fp8.h>
 
 #include <algorithm>
 #include <atomic>
+#include <initializer_list>
 
 #include "rows.cuh"
 #include "sm100.cuh"
@@ -77,14 +79,16 @@ __device__ __forceinline__ void weight_lanes(const void *w, bool w_bf16, int c, 
 __device__ __forceinline__ uint32_t e4m3_pair(float a, float b) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
 }
-// e4m3(v k) of a chunk, saturating.
-template <int VEC>
-__device__ __forceinline__ void store_e4m3(uint8_t *p, const Lanes<VEC> *l, float k) {
+// e4m3(v k) of the chunk of a row that starts at element e0, saturating.
+template <int VEC, bool SHIFT = false>
+__device__ __forceinline__ void store_e4m3(uint8_t *row, const Lanes<VEC> *l, float k, int64_t e0,
+                                           int dim) {
   Lanes<VEC> s[lanes_of<VEC>()];
   float v[VEC];
 #pragma unroll
   for (int i = 0; i < lanes_of<VEC>(); ++i) s[i] = l[i] * splat<VEC>(k);
   from_lanes<VEC>(s, v);
+  uint8_t *p = row + e0;
   if constexpr (VEC == 1) {
     *p = (uint8_t)e4m3_pair(v[0], 0.f);
   } else {
@@ -92,10 +96,15 @@ __device__ __forceinline__ void store_e4m3(uint8_t *p, const Lanes<VEC> *l, floa
 #pragma unroll
     for (int i = 0; i < VEC / 4; ++i)
       q[i] = e4m3_pair(v[4 * i], v[4 * i + 1]) | (e4m3_pair(v[4 * i + 2], v[4 * i + 3]) << 16);
-    if constexpr (VEC == 8)
+    if constexpr (SHIFT) {  // rows of bytes keep no alignment
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        if (e0 + i >= 0 && e0 + i < dim) p[i] = (uint8_t)(q[i / 4] >> (8 * (i % 4)));
+    } else if constexpr (VEC == 8) {
       *reinterpret_cast<uint2 *>(p) = make_uint2(q[0], q[1]);
-    else
+    } else {
       *reinterpret_cast<uint32_t *>(p) = q[0];
+    }
   }
 }
 // Scale of a row whose y is f t, and the factor k that takes t to its codes: with m = max|t|,
@@ -127,32 +136,83 @@ struct NormArgs {
   int w_bf16;
 };
 
-// Brings the rows of a block's next turn, which lie together, to L2: one instruction a tensor, and
-// the next turn waits for L2 in place of HBM.
+// Brings the rows of a block's next turn, which lie together, to L2 (whole 16-byte units): one
+// instruction a tensor, and the next turn waits for L2 in place of HBM.
 template <typename T, int VEC>
 __device__ __forceinline__ void prefetch_rows(const T *p, int64_t base, int per, int64_t rows,
                                               int64_t dim) {
   if (VEC == 1 || p == nullptr || base >= rows) return;
-  const int64_t n = min((int64_t)per, rows - base) * dim * (int64_t)sizeof(T);
-  sm100::bulk_prefetch_l2(p + base * dim, (uint32_t)n);
+  const uintptr_t from = (reinterpret_cast<uintptr_t>(p + base * dim) + 15) & ~(uintptr_t)15;
+  const uintptr_t to =
+      reinterpret_cast<uintptr_t>(p + (base + min((int64_t)per, rows - base)) * dim) &
+      ~(uintptr_t)15;
+  if (to > from) sm100::bulk_prefetch_l2(reinterpret_cast<const void *>(from), (uint32_t)(to - from));
 }
 
-template <typename T, int VEC, int G, bool FP8>
+// Rows whose length is no multiple of 16 bytes (SHIFT): a row's chunks start at the 16-byte boundary
+// before it, so chunk c holds elements c VEC - shift on, and its first and last may be cut.  Every
+// tensor of a call has the same shift in a row, and a thread's rows are a multiple of VEC apart, so
+// its shift, its columns and their weights are the same in every row that it takes.
+template <typename T, int VEC>
+__device__ __forceinline__ int row_shift(const T *row) {
+  return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+template <typename T, int VEC, bool SHIFT>
+__device__ __forceinline__ void load_part(RowChunk<T, VEC> &k, const T *row, int e0, int dim) {
+  if (!SHIFT || (e0 >= 0 && e0 + VEC <= dim)) {
+    k.load(row + e0);
+  } else {
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = e0 + i >= 0 && e0 + i < dim ? load_f(row, e0 + i) : 0.f;
+    k.put(v);
+  }
+}
+template <typename T, int VEC, bool SHIFT>
+__device__ __forceinline__ void store_part(const RowChunk<T, VEC> &k, T *row, int e0, int dim) {
+  if (!SHIFT || (e0 >= 0 && e0 + VEC <= dim)) {
+    k.store(row + e0);
+  } else {
+    float v[VEC];
+    k.get(v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (e0 + i >= 0 && e0 + i < dim) store_f(row, e0 + i, v[i]);
+  }
+}
+template <int VEC, bool SHIFT>
+__device__ __forceinline__ void weight_part(const void *w, bool w_bf16, int c, int e0, int dim,
+                                            Lanes<VEC> *p) {
+  if (!SHIFT) {
+    weight_lanes<VEC>(w, w_bf16, c, p);
+  } else {
+    float v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      v[i] = e0 + i >= 0 && e0 + i < dim ? weight_at(w, w_bf16, e0 + i) : 0.f;
+    to_lanes<VEC>(v, p);
+  }
+}
+
+template <typename T, int VEC, int G, bool FP8, bool SHIFT>
 __global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
 norm_forward_kernel(const NormArgs a) {
   constexpr int NV = chunks_of<VEC>();
   __shared__ float scratch[33];
   const int g = G ? G : blockDim.x;
   const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
-  const int nvec = (int)(a.dim / VEC);
   const T *x = reinterpret_cast<const T *>(a.x), *r = reinterpret_cast<const T *>(a.r);
+  const int dim = (int)a.dim;
+  const int shift =
+      SHIFT ? row_shift<T, VEC>(x + ((int64_t)blockIdx.x * per + sub) * a.dim) : 0;
+  const int nvec = (dim + shift + VEC - 1) / VEC;
   constexpr int NP = lanes_of<VEC>();
   using L = Lanes<VEC>;
   L w[NV][NP];  // a thread's columns are the same in every row
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = lane + j * g;
-    if (c < nvec) weight_lanes<VEC>(a.w, a.w_bf16, c, w[j]);
+    if (c < nvec) weight_part<VEC, SHIFT>(a.w, a.w_bf16, c, c * VEC - shift, dim, w[j]);
   }
   for (int64_t base = (int64_t)blockIdx.x * per; base < a.rows;
        base += (int64_t)gridDim.x * per) {
@@ -168,14 +228,14 @@ norm_forward_kernel(const NormArgs a) {
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       cx[j].zero();
-      if (live && c < nvec) cx[j].load(x + off + (int64_t)c * VEC);
+      if (live && c < nvec) load_part<T, VEC, SHIFT>(cx[j], x + off, c * VEC - shift, dim);
     }
     if (r) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = lane + j * g;
         cr[j].zero();
-        if (live && c < nvec) cr[j].load(r + off + (int64_t)c * VEC);
+        if (live && c < nvec) load_part<T, VEC, SHIFT>(cr[j], r + off, c * VEC - shift, dim);
       }
     }
     L sum = splat<VEC>(0.f);
@@ -190,7 +250,8 @@ norm_forward_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) v[i] = v[i] + u[i];
         put_lanes(cx[j], v);  // the stream, rounded to its type
-        if (live && c < nvec) cx[j].store(reinterpret_cast<T *>(a.h) + off + (int64_t)c * VEC);
+        if (live && c < nvec)
+          store_part<T, VEC, SHIFT>(cx[j], reinterpret_cast<T *>(a.h) + off, c * VEC - shift, dim);
         get_lanes(cx[j], v);
       }
 #pragma unroll
@@ -217,7 +278,8 @@ norm_forward_kernel(const NormArgs a) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = lane + j * g;
-        if (live && c < nvec) store_e4m3<VEC>(a.q + off + (int64_t)c * VEC, t[j], k);
+        if (live && c < nvec)
+          store_e4m3<VEC, SHIFT>(a.q + off, t[j], k, c * VEC - shift, dim);
       }
     } else {
       const L f = splat<VEC>(rstd);
@@ -230,7 +292,7 @@ norm_forward_kernel(const NormArgs a) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) v[i] = v[i] * f * w[j][i];
         put_lanes(cx[j], v);
-        cx[j].store(reinterpret_cast<T *>(a.y) + off + (int64_t)c * VEC);
+        store_part<T, VEC, SHIFT>(cx[j], reinterpret_cast<T *>(a.y) + off, c * VEC - shift, dim);
       }
     }
   }
@@ -272,7 +334,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
       const float v = load_f(h, off + c), w = weight_at(a.w, a.w_bf16, c);
       if (FP8) {
         const Single t{v * w};
-        store_e4m3<1>(a.q + off + c, &t, k);
+        store_e4m3<1>(a.q + off, &t, k, c, 0);
       } else {
         store_f(reinterpret_cast<T *>(a.y), off + c, v * rstd * w);
       }
@@ -306,7 +368,7 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t
       Lanes<VEC> l[lanes_of<VEC>()];
       u.load(p + c * VEC);
       get_lanes(u, l);
-      store_e4m3<VEC>(q + row * dim + c * VEC, l, k);
+      store_e4m3<VEC>(q + row * dim, l, k, c * VEC, 0);
     }
   }
 }
@@ -335,19 +397,38 @@ struct NormGradArgs {
   int w_bf16;
 };
 
-template <typename T, int VEC, int G>
-__global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
+template <typename T, int VEC, int G, bool SHIFT>
+__global__ void __launch_bounds__(G || SHIFT ? kSubThreads : kBlockThreads)
 norm_backward_kernel(const NormGradArgs a) {
   constexpr int NV = chunks_of<VEC>();
   __shared__ float scratch[33];
-  __shared__ float columns[G ? G * NV * VEC : 1];
+  __shared__ float columns[G ? G * NV * VEC : 1];  // (dim <= that, whatever the shift)
   const int g = G ? G : blockDim.x;
   const int lane = threadIdx.x % g, sub = threadIdx.x / g, per = blockDim.x / g;
-  const int nvec = (int)(a.dim / VEC);
   const T *hp = reinterpret_cast<const T *>(a.h), *dyp = reinterpret_cast<const T *>(a.dy);
   const T *dhp = reinterpret_cast<const T *>(a.dh);
+  const int dim = (int)a.dim;
+  const int shift =
+      SHIFT ? row_shift<T, VEC>(hp + ((int64_t)blockIdx.x * per + sub) * a.dim) : 0;
+  const int nvec = (dim + shift + VEC - 1) / VEC;
   constexpr int NP = lanes_of<VEC>();
   using L = Lanes<VEC>;
+  L kept[SHIFT ? NV : 1][NP];  // weights that are no whole chunk of memory stay in registers
+  if (SHIFT) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = lane + j * g;
+      if (c < nvec) weight_part<VEC, SHIFT>(a.w, a.w_bf16, c, c * VEC - shift, dim, kept[SHIFT ? j : 0]);
+    }
+  }
+  auto weights = [&](int j, int c, L *w) {
+    if (SHIFT) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) w[i] = kept[SHIFT ? j : 0][i];
+    } else {
+      weight_lanes<VEC>(a.w, a.w_bf16, c, w);
+    }
+  };
   L dwp[NV][NP];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -368,9 +449,10 @@ norm_backward_kernel(const NormGradArgs a) {
       const int c = lane + j * g;
       ch[j].zero(), cy[j].zero(), cs[j].zero();
       if (live && c < nvec) {
-        ch[j].load(hp + off + (int64_t)c * VEC);
-        cy[j].load(dyp + off + (int64_t)c * VEC);
-        if (dhp) cs[j].load(dhp + off + (int64_t)c * VEC);
+        const int e0 = c * VEC - shift;
+        load_part<T, VEC, SHIFT>(ch[j], hp + off, e0, dim);
+        load_part<T, VEC, SHIFT>(cy[j], dyp + off, e0, dim);
+        if (dhp) load_part<T, VEC, SHIFT>(cs[j], dhp + off, e0, dim);
       }
     }
     const float rstd = live ? __ldg(a.rstd + row) : 0.f;
@@ -382,7 +464,7 @@ norm_backward_kernel(const NormGradArgs a) {
       if (c >= nvec) continue;
       L h[NP], dy[NP], w[NP];
       get_lanes(ch[j], h), get_lanes(cy[j], dy);
-      weight_lanes<VEC>(a.w, a.w_bf16, c, w);
+      weights(j, c, w);
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const L t = dy[i] * (h[i] * f);
@@ -399,11 +481,11 @@ norm_backward_kernel(const NormGradArgs a) {
       if (!live || c >= nvec) continue;
       L h[NP], dy[NP], s[NP], w[NP];
       get_lanes(ch[j], h), get_lanes(cy[j], dy), get_lanes(cs[j], s);
-      weight_lanes<VEC>(a.w, a.w_bf16, c, w);
+      weights(j, c, w);
 #pragma unroll
       for (int i = 0; i < NP; ++i) s[i] = fma(f, fma(h[i], minus, dy[i] * w[i]), s[i]);
       put_lanes(cs[j], s);
-      cs[j].store(reinterpret_cast<T *>(a.dx) + off + (int64_t)c * VEC);
+      store_part<T, VEC, SHIFT>(cs[j], reinterpret_cast<T *>(a.dx) + off, c * VEC - shift, dim);
     }
   }
   if (!a.partial) return;
@@ -411,38 +493,49 @@ norm_backward_kernel(const NormGradArgs a) {
 #pragma unroll
   for (int j = 0; j < NV; ++j) from_lanes<VEC>(dwp[j], dw[j]);
   float *out = a.partial + (int64_t)blockIdx.x * a.dim;
-  if (G == 0) {
+  auto each_column = [&](auto &&f) {  // (column, sum) of the thread's own
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = lane + j * g;
       if (c >= nvec) continue;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) out[(int64_t)c * VEC + i] = dw[j][i];
+      for (int i = 0; i < VEC; ++i) {
+        const int col = c * VEC - shift + i;
+        if (!SHIFT || (col >= 0 && col < dim)) f(col, dw[j][i]);
+      }
     }
+  };
+  if (G == 0) {
+    each_column([&](int col, float v) { out[col] = v; });
   } else {  // the warp's rows, then one warp after another: the same order every time
+    if (!SHIFT) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
+        for (int i = 0; i < VEC; ++i)
 #pragma unroll
-        for (int o = 16; o >= (G ? G : 32); o >>= 1)
-          dw[j][i] += __shfl_xor_sync(0xFFFFFFFFu, dw[j][i], o);
+          for (int o = 16; o >= (G ? G : 32); o >>= 1)
+            dw[j][i] += __shfl_xor_sync(0xFFFFFFFFu, dw[j][i], o);
+    }
+    // lanes of different rows hold different columns where rows are shifted: one group after another
+    constexpr int kTurns = SHIFT && G ? 32 / (G ? G : 32) : 1;
+    if (SHIFT) {
+      for (int c = threadIdx.x; c < dim; c += blockDim.x) columns[c] = 0.f;
+      __syncthreads();
+    }
     for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-      if ((int)threadIdx.x / 32 == w && (threadIdx.x & 31) < (unsigned)g) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int c = lane + j * g;
-          if (c >= nvec) continue;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) {
-            float *p = columns + c * VEC + i;
-            *p = w ? *p + dw[j][i] : dw[j][i];
-          }
+      if ((int)threadIdx.x / 32 == w) {
+        for (int turn = 0; turn < kTurns; ++turn) {
+          if ((int)(threadIdx.x & 31) / g == turn)
+            each_column([&](int col, float v) {
+              columns[col] = SHIFT || w ? columns[col] + v : v;
+            });
+          __syncwarp();
         }
       }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < (int)a.dim; c += blockDim.x) out[c] = columns[c];
+    for (int c = threadIdx.x; c < dim; c += blockDim.x) out[c] = columns[c];
   }
 }
 
@@ -499,27 +592,35 @@ norm_columns_kernel(const float *__restrict__ partial, int blocks, int64_t dim, 
   }
 }
 
+// How rows are read: an element at a time, in chunks, or in chunks shifted to their boundaries.
+enum RowAccess { kScalarRows, kChunkRows, kShiftedRows };
+
 // Threads, lanes a row, row groups and blocks (at most) of a call (lanes 0: a block a row).
 struct NormPlan {
   int lanes, threads, blocks;
   int64_t groups;
-  bool vec, wide;
+  RowAccess access;
+  bool wide;
 };
 
-NormPlan norm_plan(int64_t rows, int64_t dim, int elem, bool aligned, int blocks_per_sm) {
+NormPlan norm_plan(int64_t rows, int64_t dim, int elem, RowAccess access, int blocks_per_sm) {
   NormPlan p{};
   const int vec = 16 / elem;
-  p.vec = aligned && dim % vec == 0;
-  const int nv = p.vec ? 4 : 16;
-  const int64_t nvec = p.vec ? dim / vec : dim;
+  p.access = access;
+  const int nv = access == kScalarRows ? 16 : 4;
+  const int64_t nvec = access == kScalarRows  ? dim
+                       : access == kChunkRows ? dim / vec
+                                              : cdiv(dim + vec - 1, vec);
   int64_t per = 1;
   if (nvec <= (int64_t)32 * nv) {
     p.lanes = 4;
     while ((int64_t)p.lanes * nv < nvec) p.lanes *= 2;
     p.threads = kSubThreads;
     per = kSubThreads / p.lanes;
-  } else if (nvec <= (int64_t)kBlockThreads * nv) {
+  } else if (nvec <= (int64_t)(access == kShiftedRows ? kSubThreads : kBlockThreads) * nv) {
     p.threads = (int)((cdiv(nvec, nv) + 31) / 32 * 32);
+  } else if (access == kShiftedRows) {
+    return norm_plan(rows, dim, elem, kScalarRows, blocks_per_sm);
   } else {
     p.wide = true;
     p.threads = kWideThreads;
@@ -529,6 +630,17 @@ NormPlan norm_plan(int64_t rows, int64_t dim, int elem, bool aligned, int blocks
   const int most = blocks_per_sm * std::max(1, 256 / p.threads);
   p.blocks = (int)std::min<int64_t>(p.groups, (int64_t)sm_count() * most);
   return p;
+}
+
+// `first` and `others`: the call's tensors of rows (null: none); w: its weight.
+RowAccess row_access(int64_t dim, int elem, const void *w, const void *first,
+                     std::initializer_list<const void *> others) {
+  const int vec = 16 / elem;
+  for (const void *p : others)
+    if (p && ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(first)) & 15))
+      return kScalarRows;
+  if (dim % vec == 0 && aligned16(first) && aligned16(w)) return kChunkRows;
+  return dim >= 2 * vec ? kShiftedRows : kScalarRows;
 }
 
 // The grid of a persistent kernel: as many blocks as run at once (a second, shorter wave would
@@ -544,7 +656,10 @@ int resident_blocks(const NormPlan &p) {
       n = 1;
     k.store(n);
   }
-  return (int)std::min<int64_t>(p.blocks, (int64_t)sm_count() * n);
+  const int64_t blocks = std::min<int64_t>(p.blocks, (int64_t)sm_count() * n);
+  // shifted rows of a thread lie a multiple of 8 apart (several rows a block always do)
+  return (int)(p.access == kShiftedRows && p.lanes == 0 && blocks < p.groups ? blocks / 8 * 8
+                                                                             : blocks);
 }
 
 // most blocks of an SM; each of the gradient's writes its column sums
@@ -557,47 +672,53 @@ int launch_rows(const NormPlan &p, const A &a, cudaStream_t s) {
   return blocks;
 }
 
-template <typename T, int VEC, bool FP8>
+template <typename T, int VEC, bool FP8, bool SHIFT>
 void launch_forward(const NormPlan &p, const NormArgs &a, cudaStream_t s) {
   switch (p.lanes) {
-    case 4: launch_rows<norm_forward_kernel<T, VEC, 4, FP8>>(p, a, s); break;
-    case 8: launch_rows<norm_forward_kernel<T, VEC, 8, FP8>>(p, a, s); break;
-    case 16: launch_rows<norm_forward_kernel<T, VEC, 16, FP8>>(p, a, s); break;
-    case 32: launch_rows<norm_forward_kernel<T, VEC, 32, FP8>>(p, a, s); break;
-    default: launch_rows<norm_forward_kernel<T, VEC, 0, FP8>>(p, a, s); break;
+    case 4: launch_rows<norm_forward_kernel<T, VEC, 4, FP8, SHIFT>>(p, a, s); break;
+    case 8: launch_rows<norm_forward_kernel<T, VEC, 8, FP8, SHIFT>>(p, a, s); break;
+    case 16: launch_rows<norm_forward_kernel<T, VEC, 16, FP8, SHIFT>>(p, a, s); break;
+    case 32: launch_rows<norm_forward_kernel<T, VEC, 32, FP8, SHIFT>>(p, a, s); break;
+    default: launch_rows<norm_forward_kernel<T, VEC, 0, FP8, SHIFT>>(p, a, s); break;
   }
 }
 
 template <typename T, bool FP8>
 int forward_typed(const NormArgs &a, cudaStream_t s) {
-  const bool aligned = aligned16(a.x) && aligned16(a.r) && aligned16(a.h) && aligned16(a.y) &&
-                       aligned16(a.q) && aligned16(a.w);
-  const NormPlan p = norm_plan(a.rows, a.dim, sizeof(T), aligned, kForwardBlocks);
+  RowAccess access = row_access(a.dim, sizeof(T), a.w, a.x, {a.r, a.h, a.y});
+  if (access == kChunkRows && !aligned16(a.q)) access = kShiftedRows;
+  const NormPlan p = norm_plan(a.rows, a.dim, sizeof(T), access, kForwardBlocks);
   if (p.wide)
     launch_rows<norm_forward_wide_kernel<T, FP8>>(p, a, s);
-  else if (p.vec)
-    launch_forward<T, vec_of<T>(), FP8>(p, a, s);
+  else if (p.access == kChunkRows)
+    launch_forward<T, vec_of<T>(), FP8, false>(p, a, s);
+  else if (p.access == kShiftedRows)
+    launch_forward<T, vec_of<T>(), FP8, true>(p, a, s);
   else
-    launch_forward<T, 1, FP8>(p, a, s);
+    launch_forward<T, 1, FP8, false>(p, a, s);
   return after_launch("norm_forward_kernel");
 }
 
 // The gradient's kernel; returns its blocks.
-template <typename T, int VEC>
+template <typename T, int VEC, bool SHIFT>
 int launch_backward(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
   switch (p.lanes) {
-    case 4: return launch_rows<norm_backward_kernel<T, VEC, 4>>(p, a, s);
-    case 8: return launch_rows<norm_backward_kernel<T, VEC, 8>>(p, a, s);
-    case 16: return launch_rows<norm_backward_kernel<T, VEC, 16>>(p, a, s);
-    case 32: return launch_rows<norm_backward_kernel<T, VEC, 32>>(p, a, s);
-    default: return launch_rows<norm_backward_kernel<T, VEC, 0>>(p, a, s);
+    case 4: return launch_rows<norm_backward_kernel<T, VEC, 4, SHIFT>>(p, a, s);
+    case 8: return launch_rows<norm_backward_kernel<T, VEC, 8, SHIFT>>(p, a, s);
+    case 16: return launch_rows<norm_backward_kernel<T, VEC, 16, SHIFT>>(p, a, s);
+    case 32: return launch_rows<norm_backward_kernel<T, VEC, 32, SHIFT>>(p, a, s);
+    default: return launch_rows<norm_backward_kernel<T, VEC, 0, SHIFT>>(p, a, s);
   }
 }
 
 template <typename T>
 int backward_typed(const NormPlan &p, const NormGradArgs &a, cudaStream_t s) {
   if (p.wide) return launch_rows<norm_backward_wide_kernel<T>>(p, a, s);
-  return p.vec ? launch_backward<T, vec_of<T>()>(p, a, s) : launch_backward<T, 1>(p, a, s);
+  switch (p.access) {
+    case kChunkRows: return launch_backward<T, vec_of<T>(), false>(p, a, s);
+    case kShiftedRows: return launch_backward<T, vec_of<T>(), true>(p, a, s);
+    default: return launch_backward<T, 1, false>(p, a, s);
+  }
 }
 
 int check_norm(const char *what, int64_t rows, int64_t dim, int dtype, int weight_dtype,
@@ -617,9 +738,11 @@ int check_norm(const char *what, int64_t rows, int64_t dim, int dtype, int weigh
 }
 
 int norm_grad_blocks(int64_t rows, int64_t dim, int elem) {
-  // the larger of the aligned and the unaligned plan: the size query does not see the pointers
-  return std::max(norm_plan(rows, dim, elem, true, kBackwardBlocks).blocks,
-                  norm_plan(rows, dim, elem, false, kBackwardBlocks).blocks);
+  // the most of any access: the size query does not see the pointers
+  int blocks = 0;
+  for (RowAccess a : {kScalarRows, kChunkRows, kShiftedRows})
+    blocks = std::max(blocks, norm_plan(rows, dim, elem, a, kBackwardBlocks).blocks);
+  return blocks;
 }
 
 }  // namespace
@@ -710,10 +833,8 @@ extern "C" int lnet_b200_residual_rms_norm_backward(
     return LNET_OK;
   }
   const int elem = dtype == LNET_BF16 ? 2 : 4;
-  const bool aligned =
-      aligned16(stream_in) && aligned16(dy) && aligned16(dstream) && aligned16(dx) &&
-      aligned16(weight);
-  const NormPlan p = norm_plan(rows, dim, elem, aligned, kBackwardBlocks);
+  const RowAccess access = row_access(dim, elem, weight, stream_in, {dy, dstream, dx});
+  const NormPlan p = norm_plan(rows, dim, elem, access, kBackwardBlocks);
   const size_t need = dweight ? (size_t)p.blocks * (size_t)dim * sizeof(float) : 0;
   if (need > workspace_bytes || (need && !workspace))
     return fail(LNET_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", what, need,

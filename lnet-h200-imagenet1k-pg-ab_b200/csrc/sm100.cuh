@@ -332,29 +332,12 @@ __device__ __forceinline__ uint32_t map_to_rank(const void *p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+// Arrival on CTA `rank`'s copy of `bar`.  It orders what the thread did in TMEM and shared memory;
+// a release of cluster scope would also wait for its global stores on the way.
 __device__ __forceinline__ void mbar_arrive_rank(uint64_t *bar, uint32_t rank) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
                    map_to_rank(bar, rank))
                : "memory");
-}
-// mbar_try_wait that also acquires what the other CTA of the pair released.
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint64_t *bar, uint32_t parity,
-                                                      uint32_t hint_ns) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity), "r"(hint_ns)
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait_cluster_bounded(uint64_t *bar, uint32_t parity,
-                                                          uint32_t limit) {
-  for (uint32_t i = 0; i < limit; ++i)
-    if (mbar_try_wait_cluster(bar, parity, 1000u)) return true;
-  return false;
 }
 // Four floats into CTA `rank`'s copy of `dst` (16-byte aligned); completes 16 bytes on its copy of
 // `bar`.

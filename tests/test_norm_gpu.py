@@ -23,10 +23,10 @@ FP32 = 4e-6
 HALF_ULP = {torch.float32: 0.0, torch.bfloat16: torch.finfo(torch.bfloat16).eps / 2}
 DTYPES = [torch.float32, torch.bfloat16]
 # one element, a lane group of each size, odd widths, a block a row, rows that no block holds, and
-# enough rows for a warp a row
+# many rows of odd and even widths
 SHAPES = [(1, 1), (1, 96), (7, 64), (300, 96), (5, 3, 128), (33, 257), (19, 1001), (64, 1024),
           (9, 4096), (3, 8200), (2, 8193), (2, 16392), (2, 20001), (1300, 2048), (1201, 4096),
-          (1211, 1544)]
+          (1211, 1544), (3001, 97), (2500, 1001), (700, 2049), (20011, 33)]
 
 
 def make(shape, dtype, seed, device, std=1.0):
