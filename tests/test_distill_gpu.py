@@ -258,6 +258,7 @@ def test_no_rows_no_entries_and_determinism(cuda_device):
     loss = distillation_loss(z, index[:, :0], teacher[:, :0], labels=labels, alpha=0.0)
     ref = reference(z, index[:, :0], teacher[:, :0], labels, 1.0, 0.0, "mean")
     assert float(loss) == pytest.approx(float(ref), rel=1e-5)
+    check(z, index[:, :0], teacher[:, :0], labels, 1.0, 0.0, "mean", torch.float32)
     z, index, teacher, labels = make(500, 1000, 10, torch.bfloat16, 3, cuda_device)
     z.requires_grad_()
     runs = []

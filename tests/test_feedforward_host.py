@@ -204,3 +204,15 @@ def test_feedforward_module_on_cpu():
         B200FeedForward(96, 0)
     with pytest.raises(ValueError):
         B200FeedForward(96, 384, activation="tanh")
+
+
+def test_request_layouts_match_the_header():
+    import re
+
+    from conftest import ROOT
+
+    text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "lnet_b200.h").read_text(), flags=re.S)
+    for name, py in (("lnet_b200_linear_request", _lib.LinearRequest),
+                     ("lnet_b200_distill_request", _lib.DistillRequest)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S)
+        assert re.findall(r"(\w+)\s*;", body.group(1)) == [f for f, _ in py._fields_]
