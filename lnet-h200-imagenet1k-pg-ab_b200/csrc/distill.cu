@@ -542,7 +542,7 @@ distill_resident_kernel(const ResidentArgs ra) {
     sm100::mbar_init(landed + tid, 1);
   }
   sm100::fence_barrier_init();
-  bool failed = false;  // a wait gave up: NaN from then on
+  bool failed = false;  // a wait of this thread gave up: NaN from then on
 
   int count = 0;
   for (int i = lane; i < a.n_counts; i += 32) count += a.counts[i];
@@ -619,6 +619,8 @@ distill_resident_kernel(const ResidentArgs ra) {
     held_rows = 0;
   };
   if (tid == 0 && first < a.rows) fetch_row(first, 0);
+  bool coming = true;  // the row was asked for; after a failure no more are, and those that were
+                       // are waited for: no block leaves while a copy is on its way to it
   int set = 0;
   uint32_t phase = 0;
   for (int64_t row = first; row < a.rows; row += step, phase ^= set, set ^= 1) {
@@ -626,8 +628,10 @@ distill_resident_kernel(const ResidentArgs ra) {
     const Entry *entries = ra.entries + row * slots;
     Entry e = tid < slots ? entries[tid] : Entry{-1, 0.f};
     const RowInfo info = ra.info[row];
-    if (tid == 0 && row + step < a.rows) fetch_row(row + step, set ^ 1);
-    if (!failed) failed = !sm100::mbar_wait_bounded(landed + set, phase, 1000000u);
+    const bool wanted = coming;
+    coming = !failed && row + step < a.rows;
+    if (tid == 0 && coming) fetch_row(row + step, set ^ 1);
+    if (wanted && !sm100::mbar_wait_bounded(landed + set, phase, 1000000u)) failed = true;
     // Most parts lie inside their row: without a check a chunk their loads and stores are one
     // instruction each.
     const int shift = shift_of(row);

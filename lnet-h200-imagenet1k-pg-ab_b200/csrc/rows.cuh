@@ -243,7 +243,7 @@ int raise_shared_memory(int bytes, const char *what) {
   return LNET_OK;
 }
 
-// SMs of the current device (queried once per process; every GPU of a box is
+// SMs of the current device (queried once per process; every GPU of a machine is
 // the same part).
 inline int sm_count() {
   static const int n = [] {

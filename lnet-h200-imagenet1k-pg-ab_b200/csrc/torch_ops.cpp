@@ -304,7 +304,8 @@ Tensor distill_backward(const Tensor &z, const Tensor &index, const Tensor &teac
 }
 
 // A reduced loss takes its gradient in the forward pass, while the row is on chip; the backward
-// pass scales it in place by the loss's gradient (a launch that reads one value where that is 1).
+// pass scales it in place by the loss's gradient (a launch that reads one value where that is 1;
+// for another value a bf16 gradient is rounded twice, half a unit in the last place each time).
 // The rows' losses (no reduction), and a second backward pass, take it from the logits again.
 struct DistillFunction : torch::autograd::Function<DistillFunction> {
   static Tensor forward(AutogradContext *ctx, const Tensor &logits, const Tensor &indices,
