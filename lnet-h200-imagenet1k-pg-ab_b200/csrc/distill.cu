@@ -486,9 +486,12 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 // 8; 315 with six of 64 threads; 341 with one of 256.  What bounds it is the time that a cluster's
 // blocks wait for the slowest of them (0.4 instructions a clock and scheduler), at 0.57 of the measured
 // HBM rate; the sweep-twice kernel took 637 us.  Rows of up to 128 x 4 chunks take 4 chunks a thread
-// and one block; rows that 8 blocks of 128 x 8 do not hold take up to 512 threads of 4.
-constexpr int kSmallThreads = 128;
-constexpr int kLargeThreads = 512;
+// and one block; more take as many blocks of 128 x 8 as hold them, any number up to 8 (2000 x 40000: 5
+// blocks 100 us, 8 blocks 158, the other kernel 137).  Rows that 8 do not hold are the other kernel's:
+// 2000 x 131000 took 341 us there and 485 here with 512 threads of 4 chunks.
+// Rows that start inside 16 bytes: 2000 x 50257 172 us (the other kernel 166, and 24 more for the count
+// and the sum against 16 for the teacher's side), 2000 x 40001 122 (144).
+constexpr int kResidentThreads = 128;
 constexpr int kResidentParts = 8;
 
 struct Listed {
@@ -513,23 +516,23 @@ struct ResidentArgs {
 };
 
 // NT: the block's threads where they are known, else 0.
-template <typename T, bool TWO, bool ALIGNED, int MAXT, int NV, int NT>
-__global__ void __launch_bounds__(MAXT, MAXT == kLargeThreads ? 1 : NV == 4 ? 4 : 3)
+template <typename T, bool TWO, bool ALIGNED, int NV, int NT>
+__global__ void __launch_bounds__(kResidentThreads, NV == 4 ? 4 : 3)
 distill_resident_kernel(const ResidentArgs ra) {
   constexpr int VEC = vec_of<T>();
   const DistillArgs &a = ra.d;
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
-  __shared__ float4 stats[2][kResidentParts * MAXT / 32];  // m, sum tau, sum 1
+  __shared__ float4 stats[2][kResidentParts * kResidentThreads / 32];  // m, sum tau, sum 1
   // in block 0, of every warp's entries: sum of c (r - z), sum of c, r
-  __shared__ float4 shares[2][kResidentParts * MAXT / 32];
+  __shared__ float4 shares[2][kResidentParts * kResidentThreads / 32];
   __shared__ uint64_t joined[2], landed[2];
   extern __shared__ __align__(16) uint4 row_smem[];  // two parts of a row, in turn
-  __shared__ int head[2][MAXT];   // a thread's first entry, or -1
+  __shared__ int head[2][kResidentThreads];   // a thread's first entry, or -1
   __shared__ int next[2][kEntries + 1];
   __shared__ Listed mine[2][kEntries + 1];
   __shared__ HeldRow held_set[32];
-  __shared__ double loss_sums[MAXT / 32];
+  __shared__ double loss_sums[kResidentThreads / 32];
   __shared__ int last;
   const int tid = threadIdx.x, nt = NT ? NT : blockDim.x, lane = tid & 31, warp = tid >> 5, warps = nt >> 5;
   const float kt = kLog2e / a.tau, inv_tau = 1.f / a.tau;
@@ -558,35 +561,59 @@ distill_resident_kernel(const ResidentArgs ra) {
     return ALIGNED ? 0
                    : (int)((reinterpret_cast<uintptr_t>(zb + row * a.classes) & 15) / sizeof(T));
   };
-  // Thread 0 asks for the whole chunks of a row's part: a bulk copy's unit is 16 bytes.
+  // Thread 0 asks for a row's part in whole chunks: a bulk copy's unit is 16 bytes.  A cut chunk brings
+  // its neighbours' elements along, or, where those would lie before or after the tensor, stays away.
+  auto starts_outside = [&](int64_t row, int shift) { return row * a.classes < shift; };
+  auto ends_outside = [&](int64_t row, int shift) {
+    const int over = (VEC - (classes + shift) % VEC) % VEC;
+    return (a.rows - 1 - row) * a.classes < over;
+  };
   auto fetch_row = [&](int64_t row, int buffer) {
-    const int cut = shift_of(row);
-    const int c0 = part == 0 && cut ? 1 : part * nt * NV;
-    const int c1 = min(part * nt * NV + nt * NV, (classes + cut) / VEC);
+    const int shift = shift_of(row);
+    const int c0 = part * nt * NV + (part == 0 && starts_outside(row, shift));
+    const int c1 = min(part * nt * NV + nt * NV,
+                       (classes + shift + VEC - 1) / VEC - ends_outside(row, shift));
     if (c1 > c0) {
       sm100::mbar_arrive_expect_tx(landed + buffer, (uint32_t)(c1 - c0) * 16);
       sm100::bulk_load(sm100::smem_u32(row_smem + buffer * nt * NV + c0 - part * nt * NV),
-                       zb + row * a.classes + c0 * VEC - cut, (uint32_t)(c1 - c0) * 16,
+                       zb + (row * a.classes + c0 * VEC - shift), (uint32_t)(c1 - c0) * 16,
                        landed + buffer);
     } else {
       sm100::mbar_arrive(landed + buffer);
     }
   };
+  // A cut chunk, by the thread that holds it: -inf outside the row, and what stayed away.
+  auto mend_chunk = [&](int64_t row, int buffer, int shift, int c, bool away) {
+    const int at = c - part * nt * NV;
+    if (at < 0 || at >= nt * NV || (at & (nt - 1)) != tid) return;
+    T *slot = reinterpret_cast<T *>(row_smem + buffer * nt * NV + at);
+#pragma unroll 1
+    for (int i = 0; i < VEC; ++i) {
+      const int e = c * VEC - shift + i;
+      if (e < 0 || e >= classes)
+        store_f(slot, i, -INFINITY);
+      else if (away)
+        slot[i] = zb[row * a.classes + e];
+    }
+    sm100::fence_proxy_async_smem();  // before the copy of a later row into this place
+  };
   RowChunk<T, VEC> cur[NV];
   auto load_row = [&](int64_t row, int buffer, int shift, bool whole) {
+    if (!ALIGNED && !whole) {
+      if (shift) mend_chunk(row, buffer, shift, 0, starts_outside(row, shift));
+      if ((classes + shift) % VEC)
+        mend_chunk(row, buffer, shift, (classes + shift) / VEC, ends_outside(row, shift));
+    }
     const uint4 *part_smem = row_smem + buffer * nt * NV + tid;
-    const T *z = zb + row * a.classes;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int e0 = (chunk0 + j * nt) * VEC - shift;
-      if (whole || (e0 >= 0 && e0 + VEC <= classes)) {
+      if (whole || (chunk0 + j * nt) * VEC - shift < classes) {
         const uint4 u = part_smem[j * nt];
         memcpy(&cur[j].raw, &u, 16);
       } else {
         float v[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-          v[i] = !ALIGNED && e0 + i >= 0 && e0 + i < classes ? load_f(z, e0 + i) : -INFINITY;
+        for (int i = 0; i < VEC; ++i) v[i] = -INFINITY;
         cur[j].put(v);
       }
     }
@@ -811,7 +838,7 @@ distill_resident_kernel(const ResidentArgs ra) {
           RowChunk<T, VEC> k;
           k.put(v);
           k.store(dpart + j * nt * VEC);
-        } else if (!ALIGNED) {
+        } else if (!ALIGNED && e0 < classes) {
 #pragma unroll
           for (int i = 0; i < VEC; ++i)
             if (e0 + i >= 0 && e0 + i < classes) store_f(dz, e0 + i, v[i]);
@@ -985,22 +1012,20 @@ bool resident_plan(const lnet_b200_distill_request *q, const void *dz, ResidentP
   p.aligned = zp % 16 == 0 && q->classes % VEC == 0;
   // one chunk more where a row may start inside a chunk
   const int64_t chunks = cdiv(q->classes, VEC) + (p.aligned ? 0 : 1);
-  // The smallest block that holds the row, 64 or 128 threads of 4 chunks; then 128 of 8, up to 8
-  // blocks of them; then 256 or 512 threads of 4.  (A warp a row was slower for 56 and 366 classes.)
+  // The smallest block that holds the row, 64 or 128 threads of 4 chunks; then 1 to 8 blocks of 128
+  // threads of 8.  (A warp a row was slower for 56 and 366 classes.)
   p.threads = 64, p.parts = 1, p.nv = 4;
   auto holds = [&] { return chunks <= (int64_t)p.parts * p.threads * p.nv; };
-  while (p.threads < kSmallThreads && !holds()) p.threads *= 2;
+  while (p.threads < kResidentThreads && !holds()) p.threads *= 2;
   if (!holds()) p.nv = 8;
-  while (p.parts < kResidentParts && !holds()) p.parts *= 2;
-  if (!holds()) p.nv = 4;
-  while (p.threads < kLargeThreads && !holds()) p.threads *= 2;
+  while (p.parts < kResidentParts && !holds()) ++p.parts;
   return holds();
 }
 
-template <typename T, bool TWO, bool ALIGNED, int MAXT, int NV, int NT>
+template <typename T, bool TWO, bool ALIGNED, int NV, int NT>
 int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
-  constexpr auto kernel = &distill_resident_kernel<T, TWO, ALIGNED, MAXT, NV, NT>;
-  LNET_TRY(raise_shared_memory<kernel>(2 * MAXT * NV * 16, "distill_resident_kernel"));
+  constexpr auto kernel = &distill_resident_kernel<T, TWO, ALIGNED, NV, NT>;
+  LNET_TRY(raise_shared_memory<kernel>(2 * kResidentThreads * NV * 16, "distill_resident_kernel"));
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -1014,7 +1039,7 @@ int launch_resident_typed(const ResidentPlan &p, const ResidentArgs &a, cudaStre
   cfg.dynamicSmemBytes = 2 * p.threads * NV * 16;
   // Clusters that run at once: fewer than SMs / parts, since a cluster stays inside one group of
   // SMs.  A waiting cluster would double the time of a persistent grid.
-  static std::atomic<int> known[kResidentParts + 1][kLargeThreads / 32 + 1];
+  static std::atomic<int> known[kResidentParts + 1][kResidentThreads / 32 + 1];
   std::atomic<int> &cached = known[p.parts][p.threads / 32];
   int clusters = cached.load();
   if (clusters == 0) {
@@ -1057,10 +1082,8 @@ template <typename T>
 int launch_resident(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s) {
   auto sized = [&](auto two, auto aligned) {
     constexpr bool TWO = decltype(two)::value, ALIGNED = decltype(aligned)::value;
-    if (p.threads > kSmallThreads)
-      return launch_resident_typed<T, TWO, ALIGNED, kLargeThreads, 4, 0>(p, a, s);
-    return p.nv == 4 ? launch_resident_typed<T, TWO, ALIGNED, kSmallThreads, 4, 0>(p, a, s)
-                     : launch_resident_typed<T, TWO, ALIGNED, kSmallThreads, 8, kSmallThreads>(p, a, s);
+    return p.nv == 4 ? launch_resident_typed<T, TWO, ALIGNED, 4, 0>(p, a, s)
+                     : launch_resident_typed<T, TWO, ALIGNED, 8, kResidentThreads>(p, a, s);
   };
   if (two_temperatures(a.d))
     return p.aligned ? sized(std::true_type{}, std::true_type{})

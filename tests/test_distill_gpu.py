@@ -10,12 +10,13 @@ the value (8 significant bits).
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
-from lnet_b200 import distillation_loss
+from lnet_b200 import _lib, distillation_loss
 
 pytestmark = pytest.mark.gpu
 
@@ -105,6 +106,49 @@ def check(z, index, teacher, labels, tau, alpha, reduction, dtype):
 def test_loss_and_gradient(rows, classes, top, dtype, reduction, cuda_device):
     z, index, teacher, labels = make(rows, classes, top, dtype, rows + classes, cuda_device)
     check(z, index, teacher, labels, 2.0, 0.6, reduction, dtype)
+
+
+# rows that 2 to 8 blocks share (8192 bf16 or 4096 fp32 classes each), whole and with a block of little
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("classes", [8191, 8193, 12001, 16385, 20001, 24576, 28673, 32767, 40003,
+                                     50257, 57344, 65535])
+def test_rows_of_several_blocks(classes, dtype, cuda_device):
+    z, index, teacher, labels = make(5, classes, 24, dtype, classes, cuda_device)
+    check(z, index, teacher, labels, 2.0, 0.6, "mean", dtype)
+    check(z, index, teacher, labels, 1.0, 0.6, "sum", dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,classes,top", [(1, 1, 1), (3, 3, 2), (1, 7, 3), (5, 9, 4), (4, 1003, 5),
+                                              (3, 8190, 6), (2, 20005, 30)])
+@pytest.mark.parametrize("ahead", [1, 3])
+def test_logits_and_gradient_off_a_boundary(rows, classes, top, ahead, dtype, cuda_device):
+    """The C ABI on a view that starts and ends inside 16 bytes: what lies around it stays out of the
+    loss (it is NaN) and of the gradient's stores."""
+    z, index, teacher, labels = make(rows, classes, top, dtype, classes + ahead, cuda_device)
+    n = rows * classes
+    flat = torch.full((n + 32,), math.nan, dtype=dtype, device=cuda_device)
+    flat[ahead:ahead + n] = z.reshape(-1)
+    grad = torch.full((n + 32,), 77.0, dtype=dtype, device=cuda_device)
+    size = flat.element_size()
+    q = _lib.DistillRequest(rows, classes, top, 1 if dtype == torch.bfloat16 else 0, 1,
+                            flat.data_ptr() + ahead * size, index.data_ptr(), teacher.data_ptr(),
+                            labels.data_ptr(), 2.0, 0.6)
+    lib, need = _lib.load(), ctypes.c_size_t()
+    _lib.check(lib.lnet_b200_distill_workspace_size(ctypes.byref(q), ctypes.byref(need)), "size")
+    work = torch.empty(need.value, dtype=torch.uint8, device=cuda_device)
+    loss = torch.empty((), device=cuda_device)
+    _lib.check(lib.lnet_b200_distill_forward(
+        ctypes.byref(q), work.data_ptr(), need.value, loss.data_ptr(),
+        grad.data_ptr() + ahead * size, torch.cuda.current_stream().cuda_stream), "forward")
+    assert bool((grad[:ahead] == 77).all()) and bool((grad[ahead + n:] == 77).all())
+    zg = z.clone().requires_grad_()
+    want = distillation_loss(zg, index, teacher, labels=labels, temperature=2.0, alpha=0.6,
+                             reduction="sum")
+    dz, = torch.autograd.grad(want, zg)
+    assert float((loss - want.detach()).abs()) <= 2 * FP32 * 4.0 * (rows + float(want.detach().abs()))
+    tol = 2 * HALF_ULP[dtype] * 1.01 * dz.double().abs() + 2 * FP32 * 2.2
+    assert bool(((grad[ahead:ahead + n].double().view_as(dz) - dz.double()).abs() <= tol).all())
 
 
 @pytest.mark.parametrize("tau,alpha,labelled", [(1.0, 1.0, False), (1.0, 0.5, True),
