@@ -9,13 +9,14 @@ e4m3 code half a step, 2^-4 of the value or 2^-10 of the scale below the normals
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import pytest
 import torch
 
 import lnet_b200
-from lnet_b200 import residual_rms_norm, residual_rms_norm_fp8
+from lnet_b200 import _lib, residual_rms_norm, residual_rms_norm_fp8
 
 pytestmark = pytest.mark.gpu
 
@@ -26,7 +27,8 @@ DTYPES = [torch.float32, torch.bfloat16]
 # many rows of odd and even widths
 SHAPES = [(1, 1), (1, 96), (7, 64), (300, 96), (5, 3, 128), (33, 257), (19, 1001), (64, 1024),
           (9, 4096), (3, 8200), (2, 8193), (2, 16392), (2, 20001), (1300, 2048), (1201, 4096),
-          (1211, 1544), (3001, 97), (2500, 1001), (700, 2049), (20011, 33)]
+          (1211, 1544), (3001, 97), (2500, 1001), (700, 2049), (20011, 33),
+          (300, 6795), (2100, 5001), (40, 12003)]
 
 
 def make(shape, dtype, seed, device, std=1.0):
@@ -90,6 +92,69 @@ def test_gradient(shape, dtype, weight_dtype, cuda_device):
                                      + lnet_b200.norm.RMS_NORM_EPS)
     mags = (dy.double() * xhat).abs().reshape(-1, shape[-1]).sum(0)
     close(dw, gw, weight_dtype, mags)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1, 33), (3, 17), (5, 97), (9, 1003), (2, 4100)])
+@pytest.mark.parametrize("ahead", [1, 3])
+def test_views_off_a_boundary(shape, ahead, dtype, cuda_device):
+    """The C ABI on views that start and end inside 16 bytes: what lies around them (NaN) stays out of
+    the sums, and the stores inside them."""
+    rows, dim = shape
+    n, lib = rows * dim, _lib.load()
+    kind = 1 if dtype == torch.bfloat16 else 0
+    code = torch.cuda.current_stream().cuda_stream
+
+    def view(t=None):
+        flat = torch.full((n + 32,), math.nan if t is not None else 77.0, dtype=dtype,
+                          device=cuda_device)
+        if t is not None:
+            flat[ahead:ahead + n] = t.reshape(-1)
+        return flat, flat[ahead:ahead + n].view(shape)
+
+    def alone(flat):
+        return bool((flat[:ahead] == 77).all()) and bool((flat[ahead + n:] == 77).all())
+
+    x, r, dy, dh = (make(shape, dtype, i, cuda_device) for i in range(1, 5))
+    w = 1 + make(shape[-1:], torch.float32, 5, cuda_device, 0.2)
+    (_, xv), (_, rv), (_, dyv), (_, dhv) = (view(t) for t in (x, r, dy, dh))
+    (yf, y), (hf, h), (dxf, dx) = (view() for _ in range(3))
+    rstd = torch.empty(rows, device=cuda_device)
+    eps = lnet_b200.norm.RMS_NORM_EPS
+    _lib.check(lib.lnet_b200_residual_rms_norm(
+        xv.data_ptr(), rv.data_ptr(), w.data_ptr(), kind, 0, rows, dim, eps, y.data_ptr(),
+        h.data_ptr(), rstd.data_ptr(), code), "forward")
+    assert alone(yf) and alone(hf) and torch.equal(h, stream_of(x, r))
+    ref = norm64(h, w, eps)
+    close(y, ref, dtype, ref.abs())
+    need = ctypes.c_size_t()
+    _lib.check(lib.lnet_b200_residual_rms_norm_workspace_size(kind, rows, dim, ctypes.byref(need)),
+               "size")
+    work, dw = torch.empty(need.value, dtype=torch.uint8, device=cuda_device), torch.empty_like(w)
+    # the stream of the view above (its neighbours are 77: finite, and wrong where they count)
+    _lib.check(lib.lnet_b200_residual_rms_norm_backward(
+        h.data_ptr(), rstd.data_ptr(), w.data_ptr(), dyv.data_ptr(), dhv.data_ptr(), kind, 0, rows,
+        dim, dx.data_ptr(), dw.data_ptr(), work.data_ptr(), need.value, code), "backward")
+    assert alone(dxf)
+    h64, w64 = h.double().requires_grad_(), w.double().requires_grad_()
+    gh, gw = torch.autograd.grad(norm64(h64, w64, eps), [h64, w64], dy.double())
+    close(dx, gh + dh.double(), dtype, gh.abs().amax(-1, keepdim=True) + dh.double().abs())
+    xhat = h.double() / torch.sqrt((h.double() ** 2).mean(-1, keepdim=True) + eps)
+    close(dw, gw, torch.float32, (dy.double() * xhat).abs().sum(0))
+    codes = torch.full((n + 32,), 77, dtype=torch.uint8, device=cuda_device)
+    scales = torch.empty(rows, device=cuda_device)
+    want = residual_rms_norm_fp8(x, w, r)
+    for at in (ahead, 0):  # the codes' alignment may differ from the rows'
+        codes.fill_(77)
+        _lib.check(lib.lnet_b200_residual_rms_norm_fp8(
+            xv.data_ptr(), rv.data_ptr(), w.data_ptr(), kind, 0, rows, dim, eps,
+            codes.data_ptr() + at, scales.data_ptr(), h.data_ptr(), code), "fp8")
+        assert alone(hf) and bool((codes[:at] == 77).all()) and bool((codes[at + n:] == 77).all())
+        got = codes[at:at + n].view(torch.float8_e4m3fn).view(shape)
+        assert torch.allclose(scales, want[1], rtol=1e-5, atol=0)
+        # sums of squares taken in another order: a code may round to its neighbour
+        near = (got.float() - want[0].float()).abs() <= 2 ** -3 * want[0].float().abs() + 2 ** -9
+        assert bool(near.all())
 
 
 def test_gradient_against_differences(cuda_device):
