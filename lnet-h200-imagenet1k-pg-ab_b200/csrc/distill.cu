@@ -488,7 +488,7 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 // HBM rate; the sweep-twice kernel took 637 us.  Rows of up to 128 x 4 chunks take 4 chunks a thread
 // and one block; more take as many blocks of 128 x 8 as hold them, any number up to 8 (2000 x 40000: 5
 // blocks 100 us, 8 blocks 158, the other kernel 137).  Rows that 8 do not hold are the other kernel's:
-// 2000 x 131000 took 341 us there and 485 here with 512 threads of 4 chunks.
+// 2000 x 131000 take 344 us there and took 485 here with 512 threads of 4 chunks.
 // Rows that start inside 16 bytes: 2000 x 50257 172 us (the other kernel 166, and 24 more for the count
 // and the sum against 16 for the teacher's side), 2000 x 40001 122 (144).
 constexpr int kResidentThreads = 128;
@@ -1094,9 +1094,13 @@ int launch_resident(const ResidentPlan &p, const ResidentArgs &a, cudaStream_t s
 
 template <typename T>
 int launch_rows(const lnet_b200_distill_request *q, const DistillArgs &a, cudaStream_t s) {
-  // Threads: 4 chunks of 16 bytes each, 64 to 512.
+  // Threads: 4 chunks of 16 bytes each, 64 or more; at most 512 for a row an SM, 256 from there on, 128
+  // from 4 rows an SM on, where blocks of other rows fill the waits.  512, 256, 128 and 64 at most, loss
+  // alone, fp32: 6263 x 12029 227, 95, 70, 86 us; 2000 x 32768 92, 60, 53, 63; 300 x 100003 47, 33, 47,
+  // 77; bf16: 6263 x 12029 116, 82, 64, 79; 600 x 32768 25, 23, 23, 27; 300 x 100003 35, 34, 37, 49.
   const int64_t chunks = cdiv(q->classes, vec_of<T>());
-  const int threads = (int)std::min<int64_t>(512, std::max<int64_t>(64, cdiv(chunks, 4 * 32) * 32));
+  const int most = q->rows >= 4 * sm_count() ? 128 : q->rows >= sm_count() ? 256 : 512;
+  const int threads = (int)std::min<int64_t>(most, std::max<int64_t>(64, cdiv(chunks, 4 * 32) * 32));
   // A cluster where rows alone leave SMs idle and each block keeps 4 chunks a thread (bf16 classes,
   // 4 chunks against 2: 1 x 4096 3.9 us against 4.8, 36 x 100003 10.7 against 13.7,
   // 74 x 32768 6.9 against 10.9; 5 x 100003, the other way, 7.9 against 7.2).
