@@ -485,12 +485,13 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 // elements a thread (168 registers) and clusters of 4; 317 with four of 32 elements and clusters of
 // 8; 315 with six of 64 threads; 341 with one of 256.  What bounds it is the time that a cluster's
 // blocks wait for the slowest of them (0.4 instructions a clock and scheduler), at 0.57 of the measured
-// HBM rate; the sweep-twice kernel took 637 us.  Rows of up to 128 x 4 chunks take 4 chunks a thread
+// HBM rate; the sweep-twice kernel takes 318 us.  Rows of up to 128 x 4 chunks take 4 chunks a thread
 // and one block; more take as many blocks of 128 x 8 as hold them, any number up to 8 (2000 x 40000: 5
-// blocks 100 us, 8 blocks 158, the other kernel 137).  Rows that 8 do not hold are the other kernel's:
+// blocks 101 us, 8 blocks 158, the other kernel 121).  Rows that 8 do not hold are the other kernel's:
 // 2000 x 131000 take 344 us there and took 485 here with 512 threads of 4 chunks.
-// Rows that start inside 16 bytes: 2000 x 50257 172 us (the other kernel 166, and 24 more for the count
-// and the sum against 16 for the teacher's side), 2000 x 40001 122 (144).
+// Rows that start inside 16 bytes, with the launches around the kernel: 2000 x 40001 137 us (the other
+// kernel 148), 2000 x 4097 53 (61), 2000 x 1001 43 (53); 5 to 9 % slower where the last block has
+// little to hold (2000 x 32767 136 against 126, 2000 x 50257 186 against 170).
 constexpr int kResidentThreads = 128;
 constexpr int kResidentParts = 8;
 
