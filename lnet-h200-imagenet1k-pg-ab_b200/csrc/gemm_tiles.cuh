@@ -170,7 +170,6 @@ struct TileArgs {
   // fp32 sums go to `partial` [tile - full][split][CTA][BN / 4][128 rows][4].
   int m_tiles, n_tiles, full, splits, kblocks;
   float *partial;
-  int vec;  // N is a multiple of 8 and every [M, N] tensor 16-byte aligned
 };
 
 template <int CTAS, int BN, bool FP8>
@@ -192,7 +191,7 @@ struct TileShape {
 // A warp holds a 32 x 32 block of a, a lane a row.  Rows of a block lie N elements apart, so a lane
 // that moved its own row would touch 32 lines an instruction; the block goes through shared memory
 // (64-byte rows, 16-byte units exchanged so that neither side has bank conflicts) and moves as 4
-// lanes a row, or, where rows are not 16-byte aligned, as a row an instruction.
+// lanes a row, or, where rows are not 16-byte aligned, as 8, 16 or 32 lanes a row.
 __device__ __forceinline__ uint4 *block_unit(uint8_t *block, int row, int unit) {
   return reinterpret_cast<uint4 *>(block + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
 }
@@ -212,8 +211,46 @@ __device__ __forceinline__ BlockRows block_rows(int64_t row0, int64_t M, int64_t
   for (int i = 0; i < 4; ++i) b.ok |= (row0 + (lane >> 2) + 8 * i < M ? 1u : 0u) << i;
   return b;
 }
+// The block to or from memory, U (4, 2 or 1) elements a lane, U rows an instruction.
+template <int U>
+using UnitWord = std::conditional_t<U == 4, uint2, std::conditional_t<U == 2, uint32_t, uint16_t>>;
+template <int U>
+__device__ __forceinline__ void block_out(uint8_t *block, __nv_bfloat16 *dst, const BlockRows &b,
+                                          int64_t col) {
+  using W = UnitWord<U>;
+  const int lane = threadIdx.x & 31, r0 = lane / (32 / U), c = lane % (32 / U) * U;
+  if (col + c >= b.N) return;
+  const int rows = (int)min((int64_t)32, b.M - b.row0);
+  __nv_bfloat16 *p = dst + (b.row0 + r0) * b.N + col + c;
+#pragma unroll 8
+  for (int r = r0; r < rows; r += U, p += U * b.N)
+    *reinterpret_cast<W *>(p) = *reinterpret_cast<const W *>(block_element(block, r, c));
+}
+template <int U>
+__device__ __forceinline__ void block_in(uint8_t *block, const __nv_bfloat16 *src, const BlockRows &b,
+                                         int64_t col) {
+  using W = UnitWord<U>;
+  constexpr int Q = U == 1 ? 16 : 32 / U;  // loads on their way at once
+  const int lane = threadIdx.x & 31, r0 = lane / (32 / U), c = lane % (32 / U) * U;
+  if (col + c >= b.N) return;
+  const int rows = (int)min((int64_t)32, b.M - b.row0);
+  const __nv_bfloat16 *p = src + (b.row0 + r0) * b.N + col + c;
+#pragma unroll
+  for (int s = 0; s < 32; s += Q * U) {
+    W q[Q];
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      q[i] = r0 + s + i * U < rows
+                 ? __ldg(reinterpret_cast<const W *>(p + (int64_t)(s + i * U) * b.N))
+                 : W{};
+#pragma unroll
+    for (int i = 0; i < Q; ++i)
+      *reinterpret_cast<W *>(block_element(block, r0 + s + i * U, c)) = q[i];
+  }
+}
+template <int UNIT>
 __device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv_bfloat16 *dst,
-                                            const BlockRows &b, int64_t col, bool vec) {
+                                            const BlockRows &b, int64_t col) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -222,7 +259,7 @@ __device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv
     *block_unit(block, lane, u) = c.raw;
   }
   __syncwarp();
-  if (vec) {
+  if constexpr (UNIT == 8) {
     __nv_bfloat16 *p = dst + b.at + col;
     const bool in = col + (lane & 3) * 8 < b.N;
 #pragma unroll
@@ -231,11 +268,8 @@ __device__ __forceinline__ void block_store(uint8_t *block, const float *v, __nv
         *reinterpret_cast<uint4 *>(p) = *block_unit(block, i * 8 + (lane >> 2), lane & 3);
       p += 8 * b.N;
     }
-  } else if (col + lane < b.N) {
-    __nv_bfloat16 *p = dst + b.row0 * b.N + col + lane;
-    const int rows = (int)min((int64_t)32, b.M - b.row0);
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r, p += b.N) *p = *block_element(block, r, lane);
+  } else {
+    block_out<UNIT>(block, dst, b, col);
   }
   __syncwarp();
 }
@@ -251,28 +285,16 @@ __device__ __forceinline__ void block_fetch(const __nv_bfloat16 *src, uint4 *u, 
     p += 8 * b.N;
   }
 }
-// v += the block of `src`, whose units are in `u` where `vec`.
+// v += the block of `src`, whose units are in `u` where UNIT is 8.
+template <int UNIT>
 __device__ __forceinline__ void block_add(uint8_t *block, const __nv_bfloat16 *src, const uint4 *u,
-                                          float *v, const BlockRows &b, int64_t col, bool vec) {
+                                          float *v, const BlockRows &b, int64_t col) {
   const int lane = threadIdx.x & 31;
-  if (vec) {
+  if constexpr (UNIT == 8) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) *block_unit(block, i * 8 + (lane >> 2), lane & 3) = u[i];
-  } else if (col + lane < b.N) {
-    const __nv_bfloat16 *p = src + b.row0 * b.N + col + lane;
-    const int rows = (int)min((int64_t)32, b.M - b.row0);
-#pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += 16) {  // 16 rows on their way at once
-      uint16_t q[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        q[r] = r0 + r < rows
-                   ? __ldg(reinterpret_cast<const uint16_t *>(p + (int64_t)(r0 + r) * b.N))
-                   : (uint16_t)0;
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        *reinterpret_cast<uint16_t *>(block_element(block, r0 + r, lane)) = q[r];
-    }
+  } else {
+    block_in<UNIT>(block, src, b, col);
   }
   __syncwarp();
 #pragma unroll
@@ -291,7 +313,8 @@ __device__ __forceinline__ void block_add(uint8_t *block, const __nv_bfloat16 *s
 
 // The block's 32 columns of bias and scale come from shared memory (`bias`, `scale`; scale only
 // with row scales); `res` holds the residual's units.  Every lane of the warp takes part.
-__device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, const BlockRows &b, bool vec,
+template <int UNIT>
+__device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, const BlockRows &b,
                                               float *v, int64_t col, float row_scale,
                                               const float *bias, const float *scale,
                                               uint8_t *block, const uint4 *res) {
@@ -312,10 +335,10 @@ __device__ __forceinline__ void tile_epilogue(const TileEpilogue &e, const Block
       unpair(pair(v[j + 2], v[j + 3]) + pair(q.z, q.w), v[j + 2], v[j + 3]);
     }
   }
-  if (e.pre) block_store(block, v, e.pre, b, col, vec);
+  if (e.pre) block_store<UNIT>(block, v, e.pre, b, col);
   act_values<32>(v, e.act);
-  if (e.residual) block_add(block, e.residual, res, v, b, col, vec);
-  block_store(block, v, e.out, b, col, vec);
+  if (e.residual) block_add<UNIT>(block, e.residual, res, v, b, col);
+  block_store<UNIT>(block, v, e.out, b, col);
 }
 
 // Bias and scale of `n` columns from `col` on into a warp's shared memory (0 past N).
@@ -349,7 +372,10 @@ __device__ __forceinline__ void tile_at(const TileArgs &p, int t, int &m, int &n
   m = band * kBand + t - n * (last ? (int)p.by_last.d : kBand);
 }
 
-template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
+// UNIT: elements that [M, N] tensors are moved by (8, 4, 2 or 1), of which N is a multiple and to which
+// they are aligned.  In one kernel the paths of the four slowed one another: 6329 x 2010 -> 4557 with
+// residual and pre-activation took 203 us, and takes 155 (4558 columns 118, 4556 111, 4560 103).
+template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8, int UNIT>
 __global__ void __launch_bounds__(kTileThreads, 1)
 tile_gemm_kernel(const __grid_constant__ TileArgs p) {
   using S = TileShape<CTAS, BN, FP8>;
@@ -528,7 +554,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
 #pragma unroll 1
       for (int c = 0; in && c < COLS && col0 + c < p.N; c += 32) {
         uint4 ru[4];
-        if (w.split < 0 && p.e.residual && p.vec) block_fetch(p.e.residual, ru, rows, col0 + c);
+        if (w.split < 0 && UNIT == 8 && p.e.residual) block_fetch(p.e.residual, ru, rows, col0 + c);
         float v[32];
         if (ok) {
           sm100::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + acc * BN + group * COLS + c, v);
@@ -539,7 +565,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
         }
         if (c + 32 >= COLS || col0 + c + 32 >= p.N) release();
         if (w.split < 0) {
-          tile_epilogue(p.e, rows, p.vec, v, col0 + c, rs, bias + c, scale + c, block, ru);
+          tile_epilogue<UNIT>(p.e, rows, v, col0 + c, rs, bias + c, scale + c, block, ru);
         } else {
           float4 *out = reinterpret_cast<float4 *>(p.partial) +
                         (((int64_t)(w.tile - p.full) * p.splits + w.split) * CTAS + rank) *
@@ -570,7 +596,7 @@ tile_gemm_kernel(const __grid_constant__ TileArgs p) {
 // The tiles whose k was split: their sums, added in split order, through the epilogue.  A warp takes
 // a 32 x 32 block.
 constexpr int kJoinThreads = 128;
-template <int CTAS, int BN>
+template <int CTAS, int BN, int UNIT>
 __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_constant__ TileArgs p) {
   constexpr int BLOCKS = CTAS * 4 * (BN / 32);  // of a tile
   __shared__ __align__(16) uint8_t smem[kJoinThreads / 32][2048 + 2 * 32 * 4];
@@ -590,7 +616,7 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_co
   __syncwarp();
   uint4 ru[4];
   const BlockRows rows = block_rows(row0, p.M, p.N);
-  if (p.e.residual && p.vec) block_fetch(p.e.residual, ru, rows, col);
+  if (UNIT == 8 && p.e.residual) block_fetch(p.e.residual, ru, rows, col);
   const float rs = p.e.row_scale && row0 + lane < p.M ? __ldg(p.e.row_scale + row0 + lane) : 1.f;
   float v[32];
 #pragma unroll
@@ -606,7 +632,7 @@ __global__ void __launch_bounds__(kJoinThreads) tile_join_kernel(const __grid_co
       v[4 * j] += u.x, v[4 * j + 1] += u.y, v[4 * j + 2] += u.z, v[4 * j + 3] += u.w;
     }
   }
-  tile_epilogue(p.e, rows, p.vec, v, col, rs, bias, scale, block, ru);
+  tile_epilogue<UNIT>(p.e, rows, v, col, rs, bias, scale, block, ru);
 }
 
 // ---------------------------------------------------------------- host side

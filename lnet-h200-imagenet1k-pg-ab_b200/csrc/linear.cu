@@ -349,11 +349,11 @@ ProductPlan product_plan(int64_t M, int64_t N, int kblocks) {
   return best;
 }
 
-template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
-int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
-                 cudaStream_t stream) {
+template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8, int UNIT>
+int launch_unit(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
+                cudaStream_t stream) {
   using S = TileShape<CTAS, BN, FP8>;
-  constexpr auto kernel = &tile_gemm_kernel<CTAS, BN, A_MN, B_MN, FP8>;
+  constexpr auto kernel = &tile_gemm_kernel<CTAS, BN, A_MN, B_MN, FP8, UNIT>;
   LNET_TRY(raise_shared_memory<kernel>(S::SMEM, "tile_gemm_kernel shared memory"));
   LNET_TRY(tile_tensor_map(&args.a, a, FP8, kTileM));
   LNET_TRY(tile_tensor_map(&args.b, b, FP8, S::NB));
@@ -372,9 +372,25 @@ int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &
   LNET_TRY(after_launch("tile_gemm_kernel"));
   if (q.splits == 1) return LNET_OK;
   const int blocks = (q.m_tiles * q.n_tiles - q.full) * CTAS * 4 * (BN / 32);
-  tile_join_kernel<CTAS, BN><<<(unsigned)cdiv(blocks, kJoinThreads / 32), kJoinThreads, 0, stream>>>(
+  tile_join_kernel<CTAS, BN, UNIT><<<(unsigned)cdiv(blocks, kJoinThreads / 32), kJoinThreads, 0, stream>>>(
       args);
   return after_launch("tile_join_kernel");
+}
+
+template <int CTAS, int BN, bool A_MN, bool B_MN, bool FP8>
+int launch_tiles(const ProductPlan &q, const TileOperand &a, const TileOperand &b, TileArgs &args,
+                 cudaStream_t s) {
+  const uintptr_t where = reinterpret_cast<uintptr_t>(args.e.out) |
+                          reinterpret_cast<uintptr_t>(args.e.pre) |
+                          reinterpret_cast<uintptr_t>(args.e.residual);
+  int unit = 8;
+  while (unit > 1 && (args.N % unit || where % (2 * unit))) unit /= 2;
+  switch (unit) {
+    case 8: return launch_unit<CTAS, BN, A_MN, B_MN, FP8, 8>(q, a, b, args, s);
+    case 4: return launch_unit<CTAS, BN, A_MN, B_MN, FP8, 4>(q, a, b, args, s);
+    case 2: return launch_unit<CTAS, BN, A_MN, B_MN, FP8, 2>(q, a, b, args, s);
+    default: return launch_unit<CTAS, BN, A_MN, B_MN, FP8, 1>(q, a, b, args, s);
+  }
 }
 
 template <bool A_MN, bool B_MN, bool FP8>
@@ -404,7 +420,6 @@ int product(const TileOperand &a, const TileOperand &b, const TileEpilogue &e, f
   args.by_band = FastDiv(kBand * q.n_tiles);
   args.by_last = FastDiv(q.m_tiles % kBand ? q.m_tiles % kBand : kBand);
   args.by_splits = FastDiv(q.splits);
-  args.vec = N % 8 == 0 && aligned16(e.out) && aligned16(e.pre) && aligned16(e.residual);
   return launch_kind<A_MN, B_MN, FP8>(q, a, b, args, s);
 }
 

@@ -32,7 +32,8 @@ ACTS = ["none", "relu", "silu", "gelu"]
 SHAPES = [(1, 1, 1), (1, 1024, 4096), (2, 96, 384), (3, 1001, 77), (8, 130, 50), (9, 64, 64),
           (127, 96, 129), (128, 128, 128), (129, 72, 257), (300, 1001, 1000), (257, 4096, 96),
           (1000, 40, 1000), (64, 8192, 128), (2048, 512, 2048), (4100, 264, 2056),
-          (50, 1, 3), (30, 3, 1), (4, 1003, 9)]
+          (50, 1, 3), (30, 3, 1), (4, 1003, 9), (300, 72, 1004), (270, 200, 514), (130, 8192, 130),
+          (260, 4100, 140)]
 
 
 def acc(k):
