@@ -199,14 +199,18 @@ pack_kernel(const uint8_t *__restrict__ src, int64_t rows, int64_t cols, int64_t
 // da = dy f'(pre) in bf16 (pitch `pitch`, its padding zero; null: not wanted), and the blocks'
 // column sums of the unrounded da (null: not wanted).  A thread holds VEC columns of every
 // kSlopeLanes-th row of its block's rows.  16384 x 8192, GELU: 171 us for 805 MB (0.73 of a copy's
-// rate), bound by the exponential and the polynomial (1.7 instructions a clock) next to HBM.
+// rate), bound by the exponential and the polynomial (1.7 instructions a clock) next to HBM.  Rows off
+// 16-byte boundaries take pairs of columns where they are even, else one: 6329 x 4558, ReLU, 40 us,
+// 4557 columns 74, 4560 31.
 template <int VEC, int ACT>
 __global__ void __launch_bounds__(32 * kSlopeLanes, kSlopeBlocks)
 slope_kernel(const __nv_bfloat16 *__restrict__ dy, const __nv_bfloat16 *__restrict__ pre, int64_t M,
              int64_t N, __nv_bfloat16 *__restrict__ da, int64_t pitch,
              float *__restrict__ partial) {
   __shared__ float sums[kSlopeLanes][32 * VEC];
-  constexpr int R = 2;  // rows in flight; four held registers that a fourth block needs
+  // rows in flight; four of 8 columns held registers that a fourth block needs, and eight of one or
+  // two columns took twice as long
+  constexpr int R = 2;
   const int64_t col = ((int64_t)blockIdx.x * 32 + threadIdx.x) * VEC;
   float s[VEC];
 #pragma unroll
@@ -504,7 +508,8 @@ int slope_row_blocks(int64_t M, int64_t N, int vec) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, cdiv(M, kSlopeLanes * 2)));
 }
 int slope_vec(const lnet_b200_linear_request *q, const void *pre, const void *dy) {
-  return q->outer % 8 == 0 && aligned16(pre) && aligned16(dy) ? 8 : 1;
+  const uintptr_t where = reinterpret_cast<uintptr_t>(pre) | reinterpret_cast<uintptr_t>(dy);
+  return q->outer % 8 == 0 && where % 16 == 0 ? 8 : q->outer % 2 == 0 && where % 4 == 0 ? 2 : 1;
 }
 
 // Workspace of the gradient.
@@ -689,6 +694,8 @@ extern "C" int lnet_b200_linear_backward(const lnet_b200_linear_request *req, co
     const dim3 block(32, kSlopeLanes);
     if (vec == 8)
       launch_slope<8>(grid, block, req->activation, dyp, pre, M, N, w.da, pitch, w.columns, stream);
+    else if (vec == 2)
+      launch_slope<2>(grid, block, req->activation, dyp, pre, M, N, w.da, pitch, w.columns, stream);
     else
       launch_slope<1>(grid, block, req->activation, dyp, pre, M, N, w.da, pitch, w.columns, stream);
     LNET_TRY(after_launch("linear_slope_kernel"));

@@ -44,6 +44,25 @@ struct RowChunk<__nv_bfloat16, 1> {
     raw = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
   }
 };
+template <>  // (a pair, for bf16 rows that start on 4-byte boundaries only)
+struct RowChunk<__nv_bfloat16, 2> {
+  uint32_t raw;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+    raw = __ldg(reinterpret_cast<const uint32_t *>(p));
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16 *p) const {
+    *reinterpret_cast<uint32_t *>(p) = raw;
+  }
+  __device__ __forceinline__ void zero() { raw = 0; }
+  __device__ __forceinline__ void get(float *v) const {
+    v[0] = __uint_as_float(raw << 16);
+    v[1] = __uint_as_float(raw & 0xFFFF0000u);
+  }
+  __device__ __forceinline__ void put(const float *v) {
+    const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
+    raw = *reinterpret_cast<const uint32_t *>(&b);
+  }
+};
 template <>
 struct RowChunk<float, 4> {
   float4 raw;
