@@ -17,9 +17,9 @@
 // A last wave that would leave SMs idle is split along k: those tiles' fp32 sums
 // go to memory and a second kernel joins them.
 //
-// Bound by the tensor cores: 16384 x 2048 -> 8192 bf16 takes 363 us (1510 of 1661
-// TFLOP/s measured; tensor pipe 0.90 active), 377 with GELU and the stored
-// pre-activation.  The epilogue takes 2.9 us a 256 x 256 tile (5.9 with GELU and
+// Bound by the tensor cores: 16384 x 2048 -> 8192 bf16 with GELU and the stored
+// pre-activation, and the gradient's two products, take 345 us each (1590 of 1661
+// TFLOP/s measured; tensor pipe 0.90 active without GELU).  The epilogue takes 2.9 us a 256 x 256 tile (5.9 with GELU and
 // pre-activation) behind the next tile's MMAs, and bounds the kernel where K is
 // below about 768 (1536).
 //
