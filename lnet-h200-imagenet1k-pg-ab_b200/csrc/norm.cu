@@ -131,14 +131,26 @@ __device__ __forceinline__ void store_e4m3(uint8_t *row, const Lanes<VEC> *l, fl
     }
   }
 }
-// Scale of a row whose y is f t, and the factor k that takes t to its codes: with m = max|t|,
-// s = f m / 448 and y / s = t (448 / m), two fp32 roundings from the quotient, 2^-20 of a code's
-// step.  A zero row has s = 0 and codes 0; a scale that is not finite takes its row along.
-__device__ __forceinline__ float e4m3_scale(float m, float f, float &k) {
-  const float s = f * m / kE4m3Max;
-  k = s == 0.f ? 0.f : kE4m3Max / m;
-  if (!(s < INFINITY)) k = s == s ? 0.f : s;
-  return s;
+// A row's scale s = m / 448, m = max|y|, and how its codes e4m3(y / s) are taken: y (448 / m), two fp32
+// roundings from the quotient, 2^-20 of a code's step.  Where s is below the normal numbers 448 / m
+// overflows and is no inverse of the s that is stored; there y is lifted by 2^64 first, exactly, and
+// multiplied by the inverse of the lifted s.  A zero row (or one so small that s is 0) has codes 0; a
+// scale that is not finite takes its row along.
+struct E4m3Scale {
+  float s, k;
+  bool low;
+};
+constexpr float kLift = 18446744073709551616.f;  // 2^64
+__device__ __forceinline__ E4m3Scale e4m3_scale(float m) {
+  E4m3Scale c{m / kE4m3Max, kE4m3Max / m, false};
+  if (c.s < 1.17549435e-38f) c.k = c.s == 0.f ? 0.f : 1.f / (c.s * kLift), c.low = true;
+  if (c.s == INFINITY) c.k = 0.f;
+  return c;
+}
+template <int VEC>
+__device__ __forceinline__ void e4m3_lift(Lanes<VEC> *l, float lift = kLift) {
+#pragma unroll
+  for (int i = 0; i < lanes_of<VEC>(); ++i) l[i] = l[i] * splat<VEC>(lift);
 }
 // Largest magnitude of a chunk so far.
 template <int VEC>
@@ -305,26 +317,31 @@ norm_forward_kernel(const NormArgs a) {
     const float ss = group_reduce<G, SumOp>(lane_sum(sum), scratch);
     const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
     if (a.rstd && live && lane == 0) a.rstd[row] = rstd;
-    if (FP8) {  // y = rstd t, t = h w
-      L t[NV][NP];
+    if (FP8) {
+      L t[NV][NP];  // y
+      const L f = splat<VEC>(rstd);
       float m = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (lane + j * g >= nvec) continue;
         get_lanes(cx[j], t[j]);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) t[j][i] = t[j][i] * w[j][i];
+        for (int i = 0; i < NP; ++i) t[j][i] = t[j][i] * f * w[j][i];
         m = chunk_magnitude<VEC>(m, t[j]);
       }
       m = group_reduce<G, MaxMagnitudeOp>(m, scratch);
-      float k;
-      const float scale = e4m3_scale(m, rstd, k);
-      if (live && lane == 0) a.scales[row] = scale;
+      const E4m3Scale scale = e4m3_scale(m);
+      if (live && lane == 0) a.scales[row] = scale.s;
+      if (scale.low) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+          if (lane + j * g < nvec) e4m3_lift<VEC>(t[j]);
+      }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         const int c = lane + j * g;
         if (live && c < nvec)
-          store_e4m3<VEC, SHIFT>(a.q + off, t[j], k, c * VEC - shift, dim);
+          store_e4m3<VEC, SHIFT>(a.q + off, t[j], scale.k, c * VEC - shift, dim);
       }
     } else {
       const L f = splat<VEC>(rstd);
@@ -366,29 +383,31 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
     ss = group_reduce<0, SumOp>(ss, scratch);
     const float rstd = 1.f / sqrtf(ss / (float)a.dim + a.eps);
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
-    float k = 0.f;
+    E4m3Scale scale{};
     if (FP8) {
       float m = 0.f;
       for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x)
-        m = MaxMagnitudeOp::of(m, fabsf(load_f(h, off + c) * weight_at(a.w, a.w_bf16, c)));
+        m = MaxMagnitudeOp::of(m, fabsf(load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c)));
       m = group_reduce<0, MaxMagnitudeOp>(m, scratch);
-      const float scale = e4m3_scale(m, rstd, k);
-      if (threadIdx.x == 0) a.scales[row] = scale;
+      scale = e4m3_scale(m);
+      if (threadIdx.x == 0) a.scales[row] = scale.s;
     }
     for (int64_t c = threadIdx.x; c < a.dim; c += blockDim.x) {
-      const float v = load_f(h, off + c), w = weight_at(a.w, a.w_bf16, c);
+      const float y = load_f(h, off + c) * rstd * weight_at(a.w, a.w_bf16, c);
       if (FP8) {
-        const Single t{v * w};
-        store_e4m3<1>(a.q + off, &t, k, c, 0);
+        Single t{y};
+        if (scale.low) e4m3_lift<1>(&t);
+        store_e4m3<1>(a.q + off, &t, scale.k, c, 0);
       } else {
-        store_f(reinterpret_cast<T *>(a.y), off + c, v * rstd * w);
+        store_f(reinterpret_cast<T *>(a.y), off + c, y);
       }
     }
   }
 }
 
 // A matrix's rows in e4m3 with the scale max|row| / 448: a serving program's weights, once, and the
-// activations between two 8-bit products.  A block a row, the second sweep from L1 or L2.
+// activations between two 8-bit products.  A block a row, the second sweep from L1 or L2.  The
+// grid is what runs at once: 16384 x 4096 bf16 46 us, and 62 with a block an SM more than fits.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t *q,
@@ -397,7 +416,7 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t
   const int64_t nvec = dim / VEC;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const T *p = x + row * dim;
-    float m = 0.f, k;
+    float m = 0.f;
     for (int64_t c = threadIdx.x; c < nvec; c += blockDim.x) {
       RowChunk<T, VEC> u;
       Lanes<VEC> l[lanes_of<VEC>()];
@@ -406,31 +425,18 @@ quantize_rows_kernel(const T *__restrict__ x, int64_t rows, int64_t dim, uint8_t
       m = chunk_magnitude<VEC>(m, l);
     }
     m = group_reduce<0, MaxMagnitudeOp>(m, scratch);
-    const float scale = e4m3_scale(m, 1.f, k);
-    if (threadIdx.x == 0) scales[row] = scale;
+    const E4m3Scale scale = e4m3_scale(m);
+    if (threadIdx.x == 0) scales[row] = scale.s;
+    const float lift = scale.low ? kLift : 1.f;
     for (int64_t c = threadIdx.x; c < nvec; c += blockDim.x) {
       RowChunk<T, VEC> u;
       Lanes<VEC> l[lanes_of<VEC>()];
       u.load(p + c * VEC);
       get_lanes(u, l);
-      store_e4m3<VEC>(q + row * dim, l, k, c * VEC, 0);
+      e4m3_lift<VEC>(l, lift);
+      store_e4m3<VEC>(q + row * dim, l, scale.k, c * VEC, 0);
     }
   }
-}
-
-template <typename T>
-int quantize_typed(const T *x, int64_t rows, int64_t dim, uint8_t *q, float *scales,
-                   cudaStream_t s) {
-  constexpr int VEC = vec_of<T>();
-  const bool vec = dim % VEC == 0 && aligned16(x) && aligned16(q);
-  const int64_t nvec = vec ? dim / VEC : dim;
-  const int threads = (int)std::min<int64_t>(256, (nvec + 31) / 32 * 32);
-  const int blocks = (int)std::min<int64_t>(rows, (int64_t)sm_count() * (2048 / threads));
-  if (vec)
-    quantize_rows_kernel<T, VEC><<<blocks, threads, 0, s>>>(x, rows, dim, q, scales);
-  else
-    quantize_rows_kernel<T, 1><<<blocks, threads, 0, s>>>(x, rows, dim, q, scales);
-  return after_launch("quantize_rows_kernel");
 }
 
 struct NormGradArgs {
@@ -745,6 +751,26 @@ int forward_typed(const NormArgs &a, cudaStream_t s) {
   else
     launch_forward<T, 1, FP8, false>(p, a, s);
   return after_launch("norm_forward_kernel");
+}
+
+template <typename T>
+int quantize_typed(const T *x, int64_t rows, int64_t dim, uint8_t *q, float *scales,
+                   cudaStream_t s) {
+  constexpr int VEC = vec_of<T>();
+  const bool vec = dim % VEC == 0 && aligned16(x) && aligned16(q);
+  const int64_t nvec = vec ? dim / VEC : dim;
+  NormPlan p{};
+  p.access = vec ? kChunkRows : kScalarRows;
+  p.threads = (int)std::min<int64_t>(256, (nvec + 31) / 32 * 32);
+  p.groups = rows;
+  p.blocks = (int)std::min<int64_t>(rows, (int64_t)sm_count() * (2048 / p.threads));
+  if (vec)
+    quantize_rows_kernel<T, VEC><<<resident_blocks<quantize_rows_kernel<T, VEC>>(p), p.threads, 0, s>>>(
+        x, rows, dim, q, scales);
+  else
+    quantize_rows_kernel<T, 1><<<resident_blocks<quantize_rows_kernel<T, 1>>(p), p.threads, 0, s>>>(
+        x, rows, dim, q, scales);
+  return after_launch("quantize_rows_kernel");
 }
 
 // The gradient's kernel; returns its blocks.
