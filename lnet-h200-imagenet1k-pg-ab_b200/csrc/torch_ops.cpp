@@ -6,7 +6,9 @@
 // torch.autograd.Function and ctypes a training call of a few rows took 120 us,
 // of which the kernels were 15.  Arguments are checked by the Python callers
 // (lnet_b200.norm, linear, distill); this file has no checks of its own beyond
-// the C ABI's.
+// the C ABI's, but refuses what would pass it by in silence: a forward-mode
+// derivative, which would come out as 0, and a trace, which would record the
+// outputs' allocation and not the launch.
 #define PY_SSIZE_T_CLEAN
 #include <ATen/ATen.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -15,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <optional>
 #include <string>
@@ -83,6 +86,13 @@ bool tracked(std::initializer_list<const Tensor *> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+void refuse(const char *what, std::initializer_list<const Tensor *> ts) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what,
+              " cannot be traced: use the torch.ops.lnet_b200 operator");
+  for (const Tensor *t : ts)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what,
+                " has no forward-mode derivative");
+}
 // A backward pass run with create_graph: its results raise where they are differentiated.
 variable_list once(variable_list grads, const char *what) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -148,6 +158,7 @@ struct NormFunction : torch::autograd::Function<NormFunction> {
     const int64_t need = ctx->saved_data["need"].toInt();
     const auto saved = ctx->get_saved_variables();
     const Tensor &dy = grads[0], dstream = grads[1];
+    refuse("residual_rms_norm's gradient", {&dy, &dstream});
     Tensor dx, dw;
     if (!dy.defined()) {
       dx = dstream;
@@ -253,6 +264,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const int64_t need = ctx->saved_data["need"].toInt(), act = ctx->saved_data["act"].toInt();
     variable_list g(3);
+    refuse("linear_act's gradient", {&grads[0]});
     if (need & 7) {
       const auto saved = ctx->get_saved_variables();
       c10::cuda::CUDAGuard guard(saved[0].device());
@@ -325,6 +337,7 @@ struct DistillFunction : torch::autograd::Function<DistillFunction> {
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &z = saved[0];
+    refuse("distillation_loss's gradient", {&grads[0]});
     c10::cuda::CUDAGuard guard(z.device());
     const Tensor dloss = dense(grads[0].to(at::kFloat));
     Tensor dz;
@@ -416,6 +429,7 @@ PyObject *py_norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   want_args(n, 4);
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]), r = optional_arg(args[2]);
   const double eps = float_arg(args[3]);
+  refuse("residual_rms_norm", {&x, &w, &r});
   Tensor y, stream;
   {
     NoGil gil;
@@ -438,6 +452,7 @@ PyObject *py_norm_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   want_args(n, 4);
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]), r = optional_arg(args[2]);
   const double eps = float_arg(args[3]);
+  refuse("residual_rms_norm", {&x, &w, &r});
   NormOut o;
   {
     NoGil gil;
@@ -454,6 +469,7 @@ PyObject *py_norm_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   want_args(n, 5);
   const Tensor h = tensor_arg(args[0]), rstd = tensor_arg(args[1]), w = tensor_arg(args[2]);
   const Tensor dy = tensor_arg(args[3]), dh = optional_arg(args[4]);
+  refuse("residual_rms_norm", {&h, &rstd, &w, &dy, &dh});
   Tensor dx, dw;
   {
     NoGil gil;
@@ -470,6 +486,7 @@ PyObject *py_norm_fp8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   want_args(n, 4);
   const Tensor x0 = tensor_arg(args[0]), w0 = tensor_arg(args[1]), r0 = optional_arg(args[2]);
   const double eps = float_arg(args[3]);
+  refuse("residual_rms_norm_fp8", {&x0, &w0, &r0});
   Tensor q, s, stream;
   {
     NoGil gil;
@@ -493,6 +510,7 @@ PyObject *py_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want_args(n, 1);
   const Tensor t0 = tensor_arg(args[0]);
+  refuse("quantize_rows_fp8", {&t0});
   Tensor q, s;
   {
     NoGil gil;
@@ -516,6 +534,7 @@ PyObject *py_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]);
   const Tensor b = optional_arg(args[2]), r = optional_arg(args[3]);
   const int64_t act = int_arg(args[4]);
+  refuse("linear_act", {&x, &w, &b, &r});
   Tensor y;
   {
     NoGil gil;
@@ -537,6 +556,7 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]);
   const int64_t act = int_arg(args[2]);
   const Tensor pre = optional_arg(args[3]), dy = tensor_arg(args[4]);
+  refuse("linear_act", {&x, &w, &pre, &dy});
   variable_list g;
   {
     NoGil gil;
@@ -555,6 +575,7 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x = tensor_arg(args[0]), w = tensor_arg(args[1]);
   const Tensor b = optional_arg(args[2]), r = optional_arg(args[3]);
   const int64_t act = int_arg(args[4]);
+  refuse("linear_act", {&x, &w, &b, &r});
   LinearOut out;
   {
     NoGil gil;
@@ -572,6 +593,7 @@ PyObject *py_linear_fp8(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x = tensor_arg(args[0]), xs = tensor_arg(args[1]), w = tensor_arg(args[2]);
   const Tensor ws = tensor_arg(args[3]), b = optional_arg(args[4]), r = optional_arg(args[5]);
   const int64_t act = int_arg(args[6]);
+  refuse("linear_act_fp8", {&x, &xs, &w, &ws, &b, &r});
   Tensor y;
   {
     NoGil gil;
@@ -602,6 +624,7 @@ PyObject *py_distill(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   want_args(n, 7);
   const DistillArgs a(args);
+  refuse("distillation_loss", {&a.z, &a.teacher});
   Tensor loss;
   {
     NoGil gil;
@@ -624,6 +647,7 @@ PyObject *py_distill_backward(PyObject *, PyObject *const *args, Py_ssize_t n) {
   want_args(n, 8);
   const DistillArgs a(args);
   const Tensor dloss = tensor_arg(args[7]);
+  refuse("distillation_loss", {&a.z, &a.teacher, &dloss});
   Tensor dz;
   {
     NoGil gil;

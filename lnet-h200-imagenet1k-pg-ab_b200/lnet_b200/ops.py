@@ -386,8 +386,9 @@ def distillation_loss(logits: Tensor, teacher_indices: Tensor, teacher_logits: T
     _distill._check_distill_args(logits, teacher_indices, teacher_logits, labels, temperature,
                                  alpha, reduction)
     require_cuda("lnet_b200::distillation_loss", logits)
-    return native().distill(logits.detach(), teacher_indices, teacher_logits, labels, temperature,
-                            alpha, _distill.REDUCTIONS[reduction])
+    with torch.no_grad():  # (detach would drop a tangent, which the call refuses)
+        return native().distill(logits, teacher_indices, teacher_logits, labels, temperature, alpha,
+                                _distill.REDUCTIONS[reduction])
 
 
 @distillation_loss.register_fake
