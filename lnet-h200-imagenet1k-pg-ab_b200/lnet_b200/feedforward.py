@@ -34,7 +34,8 @@ class B200FeedForward(nn.Module):
         self.norm_weight = nn.Parameter(torch.ones(model_dim, device=device))
         self.up = nn.Linear(model_dim, hidden_dim, device=device, dtype=torch.bfloat16)
         self.down = nn.Linear(hidden_dim, model_dim, device=device, dtype=torch.bfloat16)
-        self._fp8: tuple[Tensor, ...] | None = None
+        self._fp8: tuple[Tensor, ...] | None = None  # 8-bit weights and their scales
+        self._fp8_of: tuple = ()  # what they were laid out from
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
         if self._fp8 is not None:
@@ -45,24 +46,37 @@ class B200FeedForward(nn.Module):
 
     @torch.no_grad()
     def quantize_(self) -> "B200FeedForward":
-        """Serve in 8 bits from now on (no gradient) with the weights of this moment; ``train()``
-        goes back."""
+        """Serve in 8 bits from now on (no gradient); ``train()`` goes back.  The weights are laid out
+        here, and again at the next call where they have changed since (``load_state_dict``, an
+        update in place that autograd counts; after another kind call ``quantize_`` again)."""
         self.eval()
-        self._fp8 = (*quantize_rows_fp8(self.up.weight), *quantize_rows_fp8(self.down.weight))
+        self._fp8, self._fp8_of = None, ()
+        self._fp8_weights()
         return self
+
+    def _fp8_weights(self) -> tuple[Tensor, ...]:
+        """The 8-bit copies, of the weights as they are: those that are held are kept while storage
+        and version are the same (the storage is held too, so that its address stays its own)."""
+        weights = (self.up.weight, self.down.weight)
+        # inference-mode tensors count no versions
+        key = [(w.data_ptr(), 0 if w.is_inference() else w._version) for w in weights]
+        if self._fp8 is None or key != self._fp8_of[0]:
+            self._fp8 = (*quantize_rows_fp8(weights[0]), *quantize_rows_fp8(weights[1]))
+            self._fp8_of = (key, [w.detach() for w in weights])
+        return self._fp8
 
     def train(self, mode: bool = True) -> "B200FeedForward":
         if mode:
-            self._fp8 = None
+            self._fp8, self._fp8_of = None, ()
         return super().train(mode)
 
     def _apply(self, fn, recurse=True):
-        self._fp8 = None  # the copies would stay on the old device
+        self._fp8, self._fp8_of = None, ()  # the copies would stay on the old device
         return super()._apply(fn, recurse)
 
     @torch.no_grad()
     def _forward_fp8(self, x: Tensor, residual: Tensor | None) -> Tensor:
-        up, up_scale, down, down_scale = self._fp8
+        up, up_scale, down, down_scale = self._fp8_weights()
         y, y_scale, stream = residual_rms_norm_fp8(x, self.norm_weight, residual, self.eps)
         u = linear_act_fp8(y, y_scale, up, up_scale, self.up.bias, activation=self.activation)
         u, u_scale = quantize_rows_fp8(u)
