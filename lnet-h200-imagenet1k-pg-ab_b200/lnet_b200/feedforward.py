@@ -34,11 +34,12 @@ class B200FeedForward(nn.Module):
         self.norm_weight = nn.Parameter(torch.ones(model_dim, device=device))
         self.up = nn.Linear(model_dim, hidden_dim, device=device, dtype=torch.bfloat16)
         self.down = nn.Linear(hidden_dim, model_dim, device=device, dtype=torch.bfloat16)
+        self._serve_fp8 = False
         self._fp8: tuple[Tensor, ...] | None = None  # 8-bit weights and their scales
         self._fp8_of: tuple = ()  # what they were laid out from
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
-        if self._fp8 is not None:
+        if self._serve_fp8:
             return self._forward_fp8(x, residual)
         y, stream = residual_rms_norm(x, self.norm_weight, residual, self.eps)
         u = linear_act(y, self.up.weight, self.up.bias, activation=self.activation)
@@ -47,11 +48,12 @@ class B200FeedForward(nn.Module):
     @torch.no_grad()
     def quantize_(self) -> "B200FeedForward":
         """Serve in 8 bits from now on (no gradient); ``train()`` goes back.  The weights are laid out
-        here, and again at the next call where they have changed since (``load_state_dict``, an
+        here, and again at the next call where they have changed since (``load_state_dict``, ``to``, an
         update in place that autograd counts; after another kind call ``quantize_`` again)."""
         self.eval()
         self._fp8, self._fp8_of = None, ()
         self._fp8_weights()
+        self._serve_fp8 = True
         return self
 
     def _fp8_weights(self) -> tuple[Tensor, ...]:
@@ -67,11 +69,12 @@ class B200FeedForward(nn.Module):
 
     def train(self, mode: bool = True) -> "B200FeedForward":
         if mode:
+            self._serve_fp8 = False
             self._fp8, self._fp8_of = None, ()
         return super().train(mode)
 
     def _apply(self, fn, recurse=True):
-        self._fp8, self._fp8_of = None, ()  # the copies would stay on the old device
+        self._fp8, self._fp8_of = None, ()  # they would stay on the old device: the next call lays out new ones
         return super()._apply(fn, recurse)
 
     @torch.no_grad()

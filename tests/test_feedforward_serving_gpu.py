@@ -57,6 +57,19 @@ def test_weights_are_laid_out_once(cuda_device):
     assert [t.data_ptr() for t in block._fp8] == where
 
 
+def test_moves_and_copies_stay_in_8_bits(cuda_device):
+    x = tokens(cuda_device)
+    block = make(1, cuda_device)
+    plain = block(x).detach()
+    served = block.quantize_()(x)
+    assert not torch.equal(served, plain)
+    assert torch.equal(block.to(cuda_device)(x), served)
+    assert torch.equal(block.cpu().to(cuda_device)(x), served)
+    assert torch.equal(copy.deepcopy(block)(x), served)
+    assert torch.equal(block.eval()(x), served)
+    assert torch.equal(block.train()(x), plain)
+
+
 def test_a_block_made_in_inference_mode(cuda_device):
     with torch.inference_mode():
         block = make(1, cuda_device).quantize_()
