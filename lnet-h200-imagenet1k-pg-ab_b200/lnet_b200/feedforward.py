@@ -10,6 +10,7 @@ from __future__ import annotations
 import torch
 from torch import Tensor, nn
 
+from ._native import refuse_grad
 from .linear import ACTIVATIONS, linear_act, linear_act_fp8, quantize_rows_fp8
 from .norm import RMS_NORM_EPS, residual_rms_norm, residual_rms_norm_fp8
 
@@ -40,6 +41,7 @@ class B200FeedForward(nn.Module):
 
     def forward(self, x: Tensor, residual: Tensor | None = None) -> Tensor:
         if self._serve_fp8:
+            refuse_grad("B200FeedForward in 8 bits", x, residual)
             return self._forward_fp8(x, residual)
         y, stream = residual_rms_norm(x, self.norm_weight, residual, self.eps)
         u = linear_act(y, self.up.weight, self.up.bias, activation=self.activation)

@@ -75,3 +75,14 @@ def test_a_block_made_in_inference_mode(cuda_device):
         block = make(1, cuda_device).quantize_()
         out = block(tokens(cuda_device))
     assert torch.equal(out, make(1, cuda_device).quantize_()(tokens(cuda_device)))
+
+
+def test_inputs_that_want_a_gradient_are_refused(cuda_device):
+    x = tokens(cuda_device)
+    block = make(1, cuda_device).quantize_()
+    want = block(x, x)
+    for args in ((x.clone().requires_grad_(), x), (x, x.clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            block(*args)
+        with torch.no_grad():
+            assert torch.equal(block(*args), want)
