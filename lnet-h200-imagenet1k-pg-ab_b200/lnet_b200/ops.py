@@ -25,7 +25,8 @@ known output shape.  This module gives the B200 path the same surface:
   :mod:`lnet_b200.norm`, :mod:`lnet_b200.linear` and :mod:`lnet_b200.distill`, the
   first three with their gradients.  An op returns no input: without a residual
   the norm's stream is an empty tensor (it is ``x``), and without an activation
-  the linear's pre-activation is.
+  the linear's pre-activation is.  ``rstd`` and the pre-activation are there for
+  the gradient and have none of their own.
 
 ``lnet_b200::alphabet_forward`` also carries ``register_autograd`` (the
 reference's ops register their VJPs the same way,
@@ -250,7 +251,8 @@ def _none(t: Tensor) -> Tensor:
 @torch.library.custom_op("lnet_b200::residual_rms_norm", mutates_args=())
 def residual_rms_norm(x: Tensor, weight: Tensor, residual: Optional[Tensor] = None,
                       eps: float = _norm.RMS_NORM_EPS) -> tuple[Tensor, Tensor, Tensor]:
-    """``(y, stream, rstd)`` of :func:`lnet_b200.residual_rms_norm` (``rstd`` [...] fp32)."""
+    """``(y, stream, rstd)`` of :func:`lnet_b200.residual_rms_norm` (``rstd`` [...] fp32, without a
+    gradient of its own)."""
     _norm._check_norm_args(x, weight, residual, eps)
     require_cuda("lnet_b200::residual_rms_norm", x)
     y, stream, rstd = native().norm_forward(x, weight, residual, eps)
@@ -280,6 +282,7 @@ def _residual_rms_norm_context(ctx, inputs, output):
     x, weight, residual, _ = inputs
     _, stream, rstd = output
     ctx.residual = residual is not None
+    ctx.mark_non_differentiable(*([rstd] if ctx.residual else [stream, rstd]))
     ctx.save_for_backward(stream if ctx.residual else x, rstd, weight)
 
 
@@ -316,7 +319,8 @@ def _residual_rms_norm_fp8_fake(x, weight, residual=None, eps=_norm.RMS_NORM_EPS
 def linear_act(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None,
                residual: Optional[Tensor] = None,
                activation: str = "none") -> tuple[Tensor, Tensor]:
-    """``(y, pre-activation)`` of :func:`lnet_b200.linear_act`."""
+    """``(y, pre-activation)`` of :func:`lnet_b200.linear_act`; the second has no gradient of its
+    own."""
     _linear._check_linear_args(x, weight, bias, residual, activation, torch.bfloat16)
     require_cuda("lnet_b200::linear_act", x)
     y, pre = native().linear_forward(x, weight, bias, residual, _linear.ACTIVATIONS[activation])
@@ -347,6 +351,7 @@ def _linear_act_backward_fake(x, weight, activation, preact, dy):
 def _linear_act_context(ctx, inputs, output):
     x, weight, bias, residual, ctx.activation = inputs
     ctx.has = (bias is not None, residual is not None)
+    ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(x, weight, output[1])
 
 
