@@ -318,7 +318,7 @@ def load(auto_build: bool = True) -> ctypes.CDLL:
         path = Path(override) if override else _build.LIB
         if not override and auto_build and _build.needs_build():
             try:
-                _build.build()
+                _build.build_library()
             except RuntimeError:
                 if not path.exists():
                     raise

@@ -1,6 +1,7 @@
 """The host path of the feed-forward and distillation operators (``csrc/torch_ops.cpp``): a CPython
 module over the C ABI that allocates outputs, launches on torch's current stream and records
-gradients.  Built in-tree by :mod:`lnet_b200.build` and loaded on first use; there is no fallback.
+gradients.  Built in-tree by :mod:`lnet_b200.build` and loaded on first use; there is no fallback, and a
+module of other sources is not loaded.
 """
 
 from __future__ import annotations
@@ -33,13 +34,7 @@ def _load():
         if _module is not None:
             return _module
         lib = _lib.load()
-        path = _build.TORCH_OPS
-        if _build.torch_ops_stale():
-            try:
-                _build.build_torch_ops()
-            except (OSError, RuntimeError):
-                if not path.exists():
-                    raise
+        path = _build.build_torch_ops()
         loader = importlib.machinery.ExtensionFileLoader("_torch_ops", str(path))
         spec = importlib.util.spec_from_file_location("_torch_ops", str(path), loader=loader)
         module = importlib.util.module_from_spec(spec)

@@ -4,12 +4,15 @@
 ``lnet_b200/_lib/liblnet_b200.so`` (a C-ABI shared library loaded with
 ctypes), and ``csrc/torch_ops.cpp`` (the host path of the feed-forward and
 distillation operators) with g++ against torch's headers into
-``lnet_b200/_lib/_torch_ops.so``.  Rebuilds only what a source or header is
-newer than.
+``lnet_b200/_lib/_torch_ops.so``.  Rebuilds the library where a source or header
+is newer, and the module where its sources, torch or Python are others than the
+ones it was built from (``_torch_ops.stamp``): it shares structures with the
+library and with torch, and another's must not be loaded.
 """
 
 from __future__ import annotations
 
+import hashlib
 import os
 import shutil
 import subprocess
@@ -50,11 +53,24 @@ def needs_build() -> bool:
     return any(p.stat().st_mtime > mtime for p in _deps())
 
 
+def _torch_ops_stamp() -> str:
+    """What the module is built from: its sources' text, torch and Python."""
+    import torch
+
+    h = hashlib.sha256(f"{torch.__version__} {sysconfig.get_config_var('SOABI')}".encode())
+    for p in (TORCH_OPS_SOURCE, *sorted(INCLUDE.glob("*.h"))):
+        h.update(p.read_bytes())
+    return h.hexdigest()
+
+
+def _stamp_path() -> Path:
+    return TORCH_OPS.with_suffix(".stamp")
+
+
 def torch_ops_stale() -> bool:
-    if not TORCH_OPS.exists():
+    if not TORCH_OPS.exists() or not _stamp_path().exists():
         return True
-    mtime = TORCH_OPS.stat().st_mtime
-    return any(p.stat().st_mtime > mtime for p in (TORCH_OPS_SOURCE, *INCLUDE.glob("*.h")))
+    return _stamp_path().read_text() != _torch_ops_stamp()
 
 
 def _torch_ops_command(out: Path) -> list[str]:
@@ -75,18 +91,27 @@ def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
         return TORCH_OPS
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = TORCH_OPS.with_suffix(f".so.{os.getpid()}.tmp")
+    stamp = _torch_ops_stamp()
     cmd = _torch_ops_command(tmp)
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed: {' '.join(cmd)}\n{res.stdout}{res.stderr}")
+    _stamp_path().unlink(missing_ok=True)  # between the two the module counts as stale
     os.replace(tmp, TORCH_OPS)
+    _stamp_path().write_text(stamp)
     return TORCH_OPS
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
+    """The library, which needs no torch, then the module."""
+    build_library(force, verbose)
     build_torch_ops(force, verbose)
+    return LIB
+
+
+def build_library(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
     LIB_DIR.mkdir(parents=True, exist_ok=True)
