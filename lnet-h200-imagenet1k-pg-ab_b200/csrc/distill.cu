@@ -38,6 +38,8 @@ namespace {
 constexpr float kLowest = -3.402823466e+38f;
 constexpr int kCountThreads = 256;
 constexpr int kSumThreads = 1024;
+constexpr int kEntries = 256;  // most entries of a row that are corrected one by one
+constexpr int kWindow = 4096;  // classes whose masses a block holds at once
 
 struct DistillArgs {
   const void *z;
@@ -118,7 +120,11 @@ __device__ __forceinline__ void stats_add(RowStats &a, const float *v, float kt)
 // entries fetched while the row is read and sums joined by warps (10.2 with the entries after the
 // row's sums and one barrier a quantity); the chain of load, join over the block, join over the
 // cluster bounds it.
-template <typename T, bool TWO>
+// MANY: a gradient with more than kEntries entries, which are added up class by class; fewer are corrected
+// one by one, each with a look at all of them.  296 rows of 70001 bf16 classes with 64, 256, 512, 1024
+// and 4096 entries: 62, 71, 85, 117, 279 us by classes, 38, 51, 103, 298, 4067 one by one; 296 x 32768
+// with 16384 415 us and 87 ms.
+template <typename T, bool TWO, bool MANY>
 __global__ void distill_row_kernel(const DistillArgs a) {
   constexpr int VEC = vec_of<T>();
   constexpr int U = 4;  // chunks in flight a thread
@@ -334,6 +340,38 @@ __global__ void distill_row_kernel(const DistillArgs a) {
   for (int64_t i = vb + tid; i < hi; i += nt) store_f(dz, i, grad(load_f(z, i)));
   if (bad) return leave();
   __syncthreads();  // the dense part is written
+  if constexpr (MANY) {
+    // The block's classes, a window at a time: the entries' masses are added up in shared memory, in
+    // units of 2^-62, as integers (any order gives the same sum; what a p below 2^-38 loses is less
+    // than 2^-63), and a class that has some is written anew.  top classes / kWindow looks at an entry.
+    extern __shared__ unsigned long long mass[];
+    const bool whole = tsum == tsum;  // a NaN among the teacher's logits makes its row's entries NaN
+    for (int c = tid; c < kWindow; c += nt) mass[c] = 0;
+    for (int64_t w0 = lo; w0 < hi; w0 += kWindow) {
+      const int64_t n = std::min<int64_t>(kWindow, hi - w0);
+      __syncthreads();
+      if (has_t)
+        for (int64_t j = tid; j < a.top; j += nt) {
+          const int64_t at_window = index[j] - w0;
+          if (at_window < 0 || at_window >= n) continue;
+          const float t = teacher[j];
+          if (t == -INFINITY) continue;
+          const float p = exp2f((t - tmax) * kt) / tsum;
+          atomicAdd(mass + at_window, whole ? __float2ull_rn(p * 0x1p62f) : 1ull);
+        }
+      __syncthreads();
+      for (int c = tid; c < n; c += nt) {
+        const bool own_label = has_l && w0 + c == label;
+        const unsigned long long sum = mass[c];
+        if (sum == 0 && !own_label) continue;
+        mass[c] = 0;
+        float g = grad(load_f(z, w0 + c)) - ct * (whole || sum == 0 ? __ull2float_rn(sum) * 0x1p-62f : NAN);
+        if (own_label) g -= c1s;
+        store_f(dz, w0 + c, g);
+      }
+    }
+    return leave();
+  }
   // An entry named twice gets both masses: each of its threads adds them in the same order
   // and writes the same value.
   auto corrected = [&](int64_t ix) {
@@ -356,7 +394,6 @@ __global__ void distill_row_kernel(const DistillArgs a) {
 // ---------------------------------------------------------------- loss and gradient, row on chip
 // First, a warp a row, the teacher's side: the softmax p of the entries, an index named twice
 // merged into its first place, the sums that the loss needs, and how many rows count.
-constexpr int kEntries = 256;          // most entries of a row here; more take the other kernel
 constexpr int kPrepareThreads = 256;
 constexpr int kHasTeacher = 1, kHasLabel = 2, kBad = 4;
 
@@ -1118,9 +1155,11 @@ int launch_rows(const lnet_b200_distill_request *q, const DistillArgs &a, cudaSt
   cfg.numAttrs = 1;
   cfg.gridDim = dim3((unsigned)(q->rows * parts));
   cfg.blockDim = dim3(threads);
-  const cudaError_t err = two_temperatures(a)
-                              ? cudaLaunchKernelEx(&cfg, distill_row_kernel<T, true>, a)
-                              : cudaLaunchKernelEx(&cfg, distill_row_kernel<T, false>, a);
+  const bool many = a.dz && a.top > kEntries, two = two_temperatures(a);
+  if (many) cfg.dynamicSmemBytes = kWindow * sizeof(unsigned long long);
+  const auto kernel = many ? (two ? distill_row_kernel<T, true, true> : distill_row_kernel<T, false, true>)
+                           : (two ? distill_row_kernel<T, true, false> : distill_row_kernel<T, false, false>);
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, a);
   LNET_TRY(cuda_check(err, "distill_row_kernel"));
   return after_launch("distill_row_kernel");
 }
