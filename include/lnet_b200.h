@@ -455,7 +455,8 @@ int lnet_b200_residual_rms_norm(const void *x, const void *residual, const void 
                                 lnet_stream_t stream);
 
 /* The same norm with an 8-bit output: scales[row] = max|y| / 448 (fp32) and
- * values = e4m3(y / scale), rounded to nearest even; a zero row has scale 0 and values 0. */
+ * values = e4m3(y / scale), rounded to nearest even and saturating; a row whose scale is 0 (zeros, or
+ * all below 448 * 2^-150) has values 0. */
 int lnet_b200_residual_rms_norm_fp8(const void *x, const void *residual, const void *weight,
                                     int32_t dtype, int32_t weight_dtype, int64_t rows,
                                     int64_t dim, float eps, uint8_t *values, float *scales,

@@ -12,7 +12,8 @@
 //
 // Two kernels.  With a gradient, and rows that 8 blocks hold, the row stays on
 // chip (distill_resident_kernel below).  The loss alone, longer rows, and a
-// gradient whose alignment differs from z's take distill_row_kernel: one sweep
+// gradient whose alignment differs from z's or that has more than 256 entries a row
+// take distill_row_kernel: one sweep
 // reads the row for its running maximum and exponential sums (one sum for each
 // of the temperatures tau and 1 that the loss needs), a second one writes the
 // gradient from the row in L2 or L1.  In both the few entries of the teacher and
@@ -528,7 +529,8 @@ distill_prepare_kernel(const DistillArgs a, Entry *entries, RowInfo *info, int *
 // 2000 x 131000 take 344 us there and took 485 here with 512 threads of 4 chunks.
 // Rows that start inside 16 bytes, with the launches around the kernel: 2000 x 40001 137 us (the other
 // kernel 148), 2000 x 4097 53 (61), 2000 x 1001 43 (53); 5 to 9 % slower where the last block has
-// little to hold (2000 x 32767 136 against 126, 2000 x 50257 186 against 170).
+// little to hold (2000 x 32767 136 against 126, 2000 x 50257 186 against 170), which the choice between the
+// two does not look at: wherever 8 blocks hold a row it takes this one.
 constexpr int kResidentThreads = 128;
 constexpr int kResidentParts = 8;
 

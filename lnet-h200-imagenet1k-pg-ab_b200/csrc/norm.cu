@@ -16,8 +16,8 @@
 // kernels).  Rows of other lengths than a multiple of 16 bytes keep the 16-byte
 // loads, shifted to the boundaries (SHIFT).
 //
-// Measured, of the 6448 GB/s of a copy: 16384 x 4096 bf16 + residual to e4m3 77
-// us (0.95); 802816 x 96 bf16 with gradient 101 + 102 us for 616 MB each (0.94)
+// Measured, of the 6448 GB/s of a copy: 16384 x 4096 bf16 + residual to e4m3 76
+// us on the same inputs again and 82 on others in turn (0.96, 0.89); 802816 x 96 bf16 with gradient 101 + 102 us for 616 MB each (0.94)
 // and 6 us of column sums.
 #include <cuda_fp8.h>
 
@@ -247,7 +247,7 @@ __device__ __forceinline__ void weight_part(const void *w, bool w_bf16, int c, i
 
 // G lanes a row (0: the block).  8 bits at 16384 x 4096 is near two bounds, HBM and 2.1 instructions a
 // clock: a block of 128 threads a row took 95 us where a warp of 16 chunks a lane took 114, and with
-// the arithmetic in packed pairs it takes 77.
+// the arithmetic in packed pairs it takes 80 (82 since its largest value waits for rstd: of y, not of h w).
 template <typename T, int VEC, int G, bool FP8, bool SHIFT>
 __global__ void __launch_bounds__(G ? kSubThreads : kBlockThreads)
 norm_forward_kernel(const NormArgs a) {

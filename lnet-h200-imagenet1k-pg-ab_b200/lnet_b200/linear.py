@@ -60,7 +60,10 @@ def linear_act(x: Tensor, weight: Tensor, bias: Tensor | None = None,
 
     ``activation`` is ``"none"``, ``"relu"``, ``"silu"`` or ``"gelu"`` (the erf form).  Sums are
     fp32 and the result is rounded once to bfloat16.  Differentiable in ``x``, ``weight``, ``bias``
-    and ``residual``; through an activation the forward pass keeps x W^T + bias in bfloat16.
+    and ``residual``.  Through an activation the forward pass keeps a = x W^T + bias in bfloat16, the
+    gradient takes f'(a) from it, and da = dy f'(a) is rounded to bfloat16 as an operand of the products
+    for ``x`` and ``weight`` (with GELU their gradients are 2.4e-3 of themselves off, 1.7e-3 is the
+    rounding of the result alone); ``bias`` sums the unrounded da.
     """
     _check_linear_args(x, weight, bias, residual, activation, torch.bfloat16)
     require_cuda("linear_act", x)

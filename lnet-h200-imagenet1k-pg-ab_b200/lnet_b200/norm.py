@@ -59,8 +59,9 @@ def residual_rms_norm_fp8(x: Tensor, weight: Tensor, residual: Tensor | None = N
     :func:`lnet_b200.linear_act_fp8`.
 
     ``scales`` [...] = max|y| / 448 a row (fp32) and ``values`` [..., D] (``float8_e4m3fn``)
-    = y / scale rounded to nearest even; a zero row has scale 0 and values 0.  A serving form:
-    it has no gradient and refuses inputs that want one.
+    = y / scale rounded to nearest even; a zero row has scale 0 and values 0.  The quotient has two
+    fp32 roundings, so that a value within 2^-22 of a tie may take the neighbouring code.  A serving
+    form: it has no gradient and refuses inputs that want one.
     """
     _check_norm_args(x, weight, residual, eps)
     require_cuda("residual_rms_norm_fp8", x)
