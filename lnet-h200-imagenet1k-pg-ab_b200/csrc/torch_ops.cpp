@@ -73,7 +73,15 @@ int dtype_of(const Tensor &t) {
 lnet_stream_t stream_of(const Tensor &t) {
   return c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
 }
-void *ptr(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+// Null where there is no tensor, and only there: a wrapper without memory of its own (fake, functional,
+// distributed) would read as an argument that was left out.
+void *ptr(const Tensor &t) {
+  if (!t.defined()) return nullptr;
+  void *p = t.data_ptr();
+  TORCH_CHECK(p || t.numel() == 0, "a tensor without memory of its own (a fake, functional or "
+                                   "distributed wrapper) cannot be used here");
+  return p;
+}
 Tensor dense(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
 Tensor dense(const OptTensor &t) { return t.has_value() ? dense(*t) : Tensor(); }
 Tensor workspace(size_t bytes, const Tensor &like) {
