@@ -7,8 +7,9 @@
 //   dz = alpha tau (q - p) [entries] + (1 - alpha) (softmax(z) - onehot) [label >= 0].
 // A part with weight 0 is left out.  A class at -inf has q = 0 (the loss is +inf
 // where the teacher gives it mass); a row that is -inf throughout has q = 0
-// everywhere.  An index or label past the classes makes the row's loss NaN and
-// touches nothing else.
+// everywhere.  A row with neither entries nor a label has loss and gradient 0
+// whatever its logits are.  An index or label past the classes makes the row's
+// loss NaN and touches nothing else.
 //
 // Two kernels.  With a gradient, and rows that 8 blocks hold, the row stays on
 // chip (distill_resident_kernel below).  The loss alone, longer rows, and a
@@ -293,6 +294,7 @@ __global__ void distill_row_kernel(const DistillArgs a) {
   if (bad) scale = NAN;
   const float ct = has_t ? a.alpha * a.tau * scale : 0.f;
   const float c1s = has_l ? (1.f - a.alpha) * scale : 0.f;
+  const bool idle = !has_t && !has_l;  // no target: the gradient is 0 whatever the logits are
   float at = ct * inv_t, a1 = c1s * inv_1;
   if (!TWO) {
     at += a1;
@@ -302,7 +304,7 @@ __global__ void distill_row_kernel(const DistillArgs a) {
   auto grad = [&](float v) {
     float g = at * exp2_fast((v - m) * kt);
     if (TWO) g = fmaf(a1, exp2_fast((v - m) * kLog2e), g);
-    return g;
+    return idle ? 0.f : g;
   };
   const bool same_alignment =
       ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(dz)) & 15) == 0;
@@ -885,10 +887,13 @@ distill_resident_kernel(const ResidentArgs ra) {
         }
       }
     };
-    if (whole)
+    if (info.flags == 0 && !bad) {  // no target: 0 whatever the logits are
+      for (int64_t i = max(lo, 0) + tid; i < min(hi, classes); i += nt) store_f(dz, i, 0.f);
+    } else if (whole) {
       store_row(true);
-    else
+    } else {
       store_row(false);
+    }
     int j = head[set][tid];
     if (j >= 0) {
       head[set][tid] = -1;

@@ -74,7 +74,8 @@ def distillation_loss(logits: Tensor, teacher_indices: Tensor, teacher_logits: T
 
     The work grows with V and, for a gradient, with K V / 4096 where K is above 256 (K^2 below).
 
-    Classes masked to -inf have no mass; where the teacher gives one mass, the loss is +inf.  An
+    Classes masked to -inf have no mass; where the teacher gives one mass, the loss is +inf.  A row
+    without an entry or a label has loss and gradient 0, whatever its logits are (NaN, infinities).  An
     index or label past V makes its row's loss and gradient NaN.
     """
     _check_distill_args(logits, teacher_indices, teacher_logits, labels, temperature, alpha,
